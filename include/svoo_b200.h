@@ -7,9 +7,10 @@
  *   - Every pointer is a DEVICE pointer unless its name ends in `_host`.
  *   - Token tensors are bf16, row-major [BH, N, 128] (BH = batch*heads flattened,
  *     head dim D must be 128).  Labels, indices, sizes, offsets are int32.
- *     bf16 is the only element type: there is no dtype argument, and a caller that
- *     holds fp16 or fp32 activations casts them before the call (the Python front end
- *     does that and casts results back).  BH * N must be below 2^31.
+ *     bf16 is the only element type of the attention path: there is no dtype argument, and
+ *     a caller that holds fp16 or fp32 activations casts them before the call (the Python
+ *     front end does that and casts results back).  BH * N must be below 2^31.  The
+ *     token-wise operators (layer norm, linear layers; end of this file) take a SVOO_TYPE_*.
  *   - The library allocates nothing: outputs and the workspace are caller-owned.
  *     `stream` is a cudaStream_t passed as void*; all work is enqueued on it and
  *     no entry point synchronises with the host.
@@ -38,8 +39,14 @@ enum {
   SVOO_ERR_WORKSPACE = -4,   /* workspace too small (see *_workspace_bytes)      */
   SVOO_ERR_ALIGN = -5,       /* a tensor pointer is not 16-byte aligned          */
   SVOO_ERR_CLUSTERS = -6,    /* cluster count above SVOO_MAX_CLUSTERS            */
-  SVOO_ERR_STATIC_SCRATCH = -7 /* BH * ceil(N / 2048) * K above the limit of svoo_b200_sort_labels_static */
+  SVOO_ERR_STATIC_SCRATCH = -7, /* BH * ceil(N / 2048) * K above the limit of svoo_b200_sort_labels_static */
+  SVOO_ERR_TYPE = -8         /* an element type or activation that the call does not take */
 };
+
+/* Element types of the token-wise operators. */
+enum { SVOO_TYPE_BF16 = 0, SVOO_TYPE_FP16 = 1, SVOO_TYPE_FP32 = 2, SVOO_TYPE_E4M3 = 3 };
+/* Activations of svoo_b200_mm_fp8: none, GELU with its tanh formula. */
+enum { SVOO_ACT_NONE = 0, SVOO_ACT_GELU_TANH = 1 };
 
 #define SVOO_MAX_CLUSTERS 1024   /* per side; the reference ships QC=256, KC=1024 */
 /* Blocks per side that the attention-side entry points accept (svoo_b200_sparse_attn*,
@@ -376,6 +383,64 @@ int svoo_b200_qk_prep_push(const void* x, const float* weight, float eps, const 
  * its own GPU.  No counterpart in the reference (one GPU). */
 int svoo_b200_peer_barrier(void* const* peer_flags, int32_t world, int32_t rank, int32_t channel, uint32_t epoch,
                            int32_t* status, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Token-wise operators: the layer norms and linear layers of a transformer block.  Sizes may be odd and
+ * tensors of zero rows are accepted (nothing is launched, or sums are zero).  Strides and pitches are in
+ * elements.  No counterpart in the reference except where named.
+ * ------------------------------------------------------------------------------------------ */
+
+#define SVOO_MAX_NORM_COLUMNS 16384
+
+/* y = (x - mean) rstd g + o over the last dimension, rstd = 1 / sqrt(var + eps), var around the mean / C; statistics in
+ * 32 bits.  x: [batch, rows, C] of x_type, last dimension dense, rows x_row and samples x_batch apart; y: dense, x_type.
+ * gain, offset: C values of param_type (SVOO_TYPE_FP32 or x_type) per sample, gain_batch / offset_batch apart (0: one row for
+ * all); null: 1 and 0.  gain_plus_one: g = 1 + gain (AdaLN).  mean, rstd: fp32 [batch * rows], both or none.  C <= 16384.
+ * (fp32 layer norm and modulation of the block, svoo/models/wan/custom_models.py:22-108) */
+int svoo_b200_layer_norm(const void* x, int32_t x_type, int64_t batch, int64_t rows, int64_t C, int64_t x_batch, int64_t x_row,
+                         const void* gain, int64_t gain_batch, const void* offset, int64_t offset_batch, int32_t param_type,
+                         int32_t gain_plus_one, float eps, void* y, float* mean, float* rstd, void* stream);
+/* Its gradient: dx (dense, x_type) from dy [batch, rows, C] (x_type, last dimension dense), x and the statistics of the
+ * forward call.  dgain, doffset (param_type; both or none): sums over the rows of each sample, [batch, C], where
+ * per_sample != 0, otherwise over all rows, [C].  The sums run in a fixed order.  workspace: layer_norm_workspace_bytes,
+ * needed with dgain. */
+int svoo_b200_layer_norm_workspace_bytes(int64_t batch, int64_t rows, int64_t C, int32_t per_sample, int64_t* bytes_out);
+int svoo_b200_layer_norm_backward(const void* dy, int64_t dy_batch, int64_t dy_row, const void* x, int32_t x_type, int64_t batch,
+                                  int64_t rows, int64_t C, int64_t x_batch, int64_t x_row, const float* mean, const float* rstd,
+                                  const void* gain, int64_t gain_batch, int32_t param_type, int32_t gain_plus_one,
+                                  int32_t per_sample, void* dx, void* dgain, void* doffset, void* workspace,
+                                  int64_t workspace_bytes, void* stream);
+
+/* Quantisation to e4m3, one fp32 scale per block of 128: scale = max(amax / 448, 2^-126), q = e4m3(x / scale) to nearest even.
+ * A block with a value that is not finite stands for NaN.  x [M, K] of x_type (bf16, fp16, fp32), rows x_row apart.  Pitches of q are
+ * multiples of 16 >= the row's length; what lies behind a row, up to the next multiple of 16, is written as zero.
+ *   rows:    blocks along K.  q [M, q_pitch], scale[kb * scale_pitch + m], kb < ceil(K / 128), scale_pitch >= M
+ *   columns: blocks along M of the transpose.  q [K, q_pitch >= M], scale[mb * scale_pitch + k]; column_sums, if given, receives
+ *            fp32 [ceil(M / 128), K] sums of each 128 rows, which svoo_b200_column_sum adds
+ *   blocks:  squares of 128 x 128.  q [M, q_pitch], scale [ceil(M / 128), ceil(K / 128)]; qt, if given, is the transpose of q,
+ *            [K, qt_pitch >= M] */
+int svoo_b200_quantize_rows(const void* x, int32_t x_type, int64_t M, int64_t K, int64_t x_row, void* q, int64_t q_pitch, float* scale,
+                            int64_t scale_pitch, void* stream);
+int svoo_b200_quantize_columns(const void* x, int32_t x_type, int64_t M, int64_t K, int64_t x_row, void* q, int64_t q_pitch,
+                               float* scale, int64_t scale_pitch, float* column_sums, void* stream);
+int svoo_b200_quantize_blocks(const void* x, int32_t x_type, int64_t M, int64_t K, int64_t x_row, void* q, int64_t q_pitch, void* qt,
+                              int64_t qt_pitch, float* scale, void* stream);
+/* out[c] = sum over parts of partial[part][c] (fp32 [parts, C]), out of out_type. */
+int svoo_b200_column_sum(const float* partial, int64_t parts, int64_t C, void* out, int32_t out_type, void* stream);
+
+/* out[m, n] = act(sum_k a^[m, k] b^[n, k] + bias[n]) of operands in e4m3 as the quantisers leave them, sums in 32 bits.
+ * a [M, K], a_scale as of quantize_rows.  b [N, K] with b_scale[(n / 128) * b_scale_n + (k / 128) * b_scale_k] (as of
+ * quantize_blocks; swap the two for its transpose), or, with b_scale_rows != 0, b_scale[(k / 128) * b_scale_k + n] (as of
+ * quantize_rows or quantize_columns; b_scale 16-byte aligned, b_scale_k a multiple of 4; no activation, no e4m3 output).
+ * out [M, N] of out_type, rows out_pitch apart; SVOO_TYPE_E4M3: the 32-bit results quantised in blocks along N, out_pitch a
+ * multiple of 16, out_scale[nb * out_scale_pitch + m].  a and b 16-byte aligned, their pitches multiples of 16. */
+int svoo_b200_mm_fp8(const void* a, int64_t a_pitch, const float* a_scale, int64_t a_scale_pitch, const void* b, int64_t b_pitch,
+                     const float* b_scale, int64_t b_scale_n, int64_t b_scale_k, int32_t b_scale_rows, const void* bias,
+                     int32_t bias_type, int64_t M, int64_t N, int64_t K, int32_t activation, void* out, int32_t out_type,
+                     int64_t out_pitch, float* out_scale, int64_t out_scale_pitch, void* stream);
+/* Copies the product's status word of the current device to *status (device int32): 0, or 1 after a kernel gave up on a
+ * bounded wait and left rows unwritten. */
+int svoo_b200_linear_status(int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

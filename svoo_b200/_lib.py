@@ -80,6 +80,23 @@ SIGNATURES = {
     "svoo_b200_peer_barrier": (c_int, [c_void_p, c_int32, c_int32, c_int32, ctypes.c_uint32, c_void_p, c_void_p]),
     "svoo_b200_push_heads": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int64, c_int64, c_int64,
                                      c_void_p]),
+    "svoo_b200_layer_norm": (c_int, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p,
+                                     c_int64, c_int32, c_int32, c_float, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "svoo_b200_layer_norm_workspace_bytes": (c_int, [c_int64, c_int64, c_int64, c_int32, _I64P]),
+    "svoo_b200_layer_norm_backward": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64,
+                                              c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32, c_void_p,
+                                              c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "svoo_b200_quantize_rows": (c_int, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                                        c_void_p]),
+    "svoo_b200_quantize_columns": (c_int, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                                           c_void_p, c_void_p]),
+    "svoo_b200_quantize_blocks": (c_int, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                                          c_void_p, c_void_p]),
+    "svoo_b200_column_sum": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int32, c_void_p]),
+    "svoo_b200_mm_fp8": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int32,
+                                 c_void_p, c_int32, c_int64, c_int64, c_int64, c_int32, c_void_p, c_int32, c_int64, c_void_p,
+                                 c_int64, c_void_p]),
+    "svoo_b200_linear_status": (c_int, [c_void_p, c_void_p]),
     "svoo_b200_push_seq": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int64, c_int64, c_int64, c_void_p]),
 }
 

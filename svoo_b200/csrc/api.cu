@@ -98,6 +98,7 @@ const char* svoo_b200_error_string(int code) {
     case SVOO_ERR_ALIGN: return "tensor pointer is not 16-byte aligned";
     case SVOO_ERR_CLUSTERS: return "cluster count above 1024 (1026 blocks for the attention)";
     case SVOO_ERR_STATIC_SCRATCH: return "problem too large for the built-in scratch array (BH*ceil(N/2048)*K > 1048576)";
+    case SVOO_ERR_TYPE: return "an element type or activation that the call does not take";
     default: return code > 0 ? cudaGetErrorString((cudaError_t)code) : "unknown svoo_b200 error";
   }
 }

@@ -1,0 +1,160 @@
+// extern "C" entry points of the token-wise operators: argument checks and launches.
+#include "rows_common.cuh"
+
+namespace svoo {
+int norm_backward_parts(int64_t rows, int groups, int C);
+cudaError_t launch_layer_norm(int type, const NormArgs& a, cudaStream_t st);
+cudaError_t launch_layer_norm_backward(int type, const NormArgs& a, int groups, int parts, void* dgain, void* doffset, cudaStream_t st);
+cudaError_t launch_column_sum(const float* partial, int64_t parts, int64_t C, void* out, int out_type, cudaStream_t st);
+cudaError_t launch_quantize_rows(int type, const void* x, int64_t M, int64_t K, int64_t row_stride, void* q, int64_t q_pitch, float* scale,
+                                 int64_t scale_pitch, cudaStream_t st);
+cudaError_t launch_quantize_columns(int type, const void* x, int64_t M, int64_t K, int64_t row_stride, void* qt, int64_t qt_pitch,
+                                    float* scale, int64_t scale_pitch, float* column_sum, cudaStream_t st);
+cudaError_t launch_quantize_blocks(int type, const void* w, int64_t N, int64_t K, int64_t row_stride, void* q, int64_t q_pitch, void* qt,
+                                   int64_t qt_pitch, float* scale, cudaStream_t st);
+cudaError_t launch_linear_tc(const void* a, int64_t a_pitch, const float* sa, int64_t sa_pitch, const void* b, int64_t b_pitch, const float* sb,
+                             int64_t sb_n, int64_t sb_k, bool row_scales, const void* bias, int bias_type, int64_t M, int64_t N, int64_t K,
+                             bool gelu, int out_type, void* out, int64_t out_pitch, float* out_scale, int64_t out_scale_pitch, cudaStream_t st);
+cudaError_t read_linear_status(int32_t* out, cudaStream_t st);
+}  // namespace svoo
+
+using namespace svoo;
+
+namespace {
+constexpr int64_t kMaxRows = 1 << 26;            // rows and columns of a matrix: tile coordinates are 32-bit ints
+bool aligned(const void* p, int to) { return (uintptr_t)p % to == 0; }
+bool element(int type) { return type == SVOO_TYPE_BF16 || type == SVOO_TYPE_FP16 || type == SVOO_TYPE_FP32; }
+
+int check_norm(int32_t x_type, int64_t batch, int64_t rows, int64_t C, int64_t x_batch, int64_t x_row, int32_t param_type, bool per_sample) {
+  if (!element(x_type) || (param_type != SVOO_TYPE_FP32 && param_type != x_type)) return SVOO_ERR_TYPE;
+  if (batch < 0 || rows < 0 || C < 1 || C > SVOO_MAX_NORM_COLUMNS || x_batch < 0 || x_row < 0) return SVOO_ERR_SHAPE;
+  if (rows > kMaxRows || batch > kMaxRows || batch * rows > (int64_t)INT32_MAX || (per_sample && batch > 65535)) return SVOO_ERR_SHAPE;
+  return SVOO_OK;
+}
+int check_quant(const void* x, int32_t type, int64_t M, int64_t K, int64_t x_row, const void* q, int64_t q_pitch, int64_t q_cols, const float* scale) {
+  if (!element(type)) return SVOO_ERR_TYPE;
+  if (M < 0 || K < 1 || M > kMaxRows || K > kMaxRows || x_row < 0 || q_pitch < q_cols || q_pitch % 16) return SVOO_ERR_SHAPE;
+  if (M * ceil_div64(K, 128) > (int64_t)INT32_MAX - 16) return SVOO_ERR_SHAPE;
+  if (M == 0) return SVOO_OK;
+  if (!x || !q || !scale) return SVOO_ERR_NULL;
+  if (!aligned(q, 16) || !aligned(x, elem_bytes(type)) || !aligned(scale, 4)) return SVOO_ERR_ALIGN;
+  return SVOO_OK;
+}
+int64_t norm_groups(int64_t batch, int32_t per_sample) { return per_sample && batch > 1 ? batch : 1; }
+#define SVOO_TRY(expr) do { int _rc = (expr); if (_rc != SVOO_OK) return _rc; } while (0)
+}  // namespace
+
+extern "C" {
+
+int svoo_b200_layer_norm(const void* x, int32_t x_type, int64_t batch, int64_t rows, int64_t C, int64_t x_batch, int64_t x_row,
+                         const void* gain, int64_t gain_batch, const void* offset, int64_t offset_batch, int32_t param_type,
+                         int32_t gain_plus_one, float eps, void* y, float* mean, float* rstd, void* stream) {
+  SVOO_TRY(check_norm(x_type, batch, rows, C, x_batch, x_row, param_type, false));
+  if (batch * rows == 0) return SVOO_OK;
+  if (!x || !y || !mean != !rstd) return SVOO_ERR_NULL;
+  if (gain_batch < 0 || offset_batch < 0) return SVOO_ERR_SHAPE;
+  const int e = elem_bytes(x_type), pe = elem_bytes(param_type);
+  if (!aligned(x, e) || !aligned(y, e) || !aligned(gain, pe) || !aligned(offset, pe)) return SVOO_ERR_ALIGN;
+  NormArgs a = {};
+  a.x = x, a.y = y, a.gain = gain, a.offset = offset, a.mean = mean, a.rstd = rstd;
+  a.x_batch = batch == 1 ? 0 : x_batch, a.x_row = x_row, a.gain_batch = gain_batch, a.offset_batch = offset_batch;
+  a.batch = batch, a.rows = rows, a.C = (int)C, a.params_fp32 = param_type == SVOO_TYPE_FP32, a.plus_one = gain_plus_one != 0, a.eps = eps;
+  return (int)launch_layer_norm(x_type, a, (cudaStream_t)stream);
+}
+
+int svoo_b200_layer_norm_workspace_bytes(int64_t batch, int64_t rows, int64_t C, int32_t per_sample, int64_t* bytes_out) {
+  if (!bytes_out) return SVOO_ERR_NULL;
+  SVOO_TRY(check_norm(SVOO_TYPE_FP32, batch, rows, C, 0, 0, SVOO_TYPE_FP32, per_sample != 0));
+  const int64_t groups = norm_groups(batch, per_sample);
+  *bytes_out = groups * norm_backward_parts(groups > 1 ? rows : batch * rows, (int)groups, (int)C) * 2 * C * 4;
+  return SVOO_OK;
+}
+
+int svoo_b200_layer_norm_backward(const void* dy, int64_t dy_batch, int64_t dy_row, const void* x, int32_t x_type, int64_t batch,
+                                  int64_t rows, int64_t C, int64_t x_batch, int64_t x_row, const float* mean, const float* rstd,
+                                  const void* gain, int64_t gain_batch, int32_t param_type, int32_t gain_plus_one,
+                                  int32_t per_sample, void* dx, void* dgain, void* doffset, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
+  SVOO_TRY(check_norm(x_type, batch, rows, C, x_batch, x_row, param_type, per_sample != 0));
+  if (dy_batch < 0 || dy_row < 0 || gain_batch < 0) return SVOO_ERR_SHAPE;
+  if (!dgain != !doffset || (dgain && !workspace)) return SVOO_ERR_NULL;
+  if (batch == 0) return SVOO_OK;                          // no sample, no sums of one; shared sums are the caller's to clear
+  if (batch * rows > 0 && (!dy || !x || !mean || !rstd || !dx)) return SVOO_ERR_NULL;
+  if (batch * rows == 0 && !dgain) return SVOO_OK;
+  const int e = elem_bytes(x_type), pe = elem_bytes(param_type);
+  if (!aligned(x, e) || !aligned(dy, e) || !aligned(dx, e) || !aligned(gain, pe) || !aligned(dgain, pe) || !aligned(doffset, pe) ||
+      !aligned(workspace, 4) || !aligned(mean, 4) || !aligned(rstd, 4))
+    return SVOO_ERR_ALIGN;
+  const int64_t groups = norm_groups(batch, per_sample);
+  const int parts = norm_backward_parts(groups > 1 ? rows : batch * rows, (int)groups, (int)C);
+  if (dgain && workspace_bytes < groups * parts * 2 * C * 4) return SVOO_ERR_WORKSPACE;
+  NormArgs a = {};
+  a.x = x, a.dy = dy, a.dx = dx, a.gain = gain, a.mean_in = mean, a.rstd_in = rstd, a.partial = dgain ? (float*)workspace : nullptr;
+  a.x_batch = batch == 1 ? 0 : x_batch, a.x_row = x_row, a.dy_batch = batch == 1 ? 0 : dy_batch, a.dy_row = dy_row;
+  a.gain_batch = groups > 1 ? gain_batch : 0;
+  a.batch = batch, a.rows = rows, a.C = (int)C, a.params_fp32 = param_type == SVOO_TYPE_FP32, a.plus_one = gain_plus_one != 0;
+  return (int)launch_layer_norm_backward(x_type, a, (int)groups, parts, dgain, doffset, (cudaStream_t)stream);
+}
+
+int svoo_b200_quantize_rows(const void* x, int32_t x_type, int64_t M, int64_t K, int64_t x_row, void* q, int64_t q_pitch, float* scale,
+                            int64_t scale_pitch, void* stream) {
+  SVOO_TRY(check_quant(x, x_type, M, K, x_row, q, q_pitch, K, scale));
+  if (scale_pitch < M) return SVOO_ERR_SHAPE;
+  if (M == 0) return SVOO_OK;
+  return (int)launch_quantize_rows(x_type, x, M, K, x_row, q, q_pitch, scale, scale_pitch, (cudaStream_t)stream);
+}
+
+int svoo_b200_quantize_columns(const void* x, int32_t x_type, int64_t M, int64_t K, int64_t x_row, void* q, int64_t q_pitch,
+                               float* scale, int64_t scale_pitch, float* column_sums, void* stream) {
+  SVOO_TRY(check_quant(x, x_type, M, K, x_row, q, q_pitch, M, scale));
+  if (scale_pitch < K || ceil_div64(M, 128) > 65535) return SVOO_ERR_SHAPE;
+  if (M == 0) return SVOO_OK;
+  return (int)launch_quantize_columns(x_type, x, M, K, x_row, q, q_pitch, scale, scale_pitch, column_sums, (cudaStream_t)stream);
+}
+
+int svoo_b200_quantize_blocks(const void* x, int32_t x_type, int64_t M, int64_t K, int64_t x_row, void* q, int64_t q_pitch, void* qt,
+                              int64_t qt_pitch, float* scale, void* stream) {
+  SVOO_TRY(check_quant(x, x_type, M, K, x_row, q, q_pitch, K, scale));
+  if (ceil_div64(M, 128) > 65535 || (qt && (qt_pitch < M || qt_pitch % 16))) return SVOO_ERR_SHAPE;
+  if (qt && !aligned(qt, 16)) return SVOO_ERR_ALIGN;
+  if (M == 0) return SVOO_OK;
+  return (int)launch_quantize_blocks(x_type, x, M, K, x_row, q, q_pitch, qt, qt_pitch, scale, (cudaStream_t)stream);
+}
+
+int svoo_b200_column_sum(const float* partial, int64_t parts, int64_t C, void* out, int32_t out_type, void* stream) {
+  if (!element(out_type)) return SVOO_ERR_TYPE;
+  if (parts < 0 || parts > INT32_MAX || C < 1 || C > kMaxRows) return SVOO_ERR_SHAPE;
+  if ((parts && !partial) || !out) return SVOO_ERR_NULL;
+  if (!aligned(partial, 4) || !aligned(out, elem_bytes(out_type))) return SVOO_ERR_ALIGN;
+  return (int)launch_column_sum(partial, parts, C, out, out_type, (cudaStream_t)stream);
+}
+
+int svoo_b200_mm_fp8(const void* a, int64_t a_pitch, const float* a_scale, int64_t a_scale_pitch, const void* b, int64_t b_pitch,
+                     const float* b_scale, int64_t b_scale_n, int64_t b_scale_k, int32_t b_scale_rows, const void* bias,
+                     int32_t bias_type, int64_t M, int64_t N, int64_t K, int32_t activation, void* out, int32_t out_type,
+                     int64_t out_pitch, float* out_scale, int64_t out_scale_pitch, void* stream) {
+  const bool quantised = out_type == SVOO_TYPE_E4M3, gelu = activation == SVOO_ACT_GELU_TANH;
+  if (!element(out_type) && !quantised) return SVOO_ERR_TYPE;
+  if ((bias && !element(bias_type)) || (!gelu && activation != SVOO_ACT_NONE)) return SVOO_ERR_TYPE;
+  if (b_scale_rows && (gelu || quantised)) return SVOO_ERR_TYPE;
+  if (M < 0 || N < 1 || K < 1 || M > kMaxRows || N > kMaxRows || K > kMaxRows) return SVOO_ERR_SHAPE;
+  if (ceil_div64(M, 128) * ceil_div64(N, 128) > (int64_t)INT32_MAX / 2) return SVOO_ERR_SHAPE;
+  if (a_pitch < K || b_pitch < K || a_pitch % 16 || b_pitch % 16 || a_scale_pitch < M || b_scale_n < 0 || b_scale_k < 0 || out_pitch < N)
+    return SVOO_ERR_SHAPE;
+  if (b_scale_rows && (b_scale_k < N || b_scale_k % 4)) return SVOO_ERR_SHAPE;
+  if (quantised && (out_pitch % 16 || out_scale_pitch < M)) return SVOO_ERR_SHAPE;
+  if (M == 0) return SVOO_OK;
+  if (!a || !a_scale || !b || !b_scale || !out || (quantised && !out_scale)) return SVOO_ERR_NULL;
+  if (!aligned(a, 16) || !aligned(b, 16) || !aligned(a_scale, 4) || !aligned(b_scale, b_scale_rows ? 16 : 4) ||
+      !aligned(out, quantised ? 16 : elem_bytes(out_type)) || !aligned(out_scale, 4) || (bias && !aligned(bias, elem_bytes(bias_type))))
+    return SVOO_ERR_ALIGN;
+  return (int)launch_linear_tc(a, a_pitch, a_scale, a_scale_pitch, b, b_pitch, b_scale, b_scale_n, b_scale_k, b_scale_rows != 0, bias,
+                               bias_type, M, N, K, gelu, out_type, out, out_pitch, out_scale, out_scale_pitch, (cudaStream_t)stream);
+}
+
+int svoo_b200_linear_status(int32_t* status, void* stream) {
+  if (!status) return SVOO_ERR_NULL;
+  return (int)read_linear_status(status, (cudaStream_t)stream);
+}
+
+}  // extern "C"

@@ -193,6 +193,9 @@ __host__ __device__ constexpr uint32_t idesc_bf16(int M, int N, bool b_mn_major)
 // [rows, 128] bf16 row-major tensor seen as boxes of 64 columns x box_rows rows with the
 // 128-byte swizzle; out-of-range rows read as zero.  Host side.
 bool make_row_tensor_map(CUtensorMap* map, const void* ptr, int64_t rows, int box_rows);
+// [rows, K] bytes, rows `pitch` bytes apart (a multiple of 16), as boxes of 128 columns x box_rows rows with the 128-byte
+// swizzle; zero outside.  Host side.
+bool make_byte_tensor_map(CUtensorMap* map, const void* ptr, int64_t rows, int64_t K, int64_t pitch, int box_rows);
 
 }  // namespace tc
 }  // namespace svoo

@@ -1,0 +1,93 @@
+"""Linear layers in 8-bit floating point: e4m3 operands with one scale per block of 128, sums in 32 bits.
+
+Activations are quantised in every call in 1 x 128 blocks along the summed dimension, weights in 128 x 128 blocks: once, as
+an Fp8Weight, for inference, or in every call from a higher-precision weight that is being trained.
+"""
+from __future__ import annotations
+
+from typing import Optional, Union
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import ops
+from .ops import Fp8Blocks as Fp8Weight
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x [..., K] as a matrix with dense rows."""
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    return x if x.shape[1] == 1 or x.stride(1) == 1 else x.contiguous()
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        a = ops.quantize_rows(x)
+        if isinstance(weight, torch.Tensor):
+            w = ops.quantize_blocks(weight, transposed=ctx.needs_input_grad[0])
+            ctx.weight_dtype = weight.dtype
+        else:
+            w = weight
+            if ctx.needs_input_grad[0]:
+                w.transposed()
+        ctx.w = w
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None)
+        return ops.mm_fp8(a, w, bias, None, x.dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        need_x, need_w, need_b = ctx.needs_input_grad
+        x, = ctx.saved_tensors
+        grad = _rows(grad)
+        M = grad.shape[0]
+        dx = dw = db = None
+        if need_x:
+            dx = ops.mm_fp8(ops.quantize_rows(grad), ctx.w.transposed(), None, None, grad.dtype)
+        if M == 0:
+            N, K = ctx.w.shape
+            dw = torch.zeros(N, K, dtype=ctx.weight_dtype, device=grad.device) if need_w else None
+            db = torch.zeros(N, dtype=ctx.bias_dtype, device=grad.device) if need_b else None
+        elif need_w:
+            g = ops.quantize_columns(grad, ctx.bias_dtype if need_b else None)
+            g, db = g if need_b else (g, None)
+            dw = ops.mm_fp8(g, ops.quantize_columns(x), None, None, ctx.weight_dtype)
+        elif need_b:
+            db = ops.quantize_columns(grad, ctx.bias_dtype)[1]
+        return dx, dw, db
+
+
+def linear_fp8(x: torch.Tensor, weight: Union[torch.Tensor, Fp8Weight], bias: Optional[torch.Tensor] = None,
+               activation: Optional[str] = None) -> torch.Tensor:
+    """act(x weight^T + bias) for x [..., K] (bf16, fp16 or fp32) -> [..., N] of x's type.  `weight` is an Fp8Weight, or a tensor
+    [N, K] that is quantised in the call.  Gradients flow to x, to a weight that is a tensor and to bias, through
+    products in e4m3 as well: the gradient of the output is quantised in blocks along what each of them sums over, and
+    rounding counts as the identity.  An Fp8Weight is a constant; with it the gradient of x needs its transpose
+    (ops.quantize_blocks(w, transposed=True)).  An activation has no gradient here."""
+    lead = x.shape[:-1]
+    training = torch.is_grad_enabled() and (x.requires_grad or (isinstance(weight, torch.Tensor) and weight.requires_grad) or
+                                            (bias is not None and bias.requires_grad))
+    m = _rows(x)
+    if training:
+        if activation is not None:
+            raise ValueError("linear_fp8 has no gradient through an activation: apply it to the result")
+        y = _Linear.apply(m, weight, bias)
+    else:
+        w = ops.quantize_blocks(weight) if isinstance(weight, torch.Tensor) else weight
+        y = ops.mm_fp8(ops.quantize_rows(m), w, bias, activation, x.dtype)
+    return y.view(*lead, y.shape[1])
+
+
+def mlp_fp8(x: torch.Tensor, w1: Fp8Weight, bias1: Optional[torch.Tensor], w2: Fp8Weight,
+            bias2: Optional[torch.Tensor]) -> torch.Tensor:
+    """linear(gelu(linear(x, w1, bias1)), w2, bias2), GELU with its tanh formula: the feed-forward of a block.  The hidden rows are
+    quantised from their 32-bit values as the first product leaves its registers.  Inference only."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, bias1, bias2)):
+        raise ValueError("mlp_fp8 has no gradient: use two linear_fp8 around the activation")
+    h = ops.mm_fp8(ops.quantize_rows(_rows(x)), w1, bias1, "gelu", ops.E4M3)
+    y = ops.mm_fp8(h, w2, bias2, None, x.dtype)
+    return y.view(*x.shape[:-1], y.shape[1])

@@ -81,3 +81,45 @@ def test_map_words_stay_inside_the_map(tmp_path):
 
 def test_sort_takes_a_cluster_that_fits(tmp_path):
     _run(tmp_path, SORT_RULE)
+
+
+def test_token_wise_entry_points_check_their_arguments():
+    """Layer norm, quantisers and 8-bit products refuse bad arguments on the host; nothing is launched."""
+    import ctypes
+    from svoo_b200._lib import LIB as L
+    buf = ctypes.create_string_buffer(4096)
+    p = (ctypes.addressof(buf) + 255) // 256 * 256
+    norm = lambda **k: L.svoo_b200_layer_norm(*[{**dict(x=p, t=0, b=1, r=2, C=64, xb=128, xr=64, g=p, gb=0, o=p, ob=0, pt=2, one=0, eps=1e-6,  # noqa: E731
+                                                         y=p, m=None, s=None, st=None), **k}[n] for n in
+                                                 ("x", "t", "b", "r", "C", "xb", "xr", "g", "gb", "o", "ob", "pt", "one", "eps", "y", "m", "s", "st")])
+    assert norm(r=0) == 0 and norm(b=0) == 0
+    assert norm(x=None) == -1 and norm(y=None) == -1 and norm(m=p) == -1
+    assert norm(C=0) == -2 and norm(C=16385) == -2 and norm(r=-1) == -2 and norm(xr=-1) == -2 and norm(b=1 << 20, r=1 << 20) == -2
+    assert norm(t=3) == -8 and norm(t=0, pt=1) == -8
+    assert norm(x=p + 1) == -5 and norm(g=p + 2) == -5
+    out = ctypes.c_int64(0)
+    assert L.svoo_b200_layer_norm_workspace_bytes(2, 100, 64, 1, ctypes.byref(out)) == 0 and out.value >= 2 * 2 * 64 * 4
+    assert L.svoo_b200_layer_norm_workspace_bytes(70000, 100, 64, 1, ctypes.byref(out)) == -2
+    assert L.svoo_b200_layer_norm_workspace_bytes(2, 100, 64, 1, None) == -1
+    back = lambda ws, dg, do: L.svoo_b200_layer_norm_backward(p, 0, 64, p, 0, 1, 2, 64, 0, 64, p, p, p, 0, 2, 0, 0, p, dg, do, p, ws, None)  # noqa: E731
+    assert back(1 << 20, p, None) == -1 and back(4, p, p) == -4
+    assert L.svoo_b200_quantize_rows(p, 0, 4, 100, 100, p, 100, p, 4, None) == -2        # pitch not a multiple of 16
+    assert L.svoo_b200_quantize_rows(p, 0, 4, 100, 100, p, 96, p, 4, None) == -2
+    assert L.svoo_b200_quantize_rows(p, 0, 4, 100, 100, p, 112, p, 3, None) == -2
+    assert L.svoo_b200_quantize_rows(p, 3, 4, 100, 100, p, 112, p, 4, None) == -8
+    assert L.svoo_b200_quantize_rows(p, 0, 4, 100, 100, p + 8, 112, p, 4, None) == -5
+    assert L.svoo_b200_quantize_rows(p, 0, 0, 100, 100, None, 112, None, 0, None) == 0
+    assert L.svoo_b200_quantize_columns(p, 0, 100, 4, 4, p, 96, p, 4, None, None) == -2
+    assert L.svoo_b200_quantize_blocks(p, 0, 100, 4, 4, p, 16, p, 96, p, None) == -2
+    assert L.svoo_b200_quantize_blocks(p, 0, 100, 4, 4, p, 16, p + 1, 112, p, None) == -5
+    assert L.svoo_b200_column_sum(p, -1, 4, p, 2, None) == -2 and L.svoo_b200_column_sum(p, 1, 4, None, 2, None) == -1
+    d = dict(a=p, ap=64, sa=p, sap=8, b=p, bp=64, sb=p, sn=1, sk=1, rows=0, bias=None, bt=0, M=8, N=16, K=64, act=0, out=p, ot=0, op=16, os=None,
+             osp=0, st=None)
+    mm = lambda **k: L.svoo_b200_mm_fp8(*{**d, **k}.values())                             # noqa: E731
+    assert mm(M=0) == 0
+    assert mm(a=None) == -1 and mm(out=None) == -1 and mm(ot=3) == -2 and mm(ot=3, op=16, osp=8) == -1
+    assert mm(K=0) == -2 and mm(N=0) == -2 and mm(ap=72) == -2 and mm(ap=48) == -2 and mm(sap=7) == -2 and mm(op=15) == -2
+    assert mm(rows=1, sk=12) == -2 and mm(rows=1, sk=18) == -2 and mm(rows=1, sk=16, act=1) == -8 and mm(rows=1, sk=16, ot=3) == -8
+    assert mm(act=2) == -8 and mm(ot=4) == -8 and mm(bias=p, bt=3) == -8
+    assert mm(a=p + 8) == -5 and mm(rows=1, sk=16, sb=p + 4) == -5
+    assert L.svoo_b200_linear_status(None, None) == -1
