@@ -431,7 +431,7 @@ int svoo_b200_column_sum(const float* partial, int64_t parts, int64_t C, void* o
 /* out[m, n] = act(sum_k a^[m, k] b^[n, k] + bias[n]) of operands in e4m3 as the quantisers leave them, sums in 32 bits.
  * a [M, K], a_scale as of quantize_rows.  b [N, K] with b_scale[(n / 128) * b_scale_n + (k / 128) * b_scale_k] (as of
  * quantize_blocks; swap the two for its transpose), or, with b_scale_rows != 0, b_scale[(k / 128) * b_scale_k + n] (as of
- * quantize_rows or quantize_columns; b_scale 16-byte aligned, b_scale_k a multiple of 4; no activation, no e4m3 output).
+ * quantize_rows or quantize_columns; b_scale 16-byte aligned, b_scale_k a multiple of 4; no bias, activation or e4m3 output).
  * out [M, N] of out_type, rows out_pitch apart; SVOO_TYPE_E4M3: the 32-bit results quantised in blocks along N, out_pitch a
  * multiple of 16, out_scale[nb * out_scale_pitch + m].  a and b 16-byte aligned, their pitches multiples of 16. */
 int svoo_b200_mm_fp8(const void* a, int64_t a_pitch, const float* a_scale, int64_t a_scale_pitch, const void* b, int64_t b_pitch,

@@ -136,7 +136,7 @@ int svoo_b200_mm_fp8(const void* a, int64_t a_pitch, const float* a_scale, int64
   const bool quantised = out_type == SVOO_TYPE_E4M3, gelu = activation == SVOO_ACT_GELU_TANH;
   if (!element(out_type) && !quantised) return SVOO_ERR_TYPE;
   if ((bias && !element(bias_type)) || (!gelu && activation != SVOO_ACT_NONE)) return SVOO_ERR_TYPE;
-  if (b_scale_rows && (gelu || quantised)) return SVOO_ERR_TYPE;
+  if (b_scale_rows && (bias || gelu || quantised)) return SVOO_ERR_TYPE;
   if (M < 0 || N < 1 || K < 1 || M > kMaxRows || N > kMaxRows || K > kMaxRows) return SVOO_ERR_SHAPE;
   if (ceil_div64(M, 128) * ceil_div64(N, 128) > (int64_t)INT32_MAX / 2) return SVOO_ERR_SHAPE;
   if (a_pitch < K || b_pitch < K || a_pitch % 16 || b_pitch % 16 || a_scale_pitch < M || b_scale_n < 0 || b_scale_k < 0 || out_pitch < N)

@@ -340,28 +340,32 @@ static EncodeTiledFn encode_fn() {
   return fn;
 }
 
-bool make_row_tensor_map(CUtensorMap* map, const void* ptr, int64_t rows, int box_rows) {
+static bool make_map_2d(CUtensorMap* map, CUtensorMapDataType type, const void* ptr, int64_t cols, int64_t rows, int64_t pitch_bytes,
+                        int box_cols, int box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
-  const cuuint64_t dims[2] = {(cuuint64_t)kHeadDim, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)kRowBytes};
-  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)pitch_bytes};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
   const cuuint32_t estr[2] = {1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return fn(map, type, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool make_row_tensor_map(CUtensorMap* map, const void* ptr, int64_t rows, int box_rows) {
+  return make_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, ptr, kHeadDim, rows, kRowBytes, 64, box_rows);
 }
 
 bool make_byte_tensor_map(CUtensorMap* map, const void* ptr, int64_t rows, int64_t K, int64_t pitch, int box_rows) {
-  EncodeTiledFn fn = encode_fn();
-  if (!fn) return false;
-  const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)pitch};
-  const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
-  const cuuint32_t estr[2] = {1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return make_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, ptr, K, rows, pitch, 128, box_rows);
+}
+
+bool make_out_tensor_map(CUtensorMap* map, int type, const void* ptr, int64_t rows, int64_t cols, int64_t pitch) {
+  const int e = type == SVOO_TYPE_E4M3 ? 1 : type == SVOO_TYPE_FP32 ? 4 : 2;
+  const CUtensorMapDataType dt = type == SVOO_TYPE_E4M3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : type == SVOO_TYPE_FP32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : type == SVOO_TYPE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  if (e == 1) cols = align_up(cols, 16);                 // e4m3 rows are written to the next multiple of 16
+  return make_map_2d(map, dt, ptr, cols, rows, pitch * e, 128 / e, 32);
 }
 
 }  // namespace tc

@@ -9,11 +9,16 @@
 // TMEM); a scale that changes from block to block cannot be applied there, so every block starts a fresh accumulator and
 // the epilogue threads add it to their running sums in registers, times sa sb.  Two accumulators alternate.
 //
-//   warp 0       TMA producer: 128 x 128 bytes of a, 256 x 128 of b per stage (128-byte swizzle), four stages
-//   warp 1       MMA issuer: M 128, N 256, K 32
-//   warps 4-11   thread r of each group of four warps owns row r (TMEM lane r) and 128 columns, one scale block of b: the
-//                factor sa sb is one number per thread and block.  The sums (128 registers) are moved between warpgroups by
-//                setmaxnreg.  Rows leave through shared memory, so that stores are whole 128-byte lines.
+// A tile is 128 CTAS rows x TN columns, CTAS = 2: a pair of SMs (cta_group::2), each with its half of a's and of b's rows in
+// shared memory, so that a byte that was fetched feeds twice the products.
+//
+//   warp 0       TMA producer: 128 x 128 bytes of a, TN / CTAS x 128 of b per stage (128-byte swizzle)
+//   warp 1       MMA issuer (of the pair's first CTA): M 128 CTAS, N TN, K 32
+//   warp 2       copies the scales of a block of k into a ring of their own (cp.async)
+//   warp 3       brings the bias of a tile's columns to 32 bits
+//   warps 4-11   thread r of each group of four warps owns row r (TMEM lane r) and TN / 2 columns, which lie in one scale block
+//                of b: the factor sa sb is one number per thread and block.  The sums (TN / 2 registers) are moved
+//                between warpgroups by setmaxnreg.  Rows leave by TMA (boxes of 32 rows x 128 bytes) while the next tile runs.
 //
 // Every mbarrier wait is bounded; on expiry the CTA sets the status word of the device and leaves.
 #include <cuda_fp8.h>
@@ -26,14 +31,24 @@ namespace tc {
 
 constexpr int kLinThreads = 384;
 constexpr int kLinRegsSums = 216, kLinRegsService = 72;       // 2 x 128 x 216 + 128 x 72 = 384 x 168
-constexpr int kLinM = 128, kLinN = 256;
-constexpr int kLinStages = 4;
-constexpr int kLinABytes = kLinM * 128, kLinBBytes = kLinN * 128, kLinStageBytes = kLinABytes + kLinBBytes;
-constexpr int kLinOutBytes = 32 * 128;                        // staging of one warp: 32 rows x 128 bytes
-constexpr int kLinSmemData = kLinStages * kLinStageBytes + 8 * kLinOutBytes;
-constexpr int kLinSmemBytes = kLinSmemData + 256 + 1024;
-enum { LIN_FULL = 0, LIN_EMPTY = LIN_FULL + kLinStages, LIN_ACC_FULL = LIN_EMPTY + kLinStages, LIN_ACC_EMPTY = LIN_ACC_FULL + 2,
-       LIN_BARS = LIN_ACC_EMPTY + 2 };
+constexpr int kLinM = 128;                                    // rows of a CTA
+constexpr int kLinBox = 32 * 128;                             // rows leave in boxes of 32 rows x 128 bytes, two per warp in flight
+constexpr int kLinScales = 8;                                 // scale blocks in flight
+
+template <int CTAS, int TN, bool kRowScales>
+struct LinCfg {
+  static constexpr int kABytes = kLinM * 128, kBRows = TN / CTAS, kBBytes = kBRows * 128, kStageBytes = kABytes + kBBytes;
+  static constexpr int kScaleFloats = kLinM + (kRowScales ? TN : 4);       // sa of the rows, sb of the columns (or of two blocks)
+  static constexpr int kFixed = 16 * kLinBox + kLinScales * kScaleFloats * 4 + 2 * TN * 4 + 512 + 1024;
+  static constexpr int kStages = (232448 - kFixed) / kStageBytes < 8 ? (232448 - kFixed) / kStageBytes : 8;
+  static constexpr int kOut = kStages * kStageBytes, kScale = kOut + 16 * kLinBox, kBias = kScale + kLinScales * kScaleFloats * 4,
+                       kBars = kBias + 2 * TN * 4;
+  static constexpr int kSmemBytes = kBars + 512 + 1024;
+  static constexpr int FULL = 0, EMPTY = FULL + kStages, ACC_FULL = EMPTY + kStages, ACC_EMPTY = ACC_FULL + 2, SC_FULL = ACC_EMPTY + 2,
+                       SC_EMPTY = SC_FULL + kLinScales, BIAS_FULL = SC_EMPTY + kLinScales, BIAS_EMPTY = BIAS_FULL + 2, BARS = BIAS_EMPTY + 2;
+  static constexpr int kTmemColumns = 2 * TN;
+  static_assert(BARS * 8 + 16 <= 512 && kSmemBytes <= 232448 && kStages >= 3);
+};
 constexpr int kLinGroupM = 16;                                // row tiles that sweep the columns together
 
 __device__ int g_linear_status;                               // != 0 after a kernel gave up on a bounded wait
@@ -48,32 +63,63 @@ struct LinearArgs {
   float* out_scale;                             // e4m3 output: [n / 128][m]
   int64_t out_scale_pitch;
   int M, N, K;
+  bool box_out;                                 // rows of out are whole 16-byte pieces: they leave by TMA
 };
 
 // D[tmem] (+)= A[smem] B[smem]^T, e4m3
+template <int CTAS>
 __device__ __forceinline__ void umma_e4m3(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  if constexpr (CTAS == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Arrives at the barrier (at this place in every CTA of the pair) when the issued MMAs have completed.
+template <int CTAS>
+__device__ __forceinline__ void commit_all(uint32_t bar) {
+  if constexpr (CTAS == 2)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(bar), "h"((uint16_t)3) : "memory");
+  else
+    tc_commit(bar);
+}
+// TMA load into this CTA's shared memory that signals a barrier of the pair's first CTA.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t first_bar) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(first_bar) : "memory");
+}
+__device__ __forceinline__ uint32_t at_cta(uint32_t addr, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void pair_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 // Instruction descriptor of kind::f8f6f4: D fp32, A and B e4m3, both K-major.
 __host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N) {
   return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
-// 32 columns of this thread's row.  Load and wait are one statement: the registers are never live between the two.
-__device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
-      "tcgen05.wait::ld.sync.aligned;\n"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr) : "memory");
+// 16 columns of this thread's row: issue, and wait for all that were issued.  The wait takes the registers as operands, so that
+// no use of theirs can be moved before it (the kernel must not spill: a register could be saved before it is filled).
+__device__ __forceinline__ void wait_columns(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) :: "memory");
 }
 // acc += {r0, r1} * f
 __device__ __forceinline__ void scale_add2(uint64_t& acc, uint32_t r0, uint32_t r1, uint64_t f) {
@@ -116,65 +162,63 @@ struct LinTile {
   }
 };
 
-// 32 rows x 128 bytes of one warp, staged swizzled (16-byte piece p of row r at p ^ (r & 7)), to out rows row0 + r,
-// elements [n0, n0 + 128 / sizeof(T)) of which those below `limit` exist.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(src) : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+
+// One warp's staged box of 32 rows x 128 bytes (16-byte piece p of row r at p ^ (r & 7): the 128-byte swizzle) to out rows
+// row0 + r, elements [n0, n0 + 128 / sizeof(T)) of which those below N exist: rows that TMA cannot address, whose 16-byte pieces
+// are not aligned.
 template <typename T>
-__device__ __forceinline__ void store_rows(const unsigned char* stage, T* out, int64_t pitch, int row0, int M, int n0, int limit, int lane) {
+__device__ __forceinline__ void store_ragged(const unsigned char* box, const LinearArgs& a, int row0, int n0, int lane) {
   constexpr int E = 16 / (int)sizeof(T), COLS = 128 / (int)sizeof(T);
-  const bool wide = (pitch * (int)sizeof(T)) % 16 == 0 && (uintptr_t)out % 16 == 0;
-  if (wide) {
+  for (int r = 0; r < 32 && row0 + r < a.M; ++r) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = i * 4 + lane / 8, p = lane % 8, n = n0 + p * E;
-      if (row0 + r >= M) continue;
-      const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((p ^ (r & 7)) << 4));
-      T* dst = out + (int64_t)(row0 + r) * pitch + n;
-      if (n + E <= limit) {
-        *reinterpret_cast<uint4*>(dst) = v;
-      } else {
-        const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-        for (int j = 0; j < E; ++j)
-          if (n + j < limit) dst[j] = e[j];
-      }
-    }
-  } else {
-    for (int r = 0; r < 32 && row0 + r < M; ++r) {
-#pragma unroll
-      for (int c = lane; c < COLS; c += 32) {
-        if (n0 + c < limit)
-          out[(int64_t)(row0 + r) * pitch + n0 + c] = *reinterpret_cast<const T*>(stage + r * 128 + (((c / E) ^ (r & 7)) << 4) + c % E * sizeof(T));
-      }
+    for (int c = lane; c < COLS; c += 32) {
+      if (n0 + c < a.N)
+        static_cast<T*>(a.out)[(int64_t)(row0 + r) * a.out_pitch + n0 + c] =
+            *reinterpret_cast<const T*>(box + r * 128 + (((c / E) ^ (r & 7)) << 4) + c % E * sizeof(T));
     }
   }
 }
 
 // OUT: SVOO_TYPE_* of the output, SVOO_TYPE_E4M3 with scales
-template <int OUT, bool kGelu, bool kRowScales>
+template <int CTAS, int TN, int OUT, bool kGelu, bool kRowScales>
 __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-                                                                   const LinearArgs a) {
+                                                                   const __grid_constant__ CUtensorMap tm_out, const LinearArgs a) {
+  using C = LinCfg<CTAS, TN, kRowScales>;
+  constexpr int TM = kLinM * CTAS, HC = TN / 2;                  // rows of a tile, columns of a warpgroup
   extern __shared__ unsigned char smem_raw[];
-  const int tiles_m = (a.M + kLinM - 1) / kLinM, tiles_n = (a.N + kLinN - 1) / kLinN, tiles = tiles_m * tiles_n;
+  const int tiles_m = (a.M + TM - 1) / TM, tiles_n = (a.N + TN - 1) / TN, tiles = tiles_m * tiles_n;
   const int KB = (a.K + 127) / 128;
+  const int rank = CTAS == 2 ? (int)(blockIdx.x & 1) : 0, worker = blockIdx.x / CTAS, workers = gridDim.x / CTAS;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* gen = smem_raw + (base - smem_u32(smem_raw));
-  const uint32_t bars = base + kLinSmemData;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + kLinSmemData + LIN_BARS * 8);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + kLinSmemData + LIN_BARS * 8 + 8);
+  const uint32_t bars = base + C::kBars;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + C::kBars + C::BARS * 8);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + C::kBars + C::BARS * 8 + 8);
   auto bar = [&](int i) { return bars + 8u * i; };
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   if (tid == 0) {
-    for (int i = 0; i < LIN_BARS; ++i) mbar_init(bar(i), i >= LIN_ACC_EMPTY ? 256 : 1);
+    for (int i = 0; i < C::BARS; ++i)
+      mbar_init(bar(i), i >= C::BIAS_EMPTY ? 8 : i >= C::BIAS_FULL ? 32 : i >= C::SC_EMPTY ? 8 : i >= C::SC_FULL ? 32 : i >= C::ACC_EMPTY ? 8 * CTAS : 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (CTAS == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(C::kTmemColumns) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(C::kTmemColumns) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   pdl_trigger();
   tc_fence_before();
   __syncthreads();
+  if (CTAS == 2) pair_sync();                              // the other CTA's barriers are set up before they are signalled
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
@@ -183,113 +227,203 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLinRegsService));
     if (warp == 0 && lane == 0) {
       // ------------------------------------------------------------------ TMA producer
+      // The first CTA's FULL barrier counts the bytes of both.
       int it = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      for (int t = worker; t < tiles && ok; t += workers) {
         const LinTile tile(t, tiles_m, tiles_n);
         for (int kb = 0; kb < KB; ++kb, ++it) {
-          const int s = it % kLinStages;
-          if (!(ok = mbar_wait(bar(LIN_EMPTY + s), ((it / kLinStages) & 1) ^ 1, abort_flag))) break;
-          mbar_expect_tx(bar(LIN_FULL + s), kLinStageBytes);
-          const uint32_t dst = base + s * kLinStageBytes;
-          tma_load_2d(dst, &tm_a, kb * 128, tile.tm * kLinM, bar(LIN_FULL + s));
-          tma_load_2d(dst + kLinABytes, &tm_b, kb * 128, tile.tn * kLinN, bar(LIN_FULL + s));
+          const int s = it % C::kStages;
+          if (!(ok = mbar_wait(bar(C::EMPTY + s), ((it / C::kStages) & 1) ^ 1, abort_flag))) break;
+          const uint32_t dst = base + s * C::kStageBytes;
+          if constexpr (CTAS == 2) {
+            if (rank == 0) mbar_expect_tx(bar(C::FULL + s), 2 * C::kStageBytes);
+            const uint32_t full = at_cta(bar(C::FULL + s), 0);
+            tma_load_pair(dst, &tm_a, kb * 128, tile.tm * TM + rank * kLinM, full);
+            tma_load_pair(dst + C::kABytes, &tm_b, kb * 128, tile.tn * TN + rank * C::kBRows, full);
+          } else {
+            mbar_expect_tx(bar(C::FULL + s), C::kStageBytes);
+            tma_load_2d(dst, &tm_a, kb * 128, tile.tm * TM, bar(C::FULL + s));
+            tma_load_2d(dst + C::kABytes, &tm_b, kb * 128, tile.tn * TN, bar(C::FULL + s));
+          }
         }
       }
-      // copies in flight land before the CTA ends
-      if (!ok)
-        for (int s = 0; s < kLinStages; ++s)
-          if (it > s) mbar_drain(bar(LIN_FULL + s), ((it - 1 - s) / kLinStages) & 1);
-    } else if (warp == 1 && lane == 0) {
+      // copies in flight land before the CTA ends (the pair leaves together)
+      if (!ok && rank == 0)
+        for (int s = 0; s < C::kStages; ++s)
+          if (it > s) mbar_drain(bar(C::FULL + s), ((it - 1 - s) / C::kStages) & 1);
+    } else if (warp == 1 && lane == 0 && rank == 0) {
       // ------------------------------------------------------------------ MMA issuer
       int it = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      for (int t = worker; t < tiles && ok; t += workers) {
         for (int kb = 0; kb < KB; ++kb, ++it) {
-          const int s = it % kLinStages, b = it & 1;
-          if (!(ok = mbar_wait(bar(LIN_FULL + s), (it / kLinStages) & 1, abort_flag))) break;
-          if (!(ok = mbar_wait(bar(LIN_ACC_EMPTY + b), ((it >> 1) & 1) ^ 1, abort_flag))) break;
+          const int s = it % C::kStages, b = it & 1;
+          if (!(ok = mbar_wait(bar(C::FULL + s), (it / C::kStages) & 1, abort_flag))) break;
+          if (!(ok = mbar_wait(bar(C::ACC_EMPTY + b), ((it >> 1) & 1) ^ 1, abort_flag))) break;
           tc_fence_after();
-          const uint32_t as = base + s * kLinStageBytes, bs = as + kLinABytes;
+          const uint32_t as = base + s * C::kStageBytes, bs = as + C::kABytes;
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)
-            umma_e4m3(tmem + b * 256, smem_desc_sw128(as + ks * 32, 16, 1024), smem_desc_sw128(bs + ks * 32, 16, 1024),
-                      idesc_e4m3(kLinM, kLinN), ks > 0);
-          tc_commit(bar(LIN_EMPTY + s));
-          tc_commit(bar(LIN_ACC_FULL + b));
+            umma_e4m3<CTAS>(tmem + b * TN, smem_desc_sw128(as + ks * 32, 16, 1024), smem_desc_sw128(bs + ks * 32, 16, 1024),
+                            idesc_e4m3(TM, TN), ks > 0);
+          commit_all<CTAS>(bar(C::EMPTY + s));
+          commit_all<CTAS>(bar(C::ACC_FULL + b));
         }
+      }
+    } else if (warp == 2) {
+      // ------------------------------------------------------------------ scales
+      int it = 0;
+      bool ok = true;
+      const int last = (a.N - 1) / 128;
+      for (int t = worker; t < tiles && ok; t += workers) {
+        const LinTile tile(t, tiles_m, tiles_n);
+        const int row0 = tile.tm * TM + rank * kLinM, n0 = tile.tn * TN;
+        for (int kb = 0; kb < KB; ++kb, ++it) {
+          const int s = it % kLinScales;
+          ok = __all_sync(0xffffffffu, mbar_wait(bar(C::SC_EMPTY + s), ((it / kLinScales) & 1) ^ 1, abort_flag));
+          if (!ok) break;
+          const uint32_t dst = base + C::kScale + s * C::kScaleFloats * 4;
+          const float* sa = a.sa + kb * a.sa_pitch;
+#pragma unroll
+          for (int i = 0; i < kLinM / 32; ++i) {
+            const int r = i * 32 + lane;
+            copy4(dst + r * 4, sa + (row0 + r < a.M ? row0 + r : a.M - 1));
+          }
+          if (kRowScales) {
+#pragma unroll
+            for (int i = 0; i < TN / 32; ++i) {
+              const int n = i * 32 + lane;
+              copy4(dst + (kLinM + n) * 4, a.sb + kb * a.sb_k + (n0 + n < a.N ? n0 + n : a.N - 1));
+            }
+          } else if (lane < 2) {
+            const int nb = (n0 + lane * HC) / 128;
+            copy4(dst + (kLinM + lane) * 4, a.sb + (int64_t)(nb < last ? nb : last) * a.sb_n + kb * a.sb_k);
+          }
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar(C::SC_FULL + s)) : "memory");
+        }
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (!kRowScales && warp == 3 && a.bias) {
+      // ------------------------------------------------------------------ bias
+      int i = 0;
+      for (int t = worker; t < tiles; t += workers, ++i) {
+        const LinTile tile(t, tiles_m, tiles_n);
+        float v[TN / 32];
+#pragma unroll
+        for (int k = 0; k < TN / 32; ++k) v[k] = load_bias(a, tile.tn * TN + k * 32 + lane);
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(C::BIAS_EMPTY + (i & 1)), ((i >> 1) & 1) ^ 1, abort_flag))) break;
+        float* dst = reinterpret_cast<float*>(gen + C::kBias) + (i & 1) * TN;
+#pragma unroll
+        for (int k = 0; k < TN / 32; ++k) dst[k * 32 + lane] = v[k];
+        mbar_arrive(bar(C::BIAS_FULL + (i & 1)));
       }
     }
   } else {
     // -------------------------------------------------------------------- sums and epilogue
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kLinRegsSums));
     const int quad = warp & 3, half = (warp - 4) >> 2;
-    const uint32_t acc_addr = tmem + ((uint32_t)(quad * 32) << 16) + half * 128;
-    unsigned char* stage = gen + kLinStages * kLinStageBytes + (warp - 4) * kLinOutBytes;
+    const uint32_t acc_addr = tmem + ((uint32_t)(quad * 32) << 16) + half * HC;
+    const float* scales = reinterpret_cast<const float*>(gen + C::kScale);
+    unsigned char* box = gen + C::kOut + (warp - 4) * 2 * kLinBox;
+    const bool has_bias = !kRowScales && a.bias;
+    int n_tile = 0;
+    const uint32_t acc_empty = CTAS == 2 ? at_cta(bar(C::ACC_EMPTY), 0) : bar(C::ACC_EMPTY);
     int it = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const LinTile tile(t, tiles_m, tiles_n);
-      const int row0 = tile.tm * kLinM + quad * 32, row = row0 + lane, n0 = tile.tn * kLinN + half * 128;
-      const float* sa = a.sa + (row < a.M ? row : a.M - 1);
-      const int last = (a.N - 1) / 128;
-      const float* sb = kRowScales ? a.sb + n0 : a.sb + (int64_t)(n0 / 128 < last ? n0 / 128 : last) * a.sb_n;
-      uint64_t sum[64];
+    for (int t = worker; t < tiles && ok; t += workers, ++n_tile) {
+      uint64_t sum[HC / 2];
 #pragma unroll
-      for (int i = 0; i < 64; ++i) sum[i] = 0;
-      // the factors of two blocks ahead are on their way
-      float fa = sa[0], fa1 = KB > 1 ? sa[a.sa_pitch] : 0.f;
-      float fb = kRowScales ? 1.f : sb[0], fb1 = !kRowScales && KB > 1 ? sb[a.sb_k] : 1.f;
+      for (int i = 0; i < HC / 2; ++i) sum[i] = 0;
+#pragma unroll 1
       for (int kb = 0; kb < KB; ++kb, ++it) {
-        const float fa2 = kb + 2 < KB ? sa[(kb + 2) * a.sa_pitch] : 0.f;
-        const float fb2 = !kRowScales && kb + 2 < KB ? sb[(kb + 2) * a.sb_k] : 1.f;
-        const int b = it & 1;
-        ok = __all_sync(0xffffffffu, mbar_wait(bar(LIN_ACC_FULL + b), (it >> 1) & 1, abort_flag));
+        const int b = it & 1, sl = it % kLinScales;
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(C::SC_FULL + sl), (it / kLinScales) & 1, abort_flag) &&
+                                         mbar_wait(bar(C::ACC_FULL + b), (it >> 1) & 1, abort_flag));
         if (!ok) break;
         tc_fence_after();
-        const float f = fa * fb;
+        const float* sc = scales + sl * C::kScaleFloats;
+        const float f = sc[quad * 32 + lane] * (kRowScales ? 1.f : sc[kLinM + half]);
         const uint64_t f2 = pack2(f, f);
+        const uint32_t at = acc_addr + b * TN;
+        uint32_t r[2][16];
+        tmem_ld16_nowait(at, r[0]);
 #pragma unroll
-        for (int ch = 0; ch < 4; ++ch) {
-          uint32_t r[32];
-          load_columns(acc_addr + b * 256 + ch * 32, r);
+        for (int ch = 0; ch < HC / 16; ++ch) {
+          wait_columns(r[ch & 1]);
+          if (ch + 1 < HC / 16) {
+            tmem_ld16_nowait(at + (ch + 1) * 16, r[(ch + 1) & 1]);
+          } else {                                         // all columns are here: the next block may be summed over them
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if (CTAS == 2) arrive_cluster(acc_empty + 8 * b);
+              else mbar_arrive(acc_empty + 8 * b);
+            }
+          }
+          const uint32_t(&v)[16] = r[ch & 1];
           if (kRowScales) {
-            const float4* cs = reinterpret_cast<const float4*>(sb + kb * a.sb_k + ch * 32);
+            const float4* cs = reinterpret_cast<const float4*>(sc + kLinM + half * HC + ch * 16);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float4 c = n0 + ch * 32 + i * 4 < a.N ? __ldg(cs + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-              scale_add2(sum[ch * 16 + 2 * i], r[4 * i], r[4 * i + 1], mul2(pack2(c.x, c.y), f2));
-              scale_add2(sum[ch * 16 + 2 * i + 1], r[4 * i + 2], r[4 * i + 3], mul2(pack2(c.z, c.w), f2));
+            for (int i = 0; i < 4; ++i) {
+              const float4 c = cs[i];
+              scale_add2(sum[ch * 8 + 2 * i], v[4 * i], v[4 * i + 1], mul2(pack2(c.x, c.y), f2));
+              scale_add2(sum[ch * 8 + 2 * i + 1], v[4 * i + 2], v[4 * i + 3], mul2(pack2(c.z, c.w), f2));
             }
           } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) scale_add2(sum[ch * 16 + i], r[2 * i], r[2 * i + 1], f2);
+            for (int i = 0; i < 8; ++i) scale_add2(sum[ch * 8 + i], v[2 * i], v[2 * i + 1], f2);
           }
         }
-        tc_fence_before();
-        mbar_arrive(bar(LIN_ACC_EMPTY + b));
-        fa = fa1, fa1 = fa2, fb = fb1, fb1 = fb2;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::SC_EMPTY + sl));
       }
       if (!ok) break;
-      if (n0 >= a.N) continue;
-      if (a.bias) {
+      const LinTile tile(t, tiles_m, tiles_n);
+      const int row0 = tile.tm * TM + rank * kLinM + quad * 32, row = row0 + lane, n0 = tile.tn * TN + half * HC;
+      const uint32_t bias = base + C::kBias + ((n_tile & 1) * TN + half * HC) * 4;
+      if (has_bias) ok = __all_sync(0xffffffffu, mbar_wait(bar(C::BIAS_FULL + (n_tile & 1)), (n_tile >> 1) & 1, abort_flag));
+      if (!ok) break;
+      const bool skip = n0 >= a.N || row0 >= a.M;
+      // four columns at a time
+      auto finish4 = [&](int c) {
+        float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (has_bias)                                      // volatile: all of them at once would not fit the registers
+          asm volatile("ld.volatile.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(b.x), "=f"(b.y), "=f"(b.z), "=f"(b.w) : "r"(bias + c * 4));
+        float v[4] = {half_of(sum[c / 2], 0) + b.x, half_of(sum[c / 2], 1) + b.y, half_of(sum[c / 2 + 1], 0) + b.z, half_of(sum[c / 2 + 1], 1) + b.w};
+        if (kGelu) {
 #pragma unroll
-        for (int i = 0; i < 64; ++i)
-          sum[i] = pack2(half_of(sum[i], 0) + load_bias(a, n0 + 2 * i), half_of(sum[i], 1) + load_bias(a, n0 + 2 * i + 1));
-      }
-      if (kGelu) {
-#pragma unroll
-        for (int i = 0; i < 64; ++i) sum[i] = pack2(gelu_tanh(half_of(sum[i], 0)), gelu_tanh(half_of(sum[i], 1)));
-      }
+          for (int i = 0; i < 4; ++i) v[i] = gelu_tanh(v[i]);
+        }
+        sum[c / 2] = pack2(v[0], v[1]);
+        sum[c / 2 + 1] = pack2(v[2], v[3]);
+      };
+      // a box is written again when the store before the last has read it
+      auto begin_box = [&](int i) {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        __syncwarp();
+        return box + (i & 1) * kLinBox;
+      };
+      auto end_box = [&](const unsigned char* at, int n) {
+        fence_async_proxy();
+        __syncwarp();
+        if (lane == 0 && !skip) tma_store_2d(&tm_out, n, row0, smem_u32(at));
+      };
       if constexpr (OUT == SVOO_TYPE_E4M3) {
         // the thread's 128 columns are one block of its row; columns behind N are zero
+        static_assert(HC == 128);
         uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < 64; ++i)
-          top = max(top, max((uint32_t)sum[i] & 0x7fffffffu, (uint32_t)(sum[i] >> 32) & 0x7fffffffu));
+        for (int c = 0; c < HC; c += 4) {
+          finish4(c);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            top = max(top, max((uint32_t)sum[c / 2 + i] & 0x7fffffffu, (uint32_t)(sum[c / 2 + i] >> 32) & 0x7fffffffu));
+        }
         float s = __fdiv_rn(__uint_as_float(top), 448.f);
         s = s < 0x1p-126f ? 0x1p-126f : s;
-        if (row < a.M) a.out_scale[(n0 / 128) * a.out_scale_pitch + row] = s;
+        if (row < a.M && !skip) a.out_scale[(n0 / 128) * a.out_scale_pitch + row] = s;
+        unsigned char* at = begin_box(n_tile);
 #pragma unroll
         for (int p = 0; p < 8; ++p) {
           uint32_t w[4];
@@ -300,81 +434,126 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
             const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(half_of(v, 0), s), __fdiv_rn(half_of(v, 1), s)), __NV_SATFINITE, __NV_E4M3);
             w[i] = lo | hi << 16;
           }
-          *reinterpret_cast<uint4*>(stage + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(at + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        __syncwarp();
-        store_rows<uint8_t>(stage, (uint8_t*)a.out, a.out_pitch, row0, a.M, n0, (int)a.out_pitch, lane);
-        __syncwarp();
+        end_box(at, n0);
       } else {
         typedef typename ElemOf<OUT>::T T;
         constexpr int COLS = 128 / (int)sizeof(T), E = 16 / (int)sizeof(T);
 #pragma unroll
-        for (int pass = 0; pass < 128 / COLS; ++pass) {
+        for (int pass = 0; pass < HC / COLS; ++pass) {
+          unsigned char* at = begin_box(pass);
 #pragma unroll
           for (int p = 0; p < 8; ++p) {
+            const int c = pass * COLS + p * E;
             Vec<T, E> o;
 #pragma unroll
-            for (int i = 0; i < E; ++i) o.v[i] = from_f32<T>(half_of(sum[(pass * COLS + p * E + i) / 2], i & 1));
-            *reinterpret_cast<Vec<T, E>*>(stage + lane * 128 + ((p ^ (lane & 7)) << 4)) = o;
+            for (int i = 0; i < E; i += 4) finish4(c + i);
+#pragma unroll
+            for (int i = 0; i < E; ++i) o.v[i] = from_f32<T>(half_of(sum[(c + i) / 2], i & 1));
+            *reinterpret_cast<Vec<T, E>*>(at + lane * 128 + ((p ^ (lane & 7)) << 4)) = o;
           }
-          __syncwarp();
-          store_rows<T>(stage, (T*)a.out, a.out_pitch, row0, a.M, n0 + pass * COLS, a.N, lane);
-          __syncwarp();
+          if (a.box_out) {
+            end_box(at, n0 + pass * COLS);
+          } else {
+            __syncwarp();
+            if (!skip) store_ragged<T>(at, a, row0, n0 + pass * COLS, lane);
+          }
         }
       }
+      if (has_bias) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::BIAS_EMPTY + (n_tile & 1)));
+      }
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
+  if (CTAS == 2) pair_sync();
   if (tid == 0 && *abort_flag) atomicExch(&g_linear_status, 1);
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    if constexpr (CTAS == 2)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemColumns) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemColumns) : "memory");
   }
 }
 
 }  // namespace tc
 
-template <int OUT, bool kGelu, bool kRowScales>
-static cudaError_t launch_one(const CUtensorMap& ma, const CUtensorMap& mb, const tc::LinearArgs& args, cudaStream_t st) {
-  auto* kernel = &tc::linear_tc_kernel<OUT, kGelu, kRowScales>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tc::kLinSmemBytes);
+struct LinearCall {
+  const void *a, *b;
+  int64_t a_pitch, b_pitch;
+  tc::LinearArgs args;
+  cudaStream_t st;
+};
+
+template <int CTAS, int TN, int OUT, bool kGelu, bool kRowScales>
+static cudaError_t launch_tiles(const LinearCall& c) {
+  using C = tc::LinCfg<CTAS, TN, kRowScales>;
+  alignas(64) CUtensorMap ma, mb, mo = {};
+  if (!tc::make_byte_tensor_map(&ma, c.a, c.args.M, c.args.K, c.a_pitch, tc::kLinM) ||
+      !tc::make_byte_tensor_map(&mb, c.b, c.args.N, c.args.K, c.b_pitch, C::kBRows) ||
+      (c.args.box_out && !tc::make_out_tensor_map(&mo, OUT, c.args.out, c.args.M, c.args.N, c.args.out_pitch)))
+    return cudaErrorInvalidValue;
+  auto* kernel = &tc::linear_tc_kernel<CTAS, TN, OUT, kGelu, kRowScales>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
   if (e != cudaSuccess) return e;
   int dev = 0, sms = 0;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const int64_t tiles = ceil_div64(args.M, tc::kLinM) * ceil_div64(args.N, tc::kLinN);
+  const int64_t tiles = ceil_div64(c.args.M, tc::kLinM * CTAS) * ceil_div64(c.args.N, TN);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles < sms / CTAS ? tiles : sms / CTAS) * CTAS);
+  cfg.blockDim = dim3(tc::kLinThreads);
+  cfg.dynamicSmemBytes = C::kSmemBytes;
+  cfg.stream = c.st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CTAS;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CTAS == 2 ? 2 : 1;
   count_launches(1);
-  return launch_pdl(kernel, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(tc::kLinThreads), (size_t)tc::kLinSmemBytes, st, ma, mb, args);
+  return cudaLaunchKernelEx(&cfg, kernel, ma, mb, mo, c.args);
+}
+
+template <int OUT, bool kGelu, bool kRowScales>
+static cudaError_t launch_one(const LinearCall& c) {
+  return launch_tiles<2, 256, OUT, kGelu, kRowScales>(c);
 }
 
 cudaError_t launch_linear_tc(const void* a, int64_t a_pitch, const float* sa, int64_t sa_pitch, const void* b, int64_t b_pitch, const float* sb,
                              int64_t sb_n, int64_t sb_k, bool row_scales, const void* bias, int bias_type, int64_t M, int64_t N, int64_t K,
                              bool gelu, int out_type, void* out, int64_t out_pitch, float* out_scale, int64_t out_scale_pitch, cudaStream_t st) {
-  alignas(64) CUtensorMap ma, mb;
-  if (!tc::make_byte_tensor_map(&ma, a, M, K, a_pitch, tc::kLinM) || !tc::make_byte_tensor_map(&mb, b, N, K, b_pitch, tc::kLinN))
-    return cudaErrorInvalidValue;
-  const tc::LinearArgs args{sa, sb, sa_pitch, sb_n, sb_k, bias, bias_type, out, out_pitch, out_scale, out_scale_pitch, (int)M, (int)N, (int)K};
+  const int e = out_type == SVOO_TYPE_E4M3 ? 1 : elem_bytes(out_type);
+  const bool box_out = out_pitch * e % 16 == 0 && (uintptr_t)out % 16 == 0;
+  const LinearCall c{a, b, a_pitch, b_pitch,
+                     {sa, sb, sa_pitch, sb_n, sb_k, bias, bias_type, out, out_pitch, out_scale, out_scale_pitch, (int)M, (int)N, (int)K, box_out}, st};
   if (row_scales) {
     switch (out_type) {
-      case SVOO_TYPE_BF16: return launch_one<SVOO_TYPE_BF16, false, true>(ma, mb, args, st);
-      case SVOO_TYPE_FP16: return launch_one<SVOO_TYPE_FP16, false, true>(ma, mb, args, st);
-      default: return launch_one<SVOO_TYPE_FP32, false, true>(ma, mb, args, st);
+      case SVOO_TYPE_BF16: return launch_one<SVOO_TYPE_BF16, false, true>(c);
+      case SVOO_TYPE_FP16: return launch_one<SVOO_TYPE_FP16, false, true>(c);
+      default: return launch_one<SVOO_TYPE_FP32, false, true>(c);
     }
   }
   if (gelu) {
     switch (out_type) {
-      case SVOO_TYPE_BF16: return launch_one<SVOO_TYPE_BF16, true, false>(ma, mb, args, st);
-      case SVOO_TYPE_FP16: return launch_one<SVOO_TYPE_FP16, true, false>(ma, mb, args, st);
-      case SVOO_TYPE_FP32: return launch_one<SVOO_TYPE_FP32, true, false>(ma, mb, args, st);
-      default: return launch_one<SVOO_TYPE_E4M3, true, false>(ma, mb, args, st);
+      case SVOO_TYPE_BF16: return launch_one<SVOO_TYPE_BF16, true, false>(c);
+      case SVOO_TYPE_FP16: return launch_one<SVOO_TYPE_FP16, true, false>(c);
+      case SVOO_TYPE_FP32: return launch_one<SVOO_TYPE_FP32, true, false>(c);
+      default: return launch_one<SVOO_TYPE_E4M3, true, false>(c);
     }
   }
   switch (out_type) {
-    case SVOO_TYPE_BF16: return launch_one<SVOO_TYPE_BF16, false, false>(ma, mb, args, st);
-    case SVOO_TYPE_FP16: return launch_one<SVOO_TYPE_FP16, false, false>(ma, mb, args, st);
-    case SVOO_TYPE_FP32: return launch_one<SVOO_TYPE_FP32, false, false>(ma, mb, args, st);
-    default: return launch_one<SVOO_TYPE_E4M3, false, false>(ma, mb, args, st);
+    case SVOO_TYPE_BF16: return launch_one<SVOO_TYPE_BF16, false, false>(c);
+    case SVOO_TYPE_FP16: return launch_one<SVOO_TYPE_FP16, false, false>(c);
+    case SVOO_TYPE_FP32: return launch_one<SVOO_TYPE_FP32, false, false>(c);
+    default: return launch_one<SVOO_TYPE_E4M3, false, false>(c);
   }
 }
 

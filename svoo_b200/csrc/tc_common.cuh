@@ -196,6 +196,9 @@ bool make_row_tensor_map(CUtensorMap* map, const void* ptr, int64_t rows, int bo
 // [rows, K] bytes, rows `pitch` bytes apart (a multiple of 16), as boxes of 128 columns x box_rows rows with the 128-byte
 // swizzle; zero outside.  Host side.
 bool make_byte_tensor_map(CUtensorMap* map, const void* ptr, int64_t rows, int64_t K, int64_t pitch, int box_rows);
+// [rows, cols] elements of an SVOO_TYPE_*, rows `pitch` elements (a multiple of 16 bytes) apart, as boxes of 128 bytes x 32
+// rows with the 128-byte swizzle, for stores.  Host side.
+bool make_out_tensor_map(CUtensorMap* map, int type, const void* ptr, int64_t rows, int64_t cols, int64_t pitch);
 
 }  // namespace tc
 }  // namespace svoo

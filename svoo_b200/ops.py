@@ -807,7 +807,7 @@ def _e4m3_operand(q: torch.Tensor, scale: torch.Tensor, scale_shape, what: str) 
 
 def mm_fp8(a: Fp8Rows, b, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
            out_dtype: torch.dtype = torch.bfloat16):
-    """act(a b^T + bias), sums in 32 bits: a Fp8Rows [M, K]; b Fp8Blocks [N, K], or Fp8Rows [N, K] (no activation); bias [N], bf16,
+    """act(a b^T + bias), sums in 32 bits: a Fp8Rows [M, K]; b Fp8Blocks [N, K], or Fp8Rows [N, K] (then neither of the next two); bias [N], bf16,
     fp16 or fp32; activation None or "gelu" (its tanh formula).  out_dtype bf16, fp16, fp32, or float8_e4m3fn for
     the 32-bit results quantised in 1 x 128 blocks, an Fp8Rows, ready to be the next product's a."""
     M, K = a.q.shape
@@ -821,8 +821,8 @@ def mm_fp8(a: Fp8Rows, b, bias: Optional[torch.Tensor] = None, activation: Optio
     quantised = out_dtype == E4M3
     if not quantised and out_dtype not in TYPES:
         raise ValueError("out_dtype must be bf16, fp16, fp32 or float8_e4m3fn")
-    if rows and (quantised or activation is not None):
-        raise ValueError("a product of two Fp8Rows takes no activation and gives no e4m3 output")
+    if rows and (quantised or activation is not None or bias is not None):
+        raise ValueError("a product of two Fp8Rows takes no bias or activation and gives no e4m3 output")
     ap = _e4m3_operand(a.q, a.scale, (KB, M), "a")
     bp = _e4m3_operand(b.q, b.scale, (KB, N) if rows else ((N + 127) // 128, KB), "b")
     if M > 1 and a.scale.stride(1) != 1:
