@@ -2,9 +2,9 @@
 #include "rows_common.cuh"
 
 namespace svoo {
-int norm_backward_parts(int64_t rows, int groups, int C);
+int64_t norm_backward_bytes(int64_t rows, int groups, int C);
 cudaError_t launch_layer_norm(int type, const NormArgs& a, cudaStream_t st);
-cudaError_t launch_layer_norm_backward(int type, const NormArgs& a, int groups, int parts, void* dgain, void* doffset, cudaStream_t st);
+cudaError_t launch_layer_norm_backward(int type, const NormArgs& a, int groups, void* dgain, void* doffset, cudaStream_t st);
 cudaError_t launch_column_sum(const float* partial, int64_t parts, int64_t C, void* out, int out_type, cudaStream_t st);
 cudaError_t launch_quantize_rows(int type, const void* x, int64_t M, int64_t K, int64_t row_stride, void* q, int64_t q_pitch, float* scale,
                                  int64_t scale_pitch, cudaStream_t st);
@@ -12,7 +12,7 @@ cudaError_t launch_quantize_columns(int type, const void* x, int64_t M, int64_t 
                                     float* scale, int64_t scale_pitch, float* column_sum, cudaStream_t st);
 cudaError_t launch_quantize_blocks(int type, const void* w, int64_t N, int64_t K, int64_t row_stride, void* q, int64_t q_pitch, void* qt,
                                    int64_t qt_pitch, float* scale, cudaStream_t st);
-cudaError_t launch_linear_tc(const void* a, int64_t a_pitch, const float* sa, int64_t sa_pitch, const void* b, int64_t b_pitch, const float* sb,
+cudaError_t launch_linear(const void* a, int64_t a_pitch, const float* sa, int64_t sa_pitch, const void* b, int64_t b_pitch, const float* sb,
                              int64_t sb_n, int64_t sb_k, bool row_scales, const void* bias, int bias_type, int64_t M, int64_t N, int64_t K,
                              bool gelu, int out_type, void* out, int64_t out_pitch, float* out_scale, int64_t out_scale_pitch, cudaStream_t st);
 cudaError_t read_linear_status(int32_t* out, cudaStream_t st);
@@ -40,6 +40,26 @@ int check_quant(const void* x, int32_t type, int64_t M, int64_t K, int64_t x_row
   if (!aligned(q, 16) || !aligned(x, elem_bytes(type)) || !aligned(scale, 4)) return SVOO_ERR_ALIGN;
   return SVOO_OK;
 }
+int check_mm(const void* a, int64_t a_pitch, const float* a_scale, int64_t a_scale_pitch, const void* b, int64_t b_pitch, const float* b_scale,
+             int64_t b_scale_n, int64_t b_scale_k, int32_t b_scale_rows, const void* bias, int32_t bias_type, int64_t M, int64_t N, int64_t K,
+             int32_t activation, void* out, int32_t out_type, int64_t out_pitch, float* out_scale, int64_t out_scale_pitch) {
+  const bool quantised = out_type == SVOO_TYPE_E4M3, gelu = activation == SVOO_ACT_GELU_TANH;
+  if (!element(out_type) && !quantised) return SVOO_ERR_TYPE;
+  if ((bias && !element(bias_type)) || (!gelu && activation != SVOO_ACT_NONE)) return SVOO_ERR_TYPE;
+  if (b_scale_rows && (bias || gelu || quantised)) return SVOO_ERR_TYPE;
+  if (M < 0 || N < 1 || K < 1 || M > kMaxRows || N > kMaxRows || K > kMaxRows) return SVOO_ERR_SHAPE;
+  if (ceil_div64(M, 128) * ceil_div64(N, 128) > (int64_t)INT32_MAX / 2) return SVOO_ERR_SHAPE;
+  if (a_pitch < K || b_pitch < K || a_pitch % 16 || b_pitch % 16 || a_scale_pitch < M || b_scale_n < 0 || b_scale_k < 0 || out_pitch < N)
+    return SVOO_ERR_SHAPE;
+  if (b_scale_rows && (b_scale_k < N || b_scale_k % 4)) return SVOO_ERR_SHAPE;
+  if (quantised && (out_pitch % 16 || out_scale_pitch < M)) return SVOO_ERR_SHAPE;
+  if (M == 0) return SVOO_OK;
+  if (!a || !a_scale || !b || !b_scale || !out || (quantised && !out_scale)) return SVOO_ERR_NULL;
+  if (!aligned(a, 16) || !aligned(b, 16) || !aligned(a_scale, 4) || !aligned(b_scale, b_scale_rows ? 16 : 4) ||
+      !aligned(out, quantised ? 16 : elem_bytes(out_type)) || !aligned(out_scale, 4) || (bias && !aligned(bias, elem_bytes(bias_type))))
+    return SVOO_ERR_ALIGN;
+  return SVOO_OK;
+}
 int64_t norm_groups(int64_t batch, int32_t per_sample) { return per_sample && batch > 1 ? batch : 1; }
 #define SVOO_TRY(expr) do { int _rc = (expr); if (_rc != SVOO_OK) return _rc; } while (0)
 }  // namespace
@@ -59,6 +79,7 @@ int svoo_b200_layer_norm(const void* x, int32_t x_type, int64_t batch, int64_t r
   a.x = x, a.y = y, a.gain = gain, a.offset = offset, a.mean = mean, a.rstd = rstd;
   a.x_batch = batch == 1 ? 0 : x_batch, a.x_row = x_row, a.gain_batch = gain_batch, a.offset_batch = offset_batch;
   a.batch = batch, a.rows = rows, a.C = (int)C, a.params_fp32 = param_type == SVOO_TYPE_FP32, a.plus_one = gain_plus_one != 0, a.eps = eps;
+  if (!(a.status = rows_status_word())) return (int)cudaErrorInvalidDevice;
   return (int)launch_layer_norm(x_type, a, (cudaStream_t)stream);
 }
 
@@ -66,7 +87,7 @@ int svoo_b200_layer_norm_workspace_bytes(int64_t batch, int64_t rows, int64_t C,
   if (!bytes_out) return SVOO_ERR_NULL;
   SVOO_TRY(check_norm(SVOO_TYPE_FP32, batch, rows, C, 0, 0, SVOO_TYPE_FP32, per_sample != 0));
   const int64_t groups = norm_groups(batch, per_sample);
-  *bytes_out = groups * norm_backward_parts(groups > 1 ? rows : batch * rows, (int)groups, (int)C) * 2 * C * 4;
+  *bytes_out = norm_backward_bytes(groups > 1 ? rows : batch * rows, (int)groups, (int)C);
   return SVOO_OK;
 }
 
@@ -86,14 +107,14 @@ int svoo_b200_layer_norm_backward(const void* dy, int64_t dy_batch, int64_t dy_r
       !aligned(workspace, 4) || !aligned(mean, 4) || !aligned(rstd, 4))
     return SVOO_ERR_ALIGN;
   const int64_t groups = norm_groups(batch, per_sample);
-  const int parts = norm_backward_parts(groups > 1 ? rows : batch * rows, (int)groups, (int)C);
-  if (dgain && workspace_bytes < groups * parts * 2 * C * 4) return SVOO_ERR_WORKSPACE;
+  if (dgain && workspace_bytes < norm_backward_bytes(groups > 1 ? rows : batch * rows, (int)groups, (int)C)) return SVOO_ERR_WORKSPACE;
   NormArgs a = {};
   a.x = x, a.dy = dy, a.dx = dx, a.gain = gain, a.mean_in = mean, a.rstd_in = rstd, a.partial = dgain ? (float*)workspace : nullptr;
   a.x_batch = batch == 1 ? 0 : x_batch, a.x_row = x_row, a.dy_batch = batch == 1 ? 0 : dy_batch, a.dy_row = dy_row;
   a.gain_batch = groups > 1 ? gain_batch : 0;
   a.batch = batch, a.rows = rows, a.C = (int)C, a.params_fp32 = param_type == SVOO_TYPE_FP32, a.plus_one = gain_plus_one != 0;
-  return (int)launch_layer_norm_backward(x_type, a, (int)groups, parts, dgain, doffset, (cudaStream_t)stream);
+  if (!(a.status = rows_status_word())) return (int)cudaErrorInvalidDevice;
+  return (int)launch_layer_norm_backward(x_type, a, (int)groups, dgain, doffset, (cudaStream_t)stream);
 }
 
 int svoo_b200_quantize_rows(const void* x, int32_t x_type, int64_t M, int64_t K, int64_t x_row, void* q, int64_t q_pitch, float* scale,
@@ -133,23 +154,41 @@ int svoo_b200_mm_fp8(const void* a, int64_t a_pitch, const float* a_scale, int64
                      const float* b_scale, int64_t b_scale_n, int64_t b_scale_k, int32_t b_scale_rows, const void* bias,
                      int32_t bias_type, int64_t M, int64_t N, int64_t K, int32_t activation, void* out, int32_t out_type,
                      int64_t out_pitch, float* out_scale, int64_t out_scale_pitch, void* stream) {
-  const bool quantised = out_type == SVOO_TYPE_E4M3, gelu = activation == SVOO_ACT_GELU_TANH;
-  if (!element(out_type) && !quantised) return SVOO_ERR_TYPE;
-  if ((bias && !element(bias_type)) || (!gelu && activation != SVOO_ACT_NONE)) return SVOO_ERR_TYPE;
-  if (b_scale_rows && (bias || gelu || quantised)) return SVOO_ERR_TYPE;
-  if (M < 0 || N < 1 || K < 1 || M > kMaxRows || N > kMaxRows || K > kMaxRows) return SVOO_ERR_SHAPE;
-  if (ceil_div64(M, 128) * ceil_div64(N, 128) > (int64_t)INT32_MAX / 2) return SVOO_ERR_SHAPE;
-  if (a_pitch < K || b_pitch < K || a_pitch % 16 || b_pitch % 16 || a_scale_pitch < M || b_scale_n < 0 || b_scale_k < 0 || out_pitch < N)
-    return SVOO_ERR_SHAPE;
-  if (b_scale_rows && (b_scale_k < N || b_scale_k % 4)) return SVOO_ERR_SHAPE;
-  if (quantised && (out_pitch % 16 || out_scale_pitch < M)) return SVOO_ERR_SHAPE;
+  SVOO_TRY(check_mm(a, a_pitch, a_scale, a_scale_pitch, b, b_pitch, b_scale, b_scale_n, b_scale_k, b_scale_rows, bias, bias_type, M, N, K,
+                    activation, out, out_type, out_pitch, out_scale, out_scale_pitch));
   if (M == 0) return SVOO_OK;
-  if (!a || !a_scale || !b || !b_scale || !out || (quantised && !out_scale)) return SVOO_ERR_NULL;
-  if (!aligned(a, 16) || !aligned(b, 16) || !aligned(a_scale, 4) || !aligned(b_scale, b_scale_rows ? 16 : 4) ||
-      !aligned(out, quantised ? 16 : elem_bytes(out_type)) || !aligned(out_scale, 4) || (bias && !aligned(bias, elem_bytes(bias_type))))
-    return SVOO_ERR_ALIGN;
-  return (int)launch_linear_tc(a, a_pitch, a_scale, a_scale_pitch, b, b_pitch, b_scale, b_scale_n, b_scale_k, b_scale_rows != 0, bias,
-                               bias_type, M, N, K, gelu, out_type, out, out_pitch, out_scale, out_scale_pitch, (cudaStream_t)stream);
+  return (int)launch_linear(a, a_pitch, a_scale, a_scale_pitch, b, b_pitch, b_scale, b_scale_n, b_scale_k, b_scale_rows != 0, bias,
+                               bias_type, M, N, K, activation == SVOO_ACT_GELU_TANH, out_type, out, out_pitch, out_scale, out_scale_pitch,
+                            (cudaStream_t)stream);
+}
+
+int svoo_b200_linear_fp8_workspace_bytes(int64_t M, int64_t K, int64_t* bytes_out) {
+  if (!bytes_out) return SVOO_ERR_NULL;
+  if (M < 0 || K < 1 || M > kMaxRows || K > kMaxRows) return SVOO_ERR_SHAPE;
+  *bytes_out = align_up(M * align_up(K, 16), 256) + ceil_div64(K, 128) * M * 4;
+  return SVOO_OK;
+}
+
+int svoo_b200_linear_fp8(const void* x, int32_t x_type, int64_t M, int64_t K, int64_t x_row, const void* b, int64_t b_pitch,
+                         const float* b_scale, int64_t b_scale_n, int64_t b_scale_k, const void* bias, int32_t bias_type, int64_t N,
+                         int32_t activation, void* out, int32_t out_type, int64_t out_pitch, float* out_scale,
+                         int64_t out_scale_pitch, void* workspace, int64_t workspace_bytes, void* stream) {
+  int64_t need = 0;
+  SVOO_TRY(svoo_b200_linear_fp8_workspace_bytes(M, K, &need));
+  if (M > 0 && !workspace) return SVOO_ERR_NULL;
+  if (workspace_bytes < need) return SVOO_ERR_WORKSPACE;
+  if (!aligned(workspace, 16)) return SVOO_ERR_ALIGN;
+  const int64_t pitch = align_up(K, 16);
+  float* scale = reinterpret_cast<float*>(static_cast<char*>(workspace) + align_up(M * pitch, 256));
+  // the product's arguments are checked before anything is launched
+  SVOO_TRY(check_quant(x, x_type, M, K, x_row, workspace, pitch, K, scale));
+  SVOO_TRY(check_mm(workspace, pitch, scale, M, b, b_pitch, b_scale, b_scale_n, b_scale_k, 0, bias, bias_type, M, N, K, activation, out,
+                    out_type, out_pitch, out_scale, out_scale_pitch));
+  if (M == 0) return SVOO_OK;
+  const cudaError_t e = launch_quantize_rows(x_type, x, M, K, x_row, workspace, pitch, scale, M, (cudaStream_t)stream);
+  if (e != cudaSuccess) return (int)e;
+  return (int)launch_linear(workspace, pitch, scale, M, b, b_pitch, b_scale, b_scale_n, b_scale_k, false, bias, bias_type, M, N, K,
+                            activation == SVOO_ACT_GELU_TANH, out_type, out, out_pitch, out_scale, out_scale_pitch, (cudaStream_t)stream);
 }
 
 int svoo_b200_linear_status(int32_t* status, void* stream) {

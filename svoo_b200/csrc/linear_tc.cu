@@ -21,16 +21,12 @@
 //                between warpgroups by setmaxnreg.  Rows leave by TMA (boxes of 32 rows x 128 bytes) while the next tile runs.
 //
 // Every mbarrier wait is bounded; on expiry the CTA sets the status word of the device and leaves.
-#include <cuda_fp8.h>
-
-#include "rows_common.cuh"
-#include "tc_common.cuh"
+#include "linear_common.cuh"
 
 namespace svoo {
 namespace tc {
 
 constexpr int kLinThreads = 384;
-constexpr int kLinRegsSums = 216, kLinRegsService = 72;       // 2 x 128 x 216 + 128 x 72 = 384 x 168
 constexpr int kLinM = 128;                                    // rows of a CTA
 constexpr int kLinBox = 32 * 128;                             // rows leave in boxes of 32 rows x 128 bytes, two per warp in flight
 constexpr int kLinScales = 8;                                 // scale blocks in flight
@@ -47,108 +43,14 @@ struct LinCfg {
   static constexpr int FULL = 0, EMPTY = FULL + kStages, ACC_FULL = EMPTY + kStages, ACC_EMPTY = ACC_FULL + 2, SC_FULL = ACC_EMPTY + 2,
                        SC_EMPTY = SC_FULL + kLinScales, BIAS_FULL = SC_EMPTY + kLinScales, BIAS_EMPTY = BIAS_FULL + 2, BARS = BIAS_EMPTY + 2;
   static constexpr int kTmemColumns = 2 * TN;
+  // registers after setmaxnreg: without spills in the warps that read TMEM (a register could be saved before it is filled)
+  static constexpr int kRegsSums = kRowScales ? 216 : 232, kRegsService = kRowScales ? 72 : 40;
+  static_assert(256 * kRegsSums + 128 * kRegsService <= kLinThreads * 168);
   static_assert(BARS * 8 + 16 <= 512 && kSmemBytes <= 232448 && kStages >= 3);
 };
+__device__ int g_linear_status;
+
 constexpr int kLinGroupM = 16;                                // row tiles that sweep the columns together
-
-__device__ int g_linear_status;                               // != 0 after a kernel gave up on a bounded wait
-
-struct LinearArgs {
-  const float *sa, *sb;
-  int64_t sa_pitch, sb_n, sb_k;                 // sa[kb * sa_pitch + m]; sb[(n / 128) * sb_n + kb * sb_k], kRowScales: sb[kb * sb_k + n]
-  const void* bias;
-  int bias_type;
-  void* out;
-  int64_t out_pitch;                            // elements
-  float* out_scale;                             // e4m3 output: [n / 128][m]
-  int64_t out_scale_pitch;
-  int M, N, K;
-  bool box_out;                                 // rows of out are whole 16-byte pieces: they leave by TMA
-};
-
-// D[tmem] (+)= A[smem] B[smem]^T, e4m3
-template <int CTAS>
-__device__ __forceinline__ void umma_e4m3(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  if constexpr (CTAS == 2)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-}
-// Arrives at the barrier (at this place in every CTA of the pair) when the issued MMAs have completed.
-template <int CTAS>
-__device__ __forceinline__ void commit_all(uint32_t bar) {
-  if constexpr (CTAS == 2)
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                 ::"r"(bar), "h"((uint16_t)3) : "memory");
-  else
-    tc_commit(bar);
-}
-// TMA load into this CTA's shared memory that signals a barrier of the pair's first CTA.
-__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t first_bar) {
-  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(first_bar) : "memory");
-}
-__device__ __forceinline__ uint32_t at_cta(uint32_t addr, int rank) {
-  uint32_t r;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void pair_sync() {
-  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-// Instruction descriptor of kind::f8f6f4: D fp32, A and B e4m3, both K-major.
-__host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N) {
-  return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
-}
-// 16 columns of this thread's row: issue, and wait for all that were issued.  The wait takes the registers as operands, so that
-// no use of theirs can be moved before it (the kernel must not spill: a register could be saved before it is filled).
-__device__ __forceinline__ void wait_columns(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
-                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) :: "memory");
-}
-// acc += {r0, r1} * f
-__device__ __forceinline__ void scale_add2(uint64_t& acc, uint32_t r0, uint32_t r1, uint64_t f) {
-  asm("{\n\t.reg .b64 a;\n\tmov.b64 a, {%1, %2};\n\tfma.rn.f32x2 %0, a, %3, %0;\n\t}\n" : "+l"(acc) : "r"(r0), "r"(r1), "l"(f));
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float half_of(uint64_t v, int i) { return __uint_as_float((uint32_t)(i ? v >> 32 : v)); }
-
-// y / 2 (1 + tanh u) = y / (1 + exp(-2 u)), u = sqrt(2 / pi) (y + 0.044715 y^3)
-__device__ __forceinline__ float gelu_tanh(float y) {
-  const float u = 0.7978845608028654f * (y + 0.044715f * y * y * y);
-  return __fdividef(y, 1.f + fast_exp2(-2.f * 1.4426950408889634f * u));
-}
-
-__device__ __forceinline__ float load_bias(const LinearArgs& a, int n) {
-  if (n >= a.N) return 0.f;
-  if (a.bias_type == SVOO_TYPE_FP32) return __ldg(static_cast<const float*>(a.bias) + n);
-  if (a.bias_type == SVOO_TYPE_BF16) return to_f32(__ldg(static_cast<const __nv_bfloat16*>(a.bias) + n));
-  return to_f32(__ldg(static_cast<const __half*>(a.bias) + n));
-}
 
 struct LinTile {
   int tm, tn;
@@ -224,7 +126,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
   pdl_wait();
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLinRegsService));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsService));
     if (warp == 0 && lane == 0) {
       // ------------------------------------------------------------------ TMA producer
       // The first CTA's FULL barrier counts the bytes of both.
@@ -321,7 +223,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
     }
   } else {
     // -------------------------------------------------------------------- sums and epilogue
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kLinRegsSums));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsSums));
     const int quad = warp & 3, half = (warp - 4) >> 2;
     const uint32_t acc_addr = tmem + ((uint32_t)(quad * 32) << 16) + half * HC;
     const float* scales = reinterpret_cast<const float*>(gen + C::kScale);
@@ -397,6 +299,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
         }
         sum[c / 2] = pack2(v[0], v[1]);
         sum[c / 2 + 1] = pack2(v[2], v[3]);
+        asm volatile("" : "+l"(sum[c / 2]), "+l"(sum[c / 2 + 1]));      // one after the other: together they would not fit the registers
       };
       // a box is written again when the store before the last has read it
       auto begin_box = [&](int i) {
@@ -420,9 +323,9 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
           for (int i = 0; i < 2; ++i)
             top = max(top, max((uint32_t)sum[c / 2 + i] & 0x7fffffffu, (uint32_t)(sum[c / 2 + i] >> 32) & 0x7fffffffu));
         }
-        float s = __fdiv_rn(__uint_as_float(top), 448.f);
-        s = s < 0x1p-126f ? 0x1p-126f : s;
+        const float s = block_scale(top);
         if (row < a.M && !skip) a.out_scale[(n0 / 128) * a.out_scale_pitch + row] = s;
+        const BlockDivide by(s);
         unsigned char* at = begin_box(n_tile);
 #pragma unroll
         for (int p = 0; p < 8; ++p) {
@@ -430,9 +333,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const uint64_t u = sum[p * 8 + 2 * i], v = sum[p * 8 + 2 * i + 1];
-            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(half_of(u, 0), s), __fdiv_rn(half_of(u, 1), s)), __NV_SATFINITE, __NV_E4M3);
-            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(half_of(v, 0), s), __fdiv_rn(half_of(v, 1), s)), __NV_SATFINITE, __NV_E4M3);
-            w[i] = lo | hi << 16;
+            w[i] = by.e4m3x4(half_of(u, 0), half_of(u, 1), half_of(v, 0), half_of(v, 1));
           }
           *reinterpret_cast<uint4*>(at + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
@@ -471,7 +372,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
   tc_fence_before();
   __syncthreads();
   if (CTAS == 2) pair_sync();
-  if (tid == 0 && *abort_flag) atomicExch(&g_linear_status, 1);
+  if (tid == 0 && *abort_flag) atomicExch(a.status, 1);
   if (warp == 1) {
     tc_fence_after();
     if constexpr (CTAS == 2)
@@ -483,13 +384,6 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
 
 }  // namespace tc
 
-struct LinearCall {
-  const void *a, *b;
-  int64_t a_pitch, b_pitch;
-  tc::LinearArgs args;
-  cudaStream_t st;
-};
-
 template <int CTAS, int TN, int OUT, bool kGelu, bool kRowScales>
 static cudaError_t launch_tiles(const LinearCall& c) {
   using C = tc::LinCfg<CTAS, TN, kRowScales>;
@@ -499,11 +393,10 @@ static cudaError_t launch_tiles(const LinearCall& c) {
       (c.args.box_out && !tc::make_out_tensor_map(&mo, OUT, c.args.out, c.args.M, c.args.N, c.args.out_pitch)))
     return cudaErrorInvalidValue;
   auto* kernel = &tc::linear_tc_kernel<CTAS, TN, OUT, kGelu, kRowScales>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+  static uint64_t done;
+  const cudaError_t e = allow_smem(kernel, C::kSmemBytes, done);
   if (e != cudaSuccess) return e;
-  int dev = 0, sms = 0;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  constexpr int sms = 148;
   const int64_t tiles = ceil_div64(c.args.M, tc::kLinM * CTAS) * ceil_div64(c.args.N, TN);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles < sms / CTAS ? tiles : sms / CTAS) * CTAS);
@@ -527,13 +420,23 @@ static cudaError_t launch_one(const LinearCall& c) {
   return launch_tiles<2, 256, OUT, kGelu, kRowScales>(c);
 }
 
-cudaError_t launch_linear_tc(const void* a, int64_t a_pitch, const float* sa, int64_t sa_pitch, const void* b, int64_t b_pitch, const float* sb,
+cudaError_t launch_linear_split(const LinearCall& c, int out_type, bool gelu, int ranks);
+
+cudaError_t launch_linear(const void* a, int64_t a_pitch, const float* sa, int64_t sa_pitch, const void* b, int64_t b_pitch, const float* sb,
                              int64_t sb_n, int64_t sb_k, bool row_scales, const void* bias, int bias_type, int64_t M, int64_t N, int64_t K,
                              bool gelu, int out_type, void* out, int64_t out_pitch, float* out_scale, int64_t out_scale_pitch, cudaStream_t st) {
   const int e = out_type == SVOO_TYPE_E4M3 ? 1 : elem_bytes(out_type);
   const bool box_out = out_pitch * e % 16 == 0 && (uintptr_t)out % 16 == 0;
   const LinearCall c{a, b, a_pitch, b_pitch,
-                     {sa, sb, sa_pitch, sb_n, sb_k, bias, bias_type, out, out_pitch, out_scale, out_scale_pitch, (int)M, (int)N, (int)K, box_out}, st};
+                     {sa, sb, sa_pitch, sb_n, sb_k, bias, bias_type, out, out_pitch, out_scale, out_scale_pitch, (int)M, (int)N, (int)K, rows_status_word(), box_out}, st};
+  if (!c.args.status) return cudaErrorInvalidDevice;
+  const int64_t small_tiles = ceil_div64(M, 128) * ceil_div64(N, 128), KB = ceil_div64(K, 128);
+  if (!row_scales && small_tiles <= 148) {
+    int64_t ranks = 148 / small_tiles;
+    ranks = ranks > 8 ? 8 : ranks;
+    ranks = ranks > KB ? KB : ranks;
+    return launch_linear_split(c, out_type, gelu, (int)ranks);
+  }
   if (row_scales) {
     switch (out_type) {
       case SVOO_TYPE_BF16: return launch_one<SVOO_TYPE_BF16, false, true>(c);
@@ -557,10 +460,21 @@ cudaError_t launch_linear_tc(const void* a, int64_t a_pitch, const float* sa, in
   }
 }
 
+int* rows_status_word() {
+  static int* words[64];                                 // per device; every thread finds the same address
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+  int* p = __atomic_load_n(&words[dev], __ATOMIC_RELAXED);
+  if (!p) {
+    if (cudaGetSymbolAddress(reinterpret_cast<void**>(&p), tc::g_linear_status) != cudaSuccess) return nullptr;
+    __atomic_store_n(&words[dev], p, __ATOMIC_RELAXED);
+  }
+  return p;
+}
+
 cudaError_t read_linear_status(int32_t* out, cudaStream_t st) {
-  void* p = nullptr;
-  cudaError_t e = cudaGetSymbolAddress(&p, tc::g_linear_status);
-  return e == cudaSuccess ? cudaMemcpyAsync(out, p, 4, cudaMemcpyDeviceToDevice, st) : e;
+  int* p = rows_status_word();
+  return p ? cudaMemcpyAsync(out, p, 4, cudaMemcpyDeviceToDevice, st) : cudaErrorInvalidDevice;
 }
 
 }  // namespace svoo

@@ -7,6 +7,7 @@
 // Everything between the loads and the stores is in 32 bits.  The variance is taken around the mean from the row in
 // registers, so a mean far from zero costs no digits.  A row whose values are not all finite comes out NaN.
 #include "rows_common.cuh"
+#include "tc_common.cuh"
 
 namespace svoo {
 
@@ -47,6 +48,8 @@ template <typename T, int V, int NV, int TPR>
 __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) layer_norm_kernel(const NormArgs a) {
   constexpr int G = TPR < 128 ? 128 / TPR : 1;
   __shared__ float slots[2][G][TPR / 32];
+  pdl_trigger();
+  pdl_wait();
   const int g = threadIdx.x / TPR, t = threadIdx.x % TPR;
   const int64_t row = (int64_t)blockIdx.x * G + g;
   if (G > 1 && row >= a.batch * a.rows) return;          // whole warps: a row is one warp there
@@ -118,6 +121,8 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) layer_norm_kernel(const
 template <typename T, int V, int NV, int TPR>
 __global__ void __launch_bounds__(TPR) layer_norm_backward_kernel(const NormArgs a) {
   __shared__ float slots[2][2][TPR / 32];
+  pdl_trigger();
+  pdl_wait();
   const int t = threadIdx.x;
   const bool per_sample = gridDim.y > 1;
   const int64_t n = per_sample ? a.rows : a.batch * a.rows;
@@ -213,19 +218,393 @@ __global__ void __launch_bounds__(TPR) layer_norm_backward_kernel(const NormArgs
   }
 }
 
+// ---- rows of whole 16-byte pieces: fetched ahead into shared memory -----------------------------------------------------
+//
+// A group of TPR threads walks rows; cp.async.bulk brings the next kStages rows of every group while one is worked on, so that what is
+// in flight does not depend on registers or on where the group is in its arithmetic.  Gain and offset lie in shared memory in 32
+// bits for the whole walk.  TPR is small: what a row costs besides its elements (two or three sums over the threads, a
+// square root, addresses: some 200 instructions a thread) is paid by every thread of it.  (A thread per eight elements, four rows at
+// a time, parameters in registers: 243 instructions per 16 bytes, 2.9 TB/s at 32,760 x 5,120.)
+constexpr int kRingThreads = 256;
+constexpr int kForwardStages = 1;                  // the row is in registers at once, so its place is free again: three cost 15 %
+constexpr int kBackwardStages = 3;                 // the row is read twice
+
+struct RingLayout {
+  int row, ring, bars, total;                     // bytes of a row; offsets
+  __host__ __device__ RingLayout(int C, int e, int param_rows, int row_tensors, int groups, int stages) {
+    row = C * e;
+    ring = param_rows * C * 4;
+    bars = ring + groups * stages * row_tensors * row;
+    total = bars + groups * stages * 8 + 16;
+  }
+};
+
+// two 32-bit numbers
+__device__ __forceinline__ uint64_t f2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float lo2(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi2(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+
+// the elements of a 16-byte piece, in pairs
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& u, uint64_t (&p)[8 / sizeof(T)]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  if constexpr (sizeof(T) == 4) {
+    p[0] = (uint64_t)w[1] << 32 | w[0];
+    p[1] = (uint64_t)w[3] << 32 | w[2];
+  } else {
+    const Vec<T, 8>& v = *reinterpret_cast<const Vec<T, 8>*>(w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = f2(to_f32(v.v[2 * i]), to_f32(v.v[2 * i + 1]));
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack(const uint64_t (&p)[8 / sizeof(T)]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      w[i] = (uint32_t)(i & 1 ? p[i / 2] >> 32 : p[i / 2]);
+    } else {
+      Vec<T, 2> v;
+      v.v[0] = from_f32<T>(lo2(p[i]));
+      v.v[1] = from_f32<T>(hi2(p[i]));
+      w[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <int TPR>
+__device__ __forceinline__ void group_sync(int group) {
+  if (TPR == 32) __syncwarp();
+  else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(TPR) : "memory");
+}
+// N sums over a group, the same in every thread.  `slot` [warps][N] is written again only behind a barrier that every
+// thread reaches when it has read it.
+template <int TPR, int N>
+__device__ __forceinline__ void group_sums(float (&s)[N], float (*slot)[N], int group) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) s[i] = warp_sum(s[i]);
+  if (TPR == 32) return;
+  if (threadIdx.x % 32 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) slot[threadIdx.x % TPR / 32][i] = s[i];
+  }
+  group_sync<TPR>(group);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    s[i] = slot[0][i];
+#pragma unroll
+    for (int w = 1; w < TPR / 32; ++w) s[i] += slot[w][i];
+  }
+}
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+// Row r of the walk of sample `sample` (per_sample) or of all samples: pointer offset in a tensor of these strides
+__device__ __forceinline__ int64_t row_offset(const NormArgs& a, bool per_sample, int sample, int r, int64_t batch_stride, int64_t row_stride) {
+  if (per_sample) return sample * batch_stride + r * row_stride;
+  if (a.batch == 1) return r * row_stride;
+  const int b = (int)((unsigned)r / (unsigned)a.rows);
+  return b * batch_stride + (r - b * a.rows) * row_stride;
+}
+
+// gain (1 + gain, 1) and offset (0) of a sample to shared memory, 32 bits
+template <typename T>
+__device__ __forceinline__ void stage_param(const NormArgs& a, const void* p, int64_t at, float add, float none, float* dst) {
+  for (int c = threadIdx.x; c < a.C; c += kRingThreads) {
+    float v = none;
+    if (p) v = add + (a.params_fp32 ? static_cast<const float*>(p)[at + c] : to_f32(static_cast<const T*>(p)[at + c]));
+    dst[c] = v;
+  }
+}
+
+// After a wait that expired, copies in flight land before the CTA ends.
+__device__ __forceinline__ void leave(uint32_t bars, int stages, int issued, int t, volatile int* abort_flag, int* status) {
+  __syncthreads();
+  if (!*abort_flag) return;
+  if (t == 0)
+    for (int i = 0; i < stages && i < issued; ++i) tc::mbar_drain(bars + 8 * i, ((issued - 1 - i) / stages) & 1);
+  if (threadIdx.x == 0) atomicExch(status, 1);
+  __syncthreads();
+}
+
+template <typename T, int NV, int TPR>
+__global__ void __launch_bounds__(kRingThreads) layer_norm_ring_kernel(const NormArgs a) {
+  constexpr int P = 8 / (int)sizeof(T), V = 2 * P, G = kRingThreads / TPR;    // pairs and elements of a piece, groups
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ float slots[2][G][TPR / 32][1];
+  const int stages = a.stages;
+  const RingLayout lay(a.C, sizeof(T), 2, 1, G, stages);
+  float* gain = reinterpret_cast<float*>(smem);
+  float* off = gain + a.C;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + lay.bars + G * stages * 8);
+  const int group = threadIdx.x / TPR, t = threadIdx.x % TPR, nvec = a.C / V;
+  const bool per_sample = gridDim.y > 1;
+  const int n = (int)(per_sample ? a.rows : a.batch * a.rows), step = gridDim.x * G, first = blockIdx.x * G + group;
+  unsigned char* ring = smem + lay.ring + group * stages * lay.row;
+  const uint32_t bars = smem_u32(smem + lay.bars) + group * stages * 8;
+  if (t == 0) {
+    for (int i = 0; i < stages; ++i) tc::mbar_init(bars + 8 * i, 1);
+    if (threadIdx.x == 0) *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  pdl_trigger();
+  pdl_wait();
+  auto fetch = [&](int r, int s) {
+    tc::mbar_expect_tx(bars + 8 * s, lay.row);
+    bulk_load(smem_u32(ring + s * lay.row), static_cast<const T*>(a.x) + row_offset(a, per_sample, blockIdx.y, r, a.x_batch, a.x_row), lay.row,
+              bars + 8 * s);
+  };
+  int ahead = first, issued = 0;                           // the next row to fetch, fetches so far (thread 0 of the group)
+  if (t == 0)
+    for (; issued < stages && ahead < n; ++issued, ahead += step) fetch(ahead, issued);
+  stage_param<T>(a, a.gain, blockIdx.y * a.gain_batch, a.plus_one ? 1.f : 0.f, 1.f, gain);
+  stage_param<T>(a, a.offset, blockIdx.y * a.offset_batch, 0.f, 0.f, off);
+  __syncthreads();
+  const float inv_c = 1.f / a.C;
+  int s = 0, phase = 0;
+  bool ok = true;
+  for (int r = first; r < n; r += step) {
+    // a wait that expires ends the stores and the fetches, not the walk: every thread meets every barrier
+    ok = tc::mbar_wait(bars + 8 * s, phase, abort_flag) && ok;
+    uint64_t d[NV][P], sum = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = i * TPR + t;
+      if (c < nvec) {
+        unpack<T>(reinterpret_cast<const uint4*>(ring + s * lay.row)[c], d[i]);
+#pragma unroll
+        for (int k = 0; k < P; ++k) sum = add2(sum, d[i][k]);
+      }
+    }
+    float one[1] = {lo2(sum) + hi2(sum)};
+    group_sums<TPR, 1>(one, slots[0][group], group);
+    if (TPR == 32) __syncwarp();
+    // the row is in everybody's registers: its place takes another
+    if (t == 0 && ahead < n && ok) {
+      fetch(ahead, s);
+      ahead += step;
+      ++issued;
+    }
+    const float mean = one[0] * inv_c;
+    const uint64_t minus = f2(-mean, -mean);
+    sum = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (i * TPR + t < nvec) {
+#pragma unroll
+        for (int k = 0; k < P; ++k) {
+          d[i][k] = add2(d[i][k], minus);
+          sum = fma2(d[i][k], d[i][k], sum);
+        }
+      }
+    }
+    one[0] = lo2(sum) + hi2(sum);
+    group_sums<TPR, 1>(one, slots[1][group], group);
+    const float rstd = 1.f / sqrtf(one[0] * inv_c + a.eps);
+    const int64_t row = per_sample ? blockIdx.y * a.rows + r : r;
+    if (t == 0 && a.mean && ok) {
+      a.mean[row] = mean;
+      a.rstd[row] = rstd;
+    }
+    const uint64_t rs = f2(rstd, rstd);
+    uint4* y = reinterpret_cast<uint4*>(static_cast<T*>(a.y) + row * a.C);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = i * TPR + t;
+      if (c < nvec) {
+        const ulonglong2* g = reinterpret_cast<const ulonglong2*>(gain + c * V);
+        const ulonglong2* o = reinterpret_cast<const ulonglong2*>(off + c * V);
+#pragma unroll
+        for (int k = 0; k < P; k += 2) {
+          const ulonglong2 gv = g[k / 2], ov = o[k / 2];
+          d[i][k] = fma2(mul2(d[i][k], rs), gv.x, ov.x);
+          d[i][k + 1] = fma2(mul2(d[i][k + 1], rs), gv.y, ov.y);
+        }
+        if (ok) y[c] = pack<T>(d[i]);
+      }
+    }
+    if (++s == stages) s = 0, phase ^= 1;
+  }
+  leave(bars, stages, issued, t, abort_flag, a.status);
+}
+
+// x and dy rows come in together.  A thread's columns are the same in every row: their sums stay in its registers.
+template <typename T, int NV, int TPR>
+__global__ void __launch_bounds__(kRingThreads < TPR ? TPR : kRingThreads) layer_norm_backward_ring_kernel(const NormArgs a) {
+  constexpr int P = 8 / (int)sizeof(T), V = 2 * P, G = kRingThreads / TPR;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ float slots[2][G][TPR / 32][2];
+  const int stages = a.stages;
+  const RingLayout lay(a.C, sizeof(T), 1, 2, G, stages);
+  float* gain = reinterpret_cast<float*>(smem);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + lay.bars + G * stages * 8);
+  const int group = threadIdx.x / TPR, t = threadIdx.x % TPR, nvec = a.C / V;
+  const bool per_sample = gridDim.y > 1;
+  const int n = (int)(per_sample ? a.rows : a.batch * a.rows), step = gridDim.x * G, first = blockIdx.x * G + group;
+  unsigned char* ring = smem + lay.ring + group * stages * 2 * lay.row;
+  const uint32_t bars = smem_u32(smem + lay.bars) + group * stages * 8;
+  if (t == 0) {
+    for (int i = 0; i < stages; ++i) tc::mbar_init(bars + 8 * i, 1);
+    if (threadIdx.x == 0) *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  pdl_trigger();
+  pdl_wait();
+  auto fetch = [&](int r, int s) {
+    const uint32_t dst = smem_u32(ring + s * 2 * lay.row);
+    tc::mbar_expect_tx(bars + 8 * s, 2 * lay.row);
+    bulk_load(dst, static_cast<const T*>(a.x) + row_offset(a, per_sample, blockIdx.y, r, a.x_batch, a.x_row), lay.row, bars + 8 * s);
+    bulk_load(dst + lay.row, static_cast<const T*>(a.dy) + row_offset(a, per_sample, blockIdx.y, r, a.dy_batch, a.dy_row), lay.row, bars + 8 * s);
+  };
+  int ahead = first, issued = 0;
+  if (t == 0)
+    for (; issued < stages && ahead < n; ++issued, ahead += step) fetch(ahead, issued);
+  stage_param<T>(a, a.gain, blockIdx.y * a.gain_batch, a.plus_one ? 1.f : 0.f, 1.f, gain);
+  __syncthreads();
+  const float inv_c = 1.f / a.C;
+  uint64_t dg[NV][P], dof[NV][P];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int k = 0; k < P; ++k) dg[i][k] = dof[i][k] = 0;
+  int s = 0, phase = 0;
+  bool ok = true;
+  const int64_t sample_row = per_sample ? blockIdx.y * a.rows : 0;
+  float mean = 0.f, rstd = 0.f;
+  if (first < n) mean = a.mean_in[sample_row + first], rstd = a.rstd_in[sample_row + first];
+  for (int r = first, turn = 0; r < n; r += step, turn ^= 1) {
+    // a wait that expires ends the stores and the fetches, not the walk: every thread meets every barrier
+    ok = tc::mbar_wait(bars + 8 * s, phase, abort_flag) && ok;
+    const uint4* xs = reinterpret_cast<const uint4*>(ring + s * 2 * lay.row);
+    const uint4* ds = reinterpret_cast<const uint4*>(ring + (s * 2 + 1) * lay.row);
+    const uint64_t rs = f2(rstd, rstd), shift = f2(-mean * rstd, -mean * rstd);       // xhat = x rstd - mean rstd
+    uint64_t s1 = 0, s2 = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = i * TPR + t;
+      if (c < nvec) {
+        uint64_t x[P], d[P];
+        unpack<T>(xs[c], x);
+        unpack<T>(ds[c], d);
+        const ulonglong2* g = reinterpret_cast<const ulonglong2*>(gain + c * V);
+#pragma unroll
+        for (int k = 0; k < P; ++k) {
+          const ulonglong2 gv = g[k / 2];
+          const uint64_t h = fma2(x[k], rs, shift), w = mul2(d[k], k & 1 ? gv.y : gv.x);
+          dg[i][k] = fma2(d[k], h, dg[i][k]);
+          dof[i][k] = add2(dof[i][k], d[k]);
+          s1 = add2(s1, w);
+          s2 = fma2(w, h, s2);
+        }
+      }
+    }
+    float sums[2] = {lo2(s1) + hi2(s1), lo2(s2) + hi2(s2)};
+    group_sums<TPR, 2>(sums, slots[turn][group], group);
+    // dx = w rstd - (s1 + xhat s2) rstd = d g rstd + (x (-s2 rstd rstd) + (mean rstd s2 - s1) rstd)
+    const float m1 = sums[0] * inv_c, m2 = sums[1] * inv_c;
+    const uint64_t a2 = f2(-m2, -m2), a1 = f2(-m1, -m1);
+    uint4* dx = reinterpret_cast<uint4*>(static_cast<T*>(a.dx) + (sample_row + r) * a.C);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = i * TPR + t;
+      if (c < nvec) {
+        uint64_t x[P], d[P];
+        unpack<T>(xs[c], x);
+        unpack<T>(ds[c], d);
+        const ulonglong2* g = reinterpret_cast<const ulonglong2*>(gain + c * V);
+#pragma unroll
+        for (int k = 0; k < P; ++k) {
+          const ulonglong2 gv = g[k / 2];
+          const uint64_t h = fma2(x[k], rs, shift);
+          d[k] = mul2(fma2(h, a2, fma2(d[k], k & 1 ? gv.y : gv.x, a1)), rs);
+        }
+        if (ok) dx[c] = pack<T>(d);
+      }
+    }
+    group_sync<TPR>(group);                                // the row has been read: its place takes another
+    if (t == 0 && ahead < n && ok) {
+      fetch(ahead, s);
+      ahead += step;
+      ++issued;
+    }
+    if (r + step < n) mean = a.mean_in[sample_row + r + step], rstd = a.rstd_in[sample_row + r + step];
+    if (++s == stages) s = 0, phase ^= 1;
+  }
+  if (a.partial) {
+    // the groups of the CTA are added in shared memory, in order
+    __syncthreads();
+    float* acc = reinterpret_cast<float*>(smem + lay.ring);                            // [dg, do][C]: fits the ring
+    for (int k = 0; k < G; ++k) {
+      if (k == group) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int c = i * TPR + t;
+          if (c < nvec) {
+            ulonglong2* p = reinterpret_cast<ulonglong2*>(acc + c * V);
+            ulonglong2* q = reinterpret_cast<ulonglong2*>(acc + a.C + c * V);
+#pragma unroll
+            for (int j = 0; j < P; j += 2) {
+              ulonglong2 u = make_ulonglong2(dg[i][j], dg[i][j + 1]), w = make_ulonglong2(dof[i][j], dof[i][j + 1]);
+              if (k > 0) {
+                const ulonglong2 pu = p[j / 2], qw = q[j / 2];
+                u = make_ulonglong2(add2(pu.x, u.x), add2(pu.y, u.y));
+                w = make_ulonglong2(add2(qw.x, w.x), add2(qw.y, w.y));
+              }
+              p[j / 2] = u;
+              q[j / 2] = w;
+            }
+          }
+        }
+      }
+      __syncthreads();
+    }
+    float* out = a.partial + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 * a.C;
+    for (int c = threadIdx.x; c < 2 * a.C; c += kRingThreads) out[c] = acc[c];
+  }
+  leave(bars, stages, issued, t, abort_flag, a.status);
+}
+
 // out0[group][c] = sum_p partial[group][p][0][c], out1 the same of [1] (gridDim.z outputs in all): 32 columns per CTA, 32
 // warps over the parts.
 template <typename T>
 __global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restrict__ partial, int parts, int C, void* out0, void* out1,
                                                           bool out_fp32) {
+  pdl_trigger();
+  pdl_wait();
   __shared__ float sums[32][33];
   const int lane = threadIdx.x % 32, w = threadIdx.x / 32;
   const int c = blockIdx.x * 32 + lane;
   const int64_t row = gridDim.z * (int64_t)C;
   const float* p = partial + (int64_t)blockIdx.y * parts * row + blockIdx.z * (int64_t)C + c;
   float s = 0.f;
-  if (c < C)
+  if (c < C) {
+#pragma unroll 4
     for (int i = w; i < parts; i += 32) s += p[i * row];
+  }
   sums[w][lane] = s;
   __syncthreads();
   if (w == 0 && c < C) {
@@ -260,9 +639,8 @@ int norm_vector(const NormArgs& a, int e) {
 template <typename T, int V, int NF, int TPR>
 cudaError_t forward(const NormArgs& a, cudaStream_t st) {
   constexpr int G = TPR < 128 ? 128 / TPR : 1;
-  layer_norm_kernel<T, V, NF / V, TPR><<<(unsigned)ceil_div64(a.batch * a.rows, G), TPR < 128 ? 128 : TPR, 0, st>>>(a);
   count_launches(1);
-  return cudaGetLastError();
+  return launch_pdl(layer_norm_kernel<T, V, NF / V, TPR>, dim3((unsigned)ceil_div64(a.batch * a.rows, G)), dim3(TPR < 128 ? 128 : TPR), 0, st, a);
 }
 template <typename T, int V>
 cudaError_t forward_v(const NormArgs& a, cudaStream_t st) {
@@ -273,7 +651,7 @@ cudaError_t forward_v(const NormArgs& a, cudaStream_t st) {
   return forward<T, V, 64, 256>(a, st);
 }
 
-constexpr int kBwdCols = 16;                       // columns per thread of the backward kernel
+constexpr int kBwdCols = 16;                       // columns per thread of the simple backward kernel
 int backward_threads(int C) {
   int t = 32;
   while (t * kBwdCols < C) t *= 2;
@@ -281,9 +659,8 @@ int backward_threads(int C) {
 }
 template <typename T, int V, int TPR>
 cudaError_t backward(const NormArgs& a, int groups, int parts, cudaStream_t st) {
-  layer_norm_backward_kernel<T, V, kBwdCols / V, TPR><<<dim3((unsigned)parts, (unsigned)groups), TPR, 0, st>>>(a);
   count_launches(1);
-  return cudaGetLastError();
+  return launch_pdl(layer_norm_backward_kernel<T, V, kBwdCols / V, TPR>, dim3((unsigned)parts, (unsigned)groups), dim3(TPR), 0, st, a);
 }
 template <typename T, int V>
 cudaError_t backward_v(const NormArgs& a, int groups, int parts, cudaStream_t st) {
@@ -296,48 +673,144 @@ cudaError_t backward_v(const NormArgs& a, int groups, int parts, cudaStream_t st
     default: return backward<T, V, 1024>(a, groups, parts, st);
   }
 }
+
+// Threads per row of the ring kernels: at most 80 elements a thread forward (75,600 x 5,120: 128 threads 306 us, 64 threads
+// 284), 40 backward (with two sums each).
+constexpr int kRingColumns = 8192;
+int ring_threads_forward(int C) { return C <= 32 * 64 ? 32 : C <= 64 * 80 ? 64 : 128; }
+int ring_threads_backward(int C) { return C <= 32 * 40 ? 32 : C <= 64 * 40 ? 64 : C <= 128 * 40 ? 128 : 256; }
+// Stages of the backward ring: three where two CTAs of them still fit an SM, else two.
+int backward_stages(int C, int e, int groups) {
+  return 2 * (RingLayout(C, e, 1, 2, groups, kBackwardStages).total + 1536) <= 232448 ? kBackwardStages : 2;
+}
+// CTAs of a kernel that the SMs hold at this much shared memory; the answer for the last size is kept.
+constexpr int kRingSmem = 200 * 1024;
+template <typename Kernel>
+cudaError_t resident(Kernel* kernel, int smem, int64_t& kept, int& ctas) {
+  const int64_t known = __atomic_load_n(&kept, __ATOMIC_RELAXED);
+  if (known >> 8 == smem) {
+    ctas = (int)(known & 255) * 148;
+    return cudaSuccess;
+  }
+  int per_sm = 0;
+  cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kRingThreads, smem);
+  if (e != cudaSuccess) return e;
+  if (per_sm < 1) return cudaErrorInvalidConfiguration;
+  ctas = per_sm * 148;
+  __atomic_store_n(&kept, (int64_t)smem << 8 | per_sm, __ATOMIC_RELAXED);
+  return cudaSuccess;
+}
+template <typename Kernel>
+cudaError_t launch_ring(Kernel* kernel, const NormArgs& a, int64_t ctas, int groups, int smem, cudaStream_t st) {
+  count_launches(1);
+  return launch_pdl(kernel, dim3((unsigned)ctas, (unsigned)groups), dim3(kRingThreads), smem, st, a);
+}
+template <typename T, int NV, int TPR>
+cudaError_t forward_ring(NormArgs a, cudaStream_t st) {
+  constexpr int G = kRingThreads / TPR;
+  static int64_t kept;
+  const int samples = a.gain_batch || a.offset_batch ? (int)a.batch : 1;
+  a.stages = kForwardStages;
+  const int smem = RingLayout(a.C, sizeof(T), 2, 1, G, a.stages).total;
+  int fit = 0;
+  static uint64_t done;
+  cudaError_t e = allow_smem(&layer_norm_ring_kernel<T, NV, TPR>, kRingSmem, done);
+  if (e == cudaSuccess) e = resident(&layer_norm_ring_kernel<T, NV, TPR>, smem, kept, fit);
+  if (e != cudaSuccess) return e;
+  const int64_t jobs = ceil_div64(samples > 1 ? a.rows : a.batch * a.rows, G), ctas = ceil_div64(fit, samples);
+  return launch_ring(&layer_norm_ring_kernel<T, NV, TPR>, a, jobs < ctas ? jobs : ctas, samples, smem, st);
+}
+template <typename T>
+cudaError_t forward_ring_t(const NormArgs& a, cudaStream_t st) {
+  constexpr int V = 16 / (int)sizeof(T), Q = 8 / V;          // pieces per 8 elements
+  const int tpr = ring_threads_forward(a.C), nv = ceil_div(a.C / V, tpr);
+  if (tpr == 32) {
+    if (nv <= 2 * Q) return forward_ring<T, 2 * Q, 32>(a, st);
+    if (nv <= 4 * Q) return forward_ring<T, 4 * Q, 32>(a, st);
+    if (nv <= 6 * Q) return forward_ring<T, 6 * Q, 32>(a, st);
+    return forward_ring<T, 8 * Q, 32>(a, st);
+  }
+  if (tpr == 64) return nv <= 6 * Q ? forward_ring<T, 6 * Q, 64>(a, st) : forward_ring<T, 10 * Q, 64>(a, st);
+  return forward_ring<T, 8 * Q, 128>(a, st);
+}
+template <typename T, int NV, int TPR>
+cudaError_t backward_ring(NormArgs a, int groups, int parts, cudaStream_t st) {
+  constexpr int G = kRingThreads / TPR;
+  a.stages = backward_stages(a.C, sizeof(T), G);
+  static uint64_t done;
+  const cudaError_t e = allow_smem(&layer_norm_backward_ring_kernel<T, NV, TPR>, kRingSmem, done);
+  if (e != cudaSuccess) return e;
+  return launch_ring(&layer_norm_backward_ring_kernel<T, NV, TPR>, a, parts, groups, RingLayout(a.C, sizeof(T), 1, 2, G, a.stages).total, st);
+}
+template <typename T>
+cudaError_t backward_ring_t(const NormArgs& a, int groups, int parts, cudaStream_t st) {
+  constexpr int V = 16 / (int)sizeof(T), Q = 8 / V;
+  const int tpr = ring_threads_backward(a.C);
+  const bool few = ceil_div(a.C / V, tpr) <= 3 * Q;
+  switch (tpr) {
+    case 32: return few ? backward_ring<T, 3 * Q, 32>(a, groups, parts, st) : backward_ring<T, 5 * Q, 32>(a, groups, parts, st);
+    case 64: return few ? backward_ring<T, 3 * Q, 64>(a, groups, parts, st) : backward_ring<T, 5 * Q, 64>(a, groups, parts, st);
+    case 128: return few ? backward_ring<T, 3 * Q, 128>(a, groups, parts, st) : backward_ring<T, 5 * Q, 128>(a, groups, parts, st);
+    default: return few ? backward_ring<T, 3 * Q, 256>(a, groups, parts, st) : backward_ring<T, 5 * Q, 256>(a, groups, parts, st);
+  }
+}
+// Rows that the ring can fetch: whole 16-byte pieces, everywhere.  (The strides of parameters do not matter to it.)
+bool ring_rows(const NormArgs& a, int e) {
+  if (a.C > kRingColumns || a.batch * a.rows > INT32_MAX - (1 << 20)) return false;
+  for (int64_t stride : {(int64_t)a.C, a.x_batch, a.x_row, a.dy_batch, a.dy_row})
+    if (stride * e % 16) return false;
+  for (const void* p : {a.x, a.dy, (const void*)a.y, (const void*)a.dx})
+    if ((uintptr_t)p % 16) return false;
+  return true;
+}
+// by type and elements per access
+#define SVOO_NORM(fn, ...)                                                                                             \
+  (type == SVOO_TYPE_BF16 ? (v == 8 ? fn<__nv_bfloat16, 8>(__VA_ARGS__) : v == 2 ? fn<__nv_bfloat16, 2>(__VA_ARGS__) : fn<__nv_bfloat16, 1>(__VA_ARGS__)) \
+   : type == SVOO_TYPE_FP16 ? (v == 8 ? fn<__half, 8>(__VA_ARGS__) : v == 2 ? fn<__half, 2>(__VA_ARGS__) : fn<__half, 1>(__VA_ARGS__))                    \
+                            : (v == 4 ? fn<float, 4>(__VA_ARGS__) : fn<float, 1>(__VA_ARGS__)))
+#define SVOO_RING(fn, ...) \
+  (type == SVOO_TYPE_BF16 ? fn<__nv_bfloat16>(__VA_ARGS__) : type == SVOO_TYPE_FP16 ? fn<__half>(__VA_ARGS__) : fn<float>(__VA_ARGS__))
 }  // namespace
 
-// CTAs per group of the backward kernel
-int norm_backward_parts(int64_t rows, int groups, int C) {
+// CTAs per group of the backward kernels: what the SMs hold at once, at most one per row (ring: per row of every group).
+int norm_backward_parts(int64_t rows, int groups, int C, bool ring) {
   const int t = backward_threads(C);
-  int64_t parts = (int64_t)148 * (t >= 1024 ? 1 : 1024 / t > 16 ? 16 : 1024 / t) / groups;
-  if (parts < 1) parts = 1;
-  return (int)(rows < parts ? (rows < 1 ? 1 : rows) : parts);
+  const int per_sm = ring ? 2 : t >= 1024 ? 1 : 1024 / t > 16 ? 16 : 1024 / t;
+  int64_t parts = (int64_t)148 * per_sm / groups, jobs = ring ? ceil_div64(rows, kRingThreads / ring_threads_backward(C)) : rows;
+  if (parts > jobs) parts = jobs;
+  return parts < 1 ? 1 : (int)parts;
+}
+// The workspace holds what either kernel leaves, so that its size does not depend on alignment.
+int64_t norm_backward_bytes(int64_t rows, int groups, int C) {
+  const int a = norm_backward_parts(rows, groups, C, false), b = norm_backward_parts(rows, groups, C, true);
+  return (int64_t)groups * (a > b ? a : b) * 2 * C * 4;
 }
 
 cudaError_t launch_layer_norm(int type, const NormArgs& a, cudaStream_t st) {
-  const int v = norm_vector(a, elem_bytes(type));
-  switch (type) {
-    case SVOO_TYPE_BF16: return v == 8 ? forward_v<__nv_bfloat16, 8>(a, st) : v == 2 ? forward_v<__nv_bfloat16, 2>(a, st) : forward_v<__nv_bfloat16, 1>(a, st);
-    case SVOO_TYPE_FP16: return v == 8 ? forward_v<__half, 8>(a, st) : v == 2 ? forward_v<__half, 2>(a, st) : forward_v<__half, 1>(a, st);
-    default: return v == 4 ? forward_v<float, 4>(a, st) : forward_v<float, 1>(a, st);
-  }
+  const int e = elem_bytes(type);
+  if (ring_rows(a, e)) return SVOO_RING(forward_ring_t, a, st);
+  const int v = norm_vector(a, e);
+  return SVOO_NORM(forward_v, a, st);
 }
 
-cudaError_t launch_layer_norm_backward(int type, const NormArgs& a, int groups, int parts, void* dgain, void* doffset, cudaStream_t st) {
-  const int v = norm_vector(a, elem_bytes(type));
-  cudaError_t e;
-  switch (type) {
-    case SVOO_TYPE_BF16: e = v == 8 ? backward_v<__nv_bfloat16, 8>(a, groups, parts, st) : v == 2 ? backward_v<__nv_bfloat16, 2>(a, groups, parts, st) : backward_v<__nv_bfloat16, 1>(a, groups, parts, st); break;
-    case SVOO_TYPE_FP16: e = v == 8 ? backward_v<__half, 8>(a, groups, parts, st) : v == 2 ? backward_v<__half, 2>(a, groups, parts, st) : backward_v<__half, 1>(a, groups, parts, st); break;
-    default: e = v == 4 ? backward_v<float, 4>(a, groups, parts, st) : backward_v<float, 1>(a, groups, parts, st);
-  }
+cudaError_t launch_layer_norm_backward(int type, const NormArgs& a, int groups, void* dgain, void* doffset, cudaStream_t st) {
+  const int elem = elem_bytes(type), v = norm_vector(a, elem);
+  const bool ring = ring_rows(a, elem);
+  const int parts = norm_backward_parts(groups > 1 ? a.rows : a.batch * a.rows, groups, a.C, ring);
+  const cudaError_t e = ring ? SVOO_RING(backward_ring_t, a, groups, parts, st) : SVOO_NORM(backward_v, a, groups, parts, st);
   if (e != cudaSuccess || !a.partial) return e;
   const dim3 grid((unsigned)ceil_div(a.C, 32), (unsigned)groups, 2);
   const bool f32 = a.params_fp32 || type == SVOO_TYPE_FP32;
-  if (type == SVOO_TYPE_FP16) column_sum_kernel<__half><<<grid, 1024, 0, st>>>(a.partial, parts, a.C, dgain, doffset, f32);
-  else column_sum_kernel<__nv_bfloat16><<<grid, 1024, 0, st>>>(a.partial, parts, a.C, dgain, doffset, f32);
   count_launches(1);
-  return cudaGetLastError();
+  return launch_pdl(type == SVOO_TYPE_FP16 ? column_sum_kernel<__half> : column_sum_kernel<__nv_bfloat16>, grid, dim3(1024), 0, st,
+                    (const float*)a.partial, parts, a.C, dgain, doffset, f32);
 }
 
 cudaError_t launch_column_sum(const float* partial, int64_t parts, int64_t C, void* out, int out_type, cudaStream_t st) {
   const dim3 grid((unsigned)ceil_div64(C, 32));
-  if (out_type == SVOO_TYPE_FP16) column_sum_kernel<__half><<<grid, 1024, 0, st>>>(partial, (int)parts, (int)C, out, nullptr, false);
-  else column_sum_kernel<__nv_bfloat16><<<grid, 1024, 0, st>>>(partial, (int)parts, (int)C, out, nullptr, out_type == SVOO_TYPE_FP32);
   count_launches(1);
-  return cudaGetLastError();
+  return launch_pdl(out_type == SVOO_TYPE_FP16 ? column_sum_kernel<__half> : column_sum_kernel<__nv_bfloat16>, grid, dim3(1024), 0, st,
+                    partial, (int)parts, (int)C, out, (void*)nullptr, out_type == SVOO_TYPE_FP32);
 }
 
 }  // namespace svoo

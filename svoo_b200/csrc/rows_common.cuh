@@ -20,6 +20,8 @@ struct NormArgs {
   int C;
   bool params_fp32, plus_one;                   // parameters in 32 bits, or in the type of x
   float eps;
+  int stages;                                   // rows that a group of the ring kernels has on their way
+  int* status;                                  // the device's word: != 0 after a kernel gave up on a bounded wait
 };
 
 // SVOO_TYPE_* -> C++ type
@@ -62,5 +64,21 @@ __device__ __forceinline__ float warp_sum(float s) {
   for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return s;
 }
+
+// Sets a kernel's dynamic shared memory limit on the current device, once: `done` is the kernel's own, a bit per device.
+template <typename Kernel>
+inline cudaError_t allow_smem(Kernel* kernel, int bytes, uint64_t& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (__atomic_load_n(&done, __ATOMIC_ACQUIRE) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) __atomic_fetch_or(&done, bit, __ATOMIC_RELEASE);
+  return e;
+}
+
+// The status word of the token-wise kernels on the current device; null after a CUDA error.
+int* rows_status_word();
 
 }  // namespace svoo

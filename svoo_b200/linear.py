@@ -68,7 +68,6 @@ def linear_fp8(x: torch.Tensor, weight: Union[torch.Tensor, Fp8Weight], bias: Op
     products in e4m3 as well: the gradient of the output is quantised in blocks along what each of them sums over, and
     rounding counts as the identity.  An Fp8Weight is a constant; with it the gradient of x needs its transpose
     (ops.quantize_blocks(w, transposed=True)).  An activation has no gradient here."""
-    lead = x.shape[:-1]
     training = torch.is_grad_enabled() and (x.requires_grad or (isinstance(weight, torch.Tensor) and weight.requires_grad) or
                                             (bias is not None and bias.requires_grad))
     m = _rows(x)
@@ -78,8 +77,8 @@ def linear_fp8(x: torch.Tensor, weight: Union[torch.Tensor, Fp8Weight], bias: Op
         y = _Linear.apply(m, weight, bias)
     else:
         w = ops.quantize_blocks(weight) if isinstance(weight, torch.Tensor) else weight
-        y = ops.mm_fp8(ops.quantize_rows(m), w, bias, activation, x.dtype)
-    return y.view(*lead, y.shape[1])
+        y = ops.linear_fp8(m, w, bias, activation)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[1])
 
 
 def mlp_fp8(x: torch.Tensor, w1: Fp8Weight, bias1: Optional[torch.Tensor], w2: Fp8Weight,
@@ -88,6 +87,6 @@ def mlp_fp8(x: torch.Tensor, w1: Fp8Weight, bias1: Optional[torch.Tensor], w2: F
     quantised from their 32-bit values as the first product leaves its registers.  Inference only."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, bias1, bias2)):
         raise ValueError("mlp_fp8 has no gradient: use two linear_fp8 around the activation")
-    h = ops.mm_fp8(ops.quantize_rows(_rows(x)), w1, bias1, "gelu", ops.E4M3)
+    h = ops.linear_fp8(_rows(x), w1, bias1, "gelu", ops.E4M3)
     y = ops.mm_fp8(h, w2, bias2, None, x.dtype)
-    return y.view(*x.shape[:-1], y.shape[1])
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[1])

@@ -545,33 +545,24 @@ _E4M3_TYPE = 3
 _ACTIVATIONS = {None: 0, "gelu": 1}
 
 
-class _OnDevice:
-    """Makes the tensors' device the current one for a call, and knows its current stream."""
-    __slots__ = ("index", "before", "stream")
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream      # what torch.cuda.current_stream(index).cuda_stream says, without its objects
 
-    def __init__(self, *tensors: Optional[torch.Tensor]):
-        index = None
-        for t in tensors:
-            if t is None:
-                continue
-            if not t.is_cuda:
-                raise ValueError("svoo_b200 ops need CUDA tensors; there is no CPU path")
-            if index is None:
-                index = t.get_device()
-            elif t.get_device() != index:
-                raise ValueError("all tensors of a call must be on one device")
-        self.index = index
 
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        self.stream = torch.cuda.current_stream().cuda_stream
-        return self
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
+def _device(*tensors: Optional[torch.Tensor]) -> int:
+    """The index of the one CUDA device that all the tensors are on."""
+    index = -1
+    for t in tensors:
+        if t is None:
+            continue
+        at = t.get_device()
+        if at < 0:
+            raise ValueError("svoo_b200 ops need CUDA tensors; there is no CPU path")
+        if index < 0:
+            index = at
+        elif at != index:
+            raise ValueError("all tensors of a call must be on one device")
+    return index
 
 
 def _ptr(t: Optional[torch.Tensor]) -> int:
@@ -581,60 +572,56 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
 def _norm_rows(x: torch.Tensor, what: str) -> Tuple[int, int, int, int]:
     """(batch, rows, batch stride, row stride) of a tensor [..., C] whose last dimension is dense: any layout with up to three
     dimensions, dense ones beyond that."""
+    shape = x.shape
+    dims = len(shape)
     if x.dtype not in TYPES:
         raise ValueError(f"{what} must be bf16, fp16 or fp32, got {x.dtype}")
-    if x.dim() < 1 or (x.shape[-1] > 1 and x.stride(-1) != 1):
-        raise ValueError(f"the last dimension of {what} must be dense")
-    C = x.shape[-1]
-    if x.dim() == 3:
-        return x.shape[0], x.shape[1], x.stride(0), x.stride(1)
-    if x.dim() == 2:
-        return 1, x.shape[0], 0, x.stride(0)
-    if x.dim() == 1:
-        return 1, 1, 0, C
-    if not x.is_contiguous():
-        raise ValueError(f"{what} with more than three dimensions must be contiguous")
-    return 1, x.numel() // C if C else 0, 0, C
+    if dims < 1:
+        raise ValueError(f"{what} needs at least one dimension")
+    C = shape[-1]
+    if x.is_contiguous():
+        if dims == 3:
+            return shape[0], shape[1], shape[1] * C, C
+        return 1, x.numel() // C if C else 0, 0, C
+    if dims > 3 or (C > 1 and x.stride(-1) != 1):
+        raise ValueError(f"the last dimension of {what} must be dense, and all of them beyond three")
+    if dims == 3:
+        return shape[0], shape[1], x.stride(0), x.stride(1)
+    return 1, shape[0], 0, x.stride(0)
 
 
-class _NormParams:
-    """Gain and offset of a layer norm, checked against x [batch, rows, C]: pointers, strides per sample, what their
-    gradients look like."""
-    __slots__ = ("gain", "offset", "gain_batch", "offset_batch", "dtype", "plus_one", "per_sample", "like")
-
-    def __init__(self, x, weight, bias, scale, shift):
-        modulated = scale is not None or shift is not None
-        if modulated and (weight is not None or bias is not None):
-            raise ValueError("a layer norm takes weight and bias, or scale and shift, not both")
-        self.gain, self.offset = (scale, shift) if modulated else (weight, bias)
-        self.plus_one = modulated
-        self.gain_batch = self.offset_batch = 0
-        self.per_sample, self.dtype, self.like = False, torch.float32, self.gain
-        if self.gain is None:
-            if self.offset is not None:
+def _norm_params(x: torch.Tensor, weight, bias, scale, shift):
+    """Checks gain and offset against x: (gain, offset, strides of both per sample, type, whether gain means 1 + gain, whether
+    there is one per sample)."""
+    if scale is None and shift is None:
+        if weight is None:
+            if bias is not None:
                 raise ValueError("bias needs weight, and shift needs scale")
-            return
-        C = x.shape[-1]
-        self.dtype = self.gain.dtype
-        if self.dtype not in (torch.float32, x.dtype):
-            raise ValueError(f"parameters must be fp32 or of the input's type, got {self.dtype}")
-        if self.offset is not None and (self.offset.dtype != self.dtype or self.offset.shape != self.gain.shape):
-            raise ValueError("both parameters must have one type and one shape")
-        shape = tuple(self.gain.shape)
-        if not modulated:
-            if shape != (C,):
-                raise ValueError(f"weight and bias must be [{C}], got {list(shape)}")
-        else:
-            B = x.shape[0] if x.dim() == 3 else 1
-            if x.dim() > 3 or shape not in ((B, 1, C), (B, C), (1, 1, C), (1, C)):
-                raise ValueError(f"scale and shift must be [B, 1, {C}] or [B, {C}] for an input [B, S, {C}], got {list(shape)}")
-            self.per_sample = shape[0] == B and B > 1
-            if self.per_sample:
-                self.gain_batch = self.gain.stride(0)
-                self.offset_batch = 0 if self.offset is None else self.offset.stride(0)
-        for p in (self.gain, self.offset):
-            if p is not None and C > 1 and p.stride(-1) != 1:
-                raise ValueError("the last dimension of every parameter must be dense")
+            return None, None, 0, 0, torch.float32, False, False
+        shape, dtype, C = weight.shape, weight.dtype, x.shape[-1]
+        if len(shape) != 1 or shape[0] != C:
+            raise ValueError(f"weight and bias must be [{C}], got {list(shape)}")
+        gain, offset, plus_one, per_sample, gb, ob = weight, bias, False, False, 0, 0
+    else:
+        if weight is not None or bias is not None:
+            raise ValueError("a layer norm takes weight and bias, or scale and shift, not both")
+        if scale is None:
+            raise ValueError("bias needs weight, and shift needs scale")
+        shape, dtype, C = tuple(scale.shape), scale.dtype, x.shape[-1]
+        B = x.shape[0] if x.dim() == 3 else 1
+        if x.dim() > 3 or shape not in ((B, 1, C), (B, C), (1, 1, C), (1, C)):
+            raise ValueError(f"scale and shift must be [B, 1, {C}] or [B, {C}] for an input [B, S, {C}], got {list(shape)}")
+        gain, offset, plus_one = scale, shift, True
+        per_sample = shape[0] == B and B > 1
+        gb = scale.stride(0) if per_sample else 0
+        ob = shift.stride(0) if per_sample and shift is not None else 0
+    if dtype is not torch.float32 and dtype is not x.dtype:
+        raise ValueError(f"parameters must be fp32 or of the input's type, got {dtype}")
+    if offset is not None and (offset.dtype is not dtype or offset.shape != gain.shape):
+        raise ValueError("both parameters must have one type and one shape")
+    if C > 1 and (gain.stride(-1) != 1 or (offset is not None and offset.stride(-1) != 1)):
+        raise ValueError("the last dimension of every parameter must be dense")
+    return gain, offset, gb, ob, dtype, plus_one, per_sample
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -645,16 +632,25 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     Statistics in 32 bits.  Returns y, dense and of x's type; with return_stats (y, mean, rstd), fp32 of the leading dimensions.
     Not differentiable by itself: see norm.layer_norm."""
     batch, rows, xb, xr = _norm_rows(x, "x")
-    p = _NormParams(x, weight, bias, scale, shift)
-    with _OnDevice(x, p.gain, p.offset) as on:
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        mean = rstd = None
-        if return_stats:
-            mean, rstd = torch.empty((2,) + x.shape[:-1], dtype=torch.float32, device=x.device)
-        check(LIB.svoo_b200_layer_norm(x.data_ptr(), TYPES[x.dtype], batch, rows, x.shape[-1], xb, xr, _ptr(p.gain), p.gain_batch,
-                                       _ptr(p.offset), p.offset_batch, TYPES[p.dtype], p.plus_one, eps, y.data_ptr(), _ptr(mean),
-                                       _ptr(rstd), on.stream), "layer_norm")
+    gain, offset, gb, ob, dtype, plus_one, _ = _norm_params(x, weight, bias, scale, shift)
+    index = _device(x, gain, offset)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return layer_norm(x, weight, bias, scale, shift, eps, return_stats)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    mean = rstd = None
+    if return_stats:
+        mean, rstd = (x.new_empty(x.shape[:-1], dtype=torch.float32) for _ in range(2))
+    check(LIB.svoo_b200_layer_norm(x.data_ptr(), TYPES[x.dtype], batch, rows, x.shape[-1], xb, xr, _ptr(gain), gb, _ptr(offset), ob,
+                                   TYPES[dtype], plus_one, eps, y.data_ptr(), _ptr(mean), _ptr(rstd), _raw_stream(index)), "layer_norm")
     return (y, mean, rstd) if return_stats else y
+
+
+@functools.lru_cache(maxsize=1024)
+def _norm_workspace_bytes(batch: int, rows: int, C: int, per_sample: bool) -> int:
+    need = ctypes.c_int64(0)
+    check(LIB.svoo_b200_layer_norm_workspace_bytes(batch, rows, C, per_sample, ctypes.byref(need)), "layer_norm_backward")
+    return need.value
 
 
 def layer_norm_backward(grad: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
@@ -665,27 +661,28 @@ def layer_norm_backward(grad: torch.Tensor, x: torch.Tensor, mean: torch.Tensor,
     batch, rows, xb, xr = _norm_rows(x, "x")
     if grad.shape != x.shape or grad.dtype != x.dtype:
         raise ValueError("the gradient must have the shape and type of x")
-    _, _, gb, gr = _norm_rows(grad, "the gradient")
+    _, _, db, dr = _norm_rows(grad, "the gradient")
     for t in (mean, rstd):
         if t.dtype != torch.float32 or t.shape != x.shape[:-1] or not t.is_contiguous():
             raise ValueError("mean and rstd must be what layer_norm returned: contiguous fp32 of x's leading dimensions")
-    p = _NormParams(x, weight, None, scale, None)
+    gain, _, gb, _, dtype, plus_one, per_sample = _norm_params(x, weight, None, scale, None)
     C = x.shape[-1]
-    with _OnDevice(x, grad, mean, rstd, p.gain) as on:
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dgain = doffset = ws = None
-        ws_bytes = 0
-        if param_grads and p.gain is not None:
-            make = torch.zeros if batch == 0 else torch.empty
-            dgain, doffset = (make(p.gain.shape, dtype=p.dtype, device=x.device) for _ in range(2))
-            need = ctypes.c_int64(0)
-            check(LIB.svoo_b200_layer_norm_workspace_bytes(batch, rows, C, p.per_sample, ctypes.byref(need)), "layer_norm_backward")
-            ws_bytes = need.value
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
-        check(LIB.svoo_b200_layer_norm_backward(grad.data_ptr(), gb, gr, x.data_ptr(), TYPES[x.dtype], batch, rows, C, xb, xr,
-                                                mean.data_ptr(), rstd.data_ptr(), _ptr(p.gain), p.gain_batch, TYPES[p.dtype],
-                                                p.plus_one, p.per_sample, dx.data_ptr(), _ptr(dgain), _ptr(doffset), _ptr(ws), ws_bytes,
-                                                on.stream), "layer_norm_backward")
+    index = _device(x, grad, mean, rstd, gain)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return layer_norm_backward(grad, x, mean, rstd, weight, scale, param_grads)
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+    dgain = doffset = ws = None
+    ws_bytes = 0
+    if param_grads and gain is not None:
+        make = gain.new_zeros if batch == 0 else gain.new_empty
+        dgain, doffset = make(gain.shape), make(gain.shape)
+        ws_bytes = _norm_workspace_bytes(batch, rows, C, per_sample)
+        ws = x.new_empty(ws_bytes, dtype=torch.uint8)
+    check(LIB.svoo_b200_layer_norm_backward(grad.data_ptr(), db, dr, x.data_ptr(), TYPES[x.dtype], batch, rows, C, xb, xr,
+                                            mean.data_ptr(), rstd.data_ptr(), _ptr(gain), gb, TYPES[dtype], plus_one, per_sample,
+                                            dx.data_ptr(), _ptr(dgain), _ptr(doffset), _ptr(ws), ws_bytes, _raw_stream(index)),
+          "layer_norm_backward")
     return dx, dgain, doffset
 
 
@@ -732,28 +729,34 @@ def _matrix(x: torch.Tensor, what: str) -> Tuple[int, int, int]:
     """(rows, columns, row stride) of a matrix with dense rows."""
     if x.dim() != 2 or x.dtype not in TYPES:
         raise ValueError(f"{what} must be a bf16, fp16 or fp32 matrix, got {x.dtype} {tuple(x.shape)}")
-    if x.shape[1] < 1 or (x.shape[1] > 1 and x.stride(1) != 1):
+    M, K = x.shape
+    if K < 1 or (K > 1 and x.stride(1) != 1):
         raise ValueError(f"{what} needs dense rows of at least one column")
-    return x.shape[0], x.shape[1], x.stride(0) if x.shape[0] > 1 else x.shape[1]
+    return M, K, x.stride(0) if M > 1 else K
 
 
 def _pad16(n: int) -> int:
-    return (n + 15) // 16 * 16
+    return (n + 15) & ~15
 
 
-def _empty_e4m3(rows: int, cols: int, device) -> torch.Tensor:
-    return torch.empty(rows, _pad16(cols), dtype=E4M3, device=device)[:, :cols]
+def _empty_e4m3(like: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
+    pitch = _pad16(cols)
+    q = like.new_empty((rows, pitch), dtype=E4M3)
+    return q if pitch == cols else q[:, :cols]
 
 
 def quantize_rows(x: torch.Tensor) -> Fp8Rows:
     """x [M, K] (bf16, fp16, fp32; dense rows) in e4m3, one scale max(amax / 448, 2^-126) per 1 x 128 block, values to the nearest.
     A block with a value that is not finite stands for NaN."""
     M, K, stride = _matrix(x, "x")
-    with _OnDevice(x) as on:
-        q = _empty_e4m3(M, K, x.device)
-        scale = torch.empty((K + 127) // 128, M, dtype=torch.float32, device=x.device)
-        check(LIB.svoo_b200_quantize_rows(x.data_ptr(), TYPES[x.dtype], M, K, stride, q.data_ptr(), _pad16(K), scale.data_ptr(), M,
-                                          on.stream), "quantize_rows")
+    index = _device(x)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return quantize_rows(x)
+    q = _empty_e4m3(x, M, K)
+    scale = x.new_empty(((K + 127) // 128, M), dtype=torch.float32)
+    check(LIB.svoo_b200_quantize_rows(x.data_ptr(), TYPES[x.dtype], M, K, stride, q.data_ptr(), _pad16(K), scale.data_ptr(), M,
+                                      _raw_stream(index)), "quantize_rows")
     return Fp8Rows(q, scale)
 
 
@@ -763,19 +766,24 @@ def quantize_columns(x: torch.Tensor, column_sum_type: Optional[torch.dtype] = N
     M, K, stride = _matrix(x, "x")
     if M < 1:
         raise ValueError("quantize_columns needs at least one row")
-    MB = (M + 127) // 128
-    with _OnDevice(x) as on:
-        q = _empty_e4m3(K, M, x.device)
-        pitch = (K + 3) // 4 * 4
-        scale = torch.empty(MB, pitch, dtype=torch.float32, device=x.device)
-        part = None if column_sum_type is None else torch.empty(MB, K, dtype=torch.float32, device=x.device)
-        check(LIB.svoo_b200_quantize_columns(x.data_ptr(), TYPES[x.dtype], M, K, stride, q.data_ptr(), _pad16(M), scale.data_ptr(), pitch,
-                                             _ptr(part), on.stream), "quantize_columns")
-        rows = Fp8Rows(q, scale[:, :K])
-        if part is None:
-            return rows
-        sums = torch.empty(K, dtype=column_sum_type, device=x.device)
-        check(LIB.svoo_b200_column_sum(part.data_ptr(), MB, K, sums.data_ptr(), TYPES[column_sum_type], on.stream), "column_sum")
+    if column_sum_type is not None and column_sum_type not in TYPES:
+        raise ValueError("column sums are bf16, fp16 or fp32")
+    index = _device(x)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return quantize_columns(x, column_sum_type)
+    MB, pitch = (M + 127) // 128, (K + 3) // 4 * 4
+    q = _empty_e4m3(x, K, M)
+    scale = x.new_empty((MB, pitch), dtype=torch.float32)
+    part = None if column_sum_type is None else x.new_empty((MB, K), dtype=torch.float32)
+    stream = _raw_stream(index)
+    check(LIB.svoo_b200_quantize_columns(x.data_ptr(), TYPES[x.dtype], M, K, stride, q.data_ptr(), _pad16(M), scale.data_ptr(), pitch,
+                                         _ptr(part), stream), "quantize_columns")
+    rows = Fp8Rows(q, scale[:, :K])
+    if part is None:
+        return rows
+    sums = x.new_empty(K, dtype=column_sum_type)
+    check(LIB.svoo_b200_column_sum(part.data_ptr(), MB, K, sums.data_ptr(), TYPES[column_sum_type], stream), "column_sum")
     return rows, sums
 
 
@@ -784,44 +792,55 @@ def quantize_blocks(w: torch.Tensor, transposed: bool = False) -> Fp8Blocks:
     N, K, stride = _matrix(w, "w")
     if N < 1:
         raise ValueError("quantize_blocks needs at least one row")
-    with _OnDevice(w) as on:
-        q = _empty_e4m3(N, K, w.device)
-        qt = _empty_e4m3(K, N, w.device) if transposed else None
-        scale = torch.empty((N + 127) // 128, (K + 127) // 128, dtype=torch.float32, device=w.device)
-        check(LIB.svoo_b200_quantize_blocks(w.data_ptr(), TYPES[w.dtype], N, K, stride, q.data_ptr(), _pad16(K), _ptr(qt), _pad16(N),
-                                            scale.data_ptr(), on.stream), "quantize_blocks")
+    index = _device(w)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return quantize_blocks(w, transposed)
+    q = _empty_e4m3(w, N, K)
+    qt = _empty_e4m3(w, K, N) if transposed else None
+    scale = w.new_empty(((N + 127) // 128, (K + 127) // 128), dtype=torch.float32)
+    check(LIB.svoo_b200_quantize_blocks(w.data_ptr(), TYPES[w.dtype], N, K, stride, q.data_ptr(), _pad16(K), _ptr(qt), _pad16(N),
+                                        scale.data_ptr(), _raw_stream(index)), "quantize_blocks")
     return Fp8Blocks(q, scale, qt)
 
 
 def _e4m3_operand(q: torch.Tensor, scale: torch.Tensor, scale_shape, what: str) -> int:
     """Pitch of an e4m3 matrix; checks it and the shape of its scales."""
-    if q.dtype != E4M3 or q.dim() != 2 or q.shape[1] < 1 or (q.shape[1] > 1 and q.stride(1) != 1):
+    if q.dtype is not E4M3 or q.dim() != 2 or q.shape[1] < 1 or (q.shape[1] > 1 and q.stride(1) != 1):
         raise ValueError(f"{what} must be an e4m3 matrix with dense rows")
     pitch = q.stride(0) if q.shape[0] > 1 else _pad16(q.shape[1])
     if pitch % 16 or pitch < q.shape[1] or q.data_ptr() % 16:
         raise ValueError(f"{what} needs rows a multiple of 16 bytes apart and a 16-byte aligned start")
-    if scale.dtype != torch.float32 or tuple(scale.shape) != scale_shape:
+    if scale.dtype is not torch.float32 or scale.shape != scale_shape:
         raise ValueError(f"the scales of {what} must be fp32 {list(scale_shape)}, got {scale.dtype} {list(scale.shape)}")
     return pitch
 
 
+def _product_output(like: torch.Tensor, M: int, N: int, bias, activation, out_dtype):
+    """Checks bias, activation and type; (out, its scales or None, pitch, type number)."""
+    if activation not in _ACTIVATIONS:
+        raise ValueError("activation must be None or 'gelu'")
+    if bias is not None and (bias.dtype not in TYPES or bias.dim() != 1 or bias.shape[0] != N or (N > 1 and bias.stride(0) != 1)):
+        raise ValueError(f"bias must be a dense [{N}] of bf16, fp16 or fp32")
+    if out_dtype is E4M3:
+        return _empty_e4m3(like, M, N), like.new_empty(((N + 127) // 128, M), dtype=torch.float32), _pad16(N), _E4M3_TYPE
+    if out_dtype not in TYPES:
+        raise ValueError("out_dtype must be bf16, fp16, fp32 or float8_e4m3fn")
+    return like.new_empty((M, N), dtype=out_dtype), None, N, TYPES[out_dtype]
+
+
 def mm_fp8(a: Fp8Rows, b, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
            out_dtype: torch.dtype = torch.bfloat16):
-    """act(a b^T + bias), sums in 32 bits: a Fp8Rows [M, K]; b Fp8Blocks [N, K], or Fp8Rows [N, K] (then neither of the next two); bias [N], bf16,
-    fp16 or fp32; activation None or "gelu" (its tanh formula).  out_dtype bf16, fp16, fp32, or float8_e4m3fn for
+    """act(a b^T + bias), sums in 32 bits: a Fp8Rows [M, K]; b Fp8Blocks [N, K], or Fp8Rows [N, K] (then neither of the next two); bias
+    [N], bf16, fp16 or fp32; activation None or "gelu" (its tanh formula).  out_dtype bf16, fp16, fp32, or float8_e4m3fn for
     the 32-bit results quantised in 1 x 128 blocks, an Fp8Rows, ready to be the next product's a."""
     M, K = a.q.shape
     N = b.q.shape[0]
     KB = (K + 127) // 128
     rows = isinstance(b, Fp8Rows)
-    if b.q.shape[1] != K:
+    if b.q.shape[1] != K or N < 1:
         raise ValueError(f"a [{M}, {K}] and b {list(b.q.shape)} do not sum over the same length")
-    if activation not in _ACTIVATIONS:
-        raise ValueError("activation must be None or 'gelu'")
-    quantised = out_dtype == E4M3
-    if not quantised and out_dtype not in TYPES:
-        raise ValueError("out_dtype must be bf16, fp16, fp32 or float8_e4m3fn")
-    if rows and (quantised or activation is not None or bias is not None):
+    if rows and (out_dtype is E4M3 or activation is not None or bias is not None):
         raise ValueError("a product of two Fp8Rows takes no bias or activation and gives no e4m3 output")
     ap = _e4m3_operand(a.q, a.scale, (KB, M), "a")
     bp = _e4m3_operand(b.q, b.scale, (KB, N) if rows else ((N + 127) // 128, KB), "b")
@@ -832,21 +851,40 @@ def mm_fp8(a: Fp8Rows, b, bias: Optional[torch.Tensor] = None, activation: Optio
         sk = (N + 3) // 4 * 4
     if rows and (N > 1 and b.scale.stride(1) != 1 or sk % 4 or sk < N or b.scale.data_ptr() % 16):
         raise ValueError("the scales of b must be dense along its rows, with a 16-byte aligned start and pitch")
-    if bias is not None and (bias.dtype not in TYPES or tuple(bias.shape) != (N,) or (N > 1 and bias.stride(0) != 1)):
-        raise ValueError(f"bias must be a dense [{N}] of bf16, fp16 or fp32")
-    with _OnDevice(a.q, a.scale, b.q, b.scale, bias) as on:
-        dev = a.q.device
-        out_scale = None
-        if quantised:
-            out = _empty_e4m3(M, N, dev)
-            out_scale = torch.empty((N + 127) // 128, M, dtype=torch.float32, device=dev)
-        else:
-            out = torch.empty(M, N, dtype=out_dtype, device=dev)
-        check(LIB.svoo_b200_mm_fp8(a.q.data_ptr(), ap, a.scale.data_ptr(), a.scale.stride(0) if KB > 1 else M, b.q.data_ptr(), bp,
-                                   b.scale.data_ptr(), sn, sk, rows, _ptr(bias), 0 if bias is None else TYPES[bias.dtype], M, N, K,
-                                   _ACTIVATIONS[activation], out.data_ptr(), _E4M3_TYPE if quantised else TYPES[out_dtype],
-                                   _pad16(N) if quantised else N, _ptr(out_scale), M, on.stream), "mm_fp8")
-    return Fp8Rows(out, out_scale) if quantised else out
+    index = _device(a.q, a.scale, b.q, b.scale, bias)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return mm_fp8(a, b, bias, activation, out_dtype)
+    out, out_scale, pitch, kind = _product_output(a.q, M, N, bias, activation, out_dtype)
+    check(LIB.svoo_b200_mm_fp8(a.q.data_ptr(), ap, a.scale.data_ptr(), a.scale.stride(0) if KB > 1 else M, b.q.data_ptr(), bp,
+                               b.scale.data_ptr(), sn, sk, rows, _ptr(bias), 0 if bias is None else TYPES[bias.dtype], M, N, K,
+                               _ACTIVATIONS[activation], out.data_ptr(), kind, pitch, _ptr(out_scale), M, _raw_stream(index)), "mm_fp8")
+    return out if out_scale is None else Fp8Rows(out, out_scale)
+
+
+def linear_fp8(x: torch.Tensor, w: Fp8Blocks, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
+               out_dtype: Optional[torch.dtype] = None):
+    """mm_fp8(quantize_rows(x), w, bias, activation, out_dtype or x's type) in one call, with the same result: x [M, K] (bf16, fp16,
+    fp32; dense rows)."""
+    M, K, stride = _matrix(x, "x")
+    q, scale = w.q, w.scale
+    N = q.shape[0]
+    KB = (K + 127) // 128
+    if q.shape[1] != K or N < 1:
+        raise ValueError(f"x [{M}, {K}] and w {list(q.shape)} do not sum over the same length")
+    wp = _e4m3_operand(q, scale, ((N + 127) // 128, KB), "w")
+    index = _device(x, q, scale, bias)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return linear_fp8(x, w, bias, activation, out_dtype)
+    out, out_scale, pitch, kind = _product_output(x, M, N, bias, activation, out_dtype or x.dtype)
+    ws_bytes = (M * _pad16(K) + 255) // 256 * 256 + KB * M * 4
+    ws = x.new_empty(ws_bytes, dtype=torch.uint8)
+    check(LIB.svoo_b200_linear_fp8(x.data_ptr(), TYPES[x.dtype], M, K, stride, q.data_ptr(), wp, scale.data_ptr(), scale.stride(0),
+                                   scale.stride(1), _ptr(bias), 0 if bias is None else TYPES[bias.dtype], N, _ACTIVATIONS[activation],
+                                   out.data_ptr(), kind, pitch, _ptr(out_scale), M, ws.data_ptr(), ws_bytes, _raw_stream(index)),
+          "linear_fp8")
+    return out if out_scale is None else Fp8Rows(out, out_scale)
 
 
 def linear_status(device: torch.device) -> int:
