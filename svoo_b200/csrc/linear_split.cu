@@ -21,8 +21,9 @@ constexpr int kSplitScaleFloats = kSplitM + 4;
 constexpr int kSplitData = kSplitStages * kSplitStageBytes, kSplitBars = kSplitData + kSplitScales * kSplitScaleFloats * 4;
 constexpr int kSplitSmem = kSplitBars + 512 + 1024;
 static_assert(kSplitM * kSplitN * 4 <= kSplitData, "the sums of the tile take the place of the operands");
-enum { SPL_FULL = 0, SPL_EMPTY = SPL_FULL + kSplitStages, SPL_ACC_FULL = SPL_EMPTY + kSplitStages, SPL_ACC_EMPTY = SPL_ACC_FULL + 2,
-       SPL_SC_FULL = SPL_ACC_EMPTY + 2, SPL_SC_EMPTY = SPL_SC_FULL + kSplitScales, SPL_BARS = SPL_SC_EMPTY + kSplitScales };
+constexpr int kSplitAcc = 2;                                  // accumulators (four are no faster)
+enum { SPL_FULL = 0, SPL_EMPTY = SPL_FULL + kSplitStages, SPL_ACC_FULL = SPL_EMPTY + kSplitStages, SPL_ACC_EMPTY = SPL_ACC_FULL + kSplitAcc,
+       SPL_SC_FULL = SPL_ACC_EMPTY + kSplitAcc, SPL_SC_EMPTY = SPL_SC_FULL + kSplitScales, SPL_BARS = SPL_SC_EMPTY + kSplitScales };
 
 __device__ __forceinline__ float4 load_cluster(uint32_t addr) {
   float4 v;
@@ -46,13 +47,17 @@ __global__ void __launch_bounds__(kSplitThreads, 1) linear_split_kernel(const __
   auto bar = [&](int i) { return bars + 8u * i; };
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int row0 = tm * kSplitM, n0 = tn * kSplitN;
+  if (tid == 32) {
+    prefetch_map(&tm_a);
+    prefetch_map(&tm_b);
+  }
   if (tid == 0) {
     for (int i = 0; i < SPL_BARS; ++i) mbar_init(bar(i), i >= SPL_SC_EMPTY ? 8 : i >= SPL_SC_FULL ? 32 : i >= SPL_ACC_EMPTY ? 8 : 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(2 * kSplitN) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kSplitAcc * kSplitN) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_trigger();
@@ -78,9 +83,9 @@ __global__ void __launch_bounds__(kSplitThreads, 1) linear_split_kernel(const __
         if (it > s) mbar_drain(bar(SPL_FULL + s), ((it - 1 - s) / kSplitStages) & 1);
   } else if (warp == 1 && lane == 0) {
     for (int it = 0; it < kb1 - kb0; ++it) {
-      const int s = it % kSplitStages, b = it & 1;
+      const int s = it % kSplitStages, b = it % kSplitAcc;
       if (!mbar_wait(bar(SPL_FULL + s), (it / kSplitStages) & 1, abort_flag)) break;
-      if (!mbar_wait(bar(SPL_ACC_EMPTY + b), ((it >> 1) & 1) ^ 1, abort_flag)) break;
+      if (!mbar_wait(bar(SPL_ACC_EMPTY + b), ((it / kSplitAcc) & 1) ^ 1, abort_flag)) break;
       tc_fence_after();
       const uint32_t as = base + s * kSplitStageBytes, bs = as + kSplitM * 128;
 #pragma unroll
@@ -113,9 +118,9 @@ __global__ void __launch_bounds__(kSplitThreads, 1) linear_split_kernel(const __
     for (int i = 0; i < 32; ++i) sum[i] = 0;
 #pragma unroll 1
     for (int it = 0; it < kb1 - kb0; ++it) {
-      const int b = it & 1, sl = it % kSplitScales;
+      const int b = it % kSplitAcc, sl = it % kSplitScales;
       if (!__all_sync(0xffffffffu, mbar_wait(bar(SPL_SC_FULL + sl), (it / kSplitScales) & 1, abort_flag) &&
-                                       mbar_wait(bar(SPL_ACC_FULL + b), (it >> 1) & 1, abort_flag)))
+                                       mbar_wait(bar(SPL_ACC_FULL + b), (it / kSplitAcc) & 1, abort_flag)))
         break;
       tc_fence_after();
       const float* sc = reinterpret_cast<const float*>(gen + kSplitData) + sl * kSplitScaleFloats;
@@ -157,11 +162,14 @@ __global__ void __launch_bounds__(kSplitThreads, 1) linear_split_kernel(const __
   const int r1 = rows * (rank + 1) / ranks;
   for (int r = rows * rank / ranks + warp; r < r1; r += kSplitThreads / 32) {
     const uint32_t at = base + r * kSplitN * 4 + ((lane ^ (r & 31)) << 4);
+    float4 part[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < ranks) part[k] = load_cluster(at_cta(at, k));
     float v[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < ranks; ++k) {
-      const float4 t = load_cluster(at_cta(at, k));
-      v[0] += t.x, v[1] += t.y, v[2] += t.z, v[3] += t.w;
-    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < ranks) v[0] += part[k].x, v[1] += part[k].y, v[2] += part[k].z, v[3] += part[k].w;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       v[i] += bias[i];
@@ -194,7 +202,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) linear_split_kernel(const __
   if (tid == 0 && *abort_flag) atomicExch(a.status, 1);
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kSplitN) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kSplitAcc * kSplitN) : "memory");
   }
 }
 
@@ -225,6 +233,43 @@ static cudaError_t launch_split_one(const LinearCall& c, int ranks) {
   cfg.numAttrs = 2;
   count_launches(1);
   return cudaLaunchKernelEx(&cfg, kernel, ma, mb, c.args);
+}
+
+// Clusters of each size that the device holds at once (a cluster stays inside one GPC, so sizes that do not divide one leave SMs
+// idle); asked for once per device.
+static int clusters_of(int ranks) {
+  static int known[64][9];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 0;
+  int n = __atomic_load_n(&known[dev][ranks], __ATOMIC_RELAXED);
+  if (n == 0) {
+    auto* kernel = &tc::linear_split_kernel<SVOO_TYPE_BF16, false>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tc::kSplitSmem) != cudaSuccess) return 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ranks, 148);
+    cfg.blockDim = dim3(tc::kSplitThreads);
+    cfg.dynamicSmemBytes = tc::kSplitSmem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)ranks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) return 0;
+    __atomic_store_n(&known[dev][ranks], n < 1 ? -1 : n, __ATOMIC_RELAXED);
+  }
+  return n < 0 ? 0 : n;
+}
+
+// CTAs per tile: as many as run at once, each with two blocks of k or more; 0 where the tiles alone fill the device.
+// us for 40 tiles of 5,120 columns, 40 blocks: 18.2 / 12.3 / 11.3 with 1 / 2 / 3 CTAs, 15.3 with 4 (two rounds);
+// 21 tiles, 8 blocks (333 x 777 x 1,000): 9.4 / 7.4 / 7.1 / 6.5 with 1 / 2 / 3 / 4, 13.9 with 7;
+// 9 tiles, 63 blocks (300 x 300 x 8,000): 28.7 / 17.1 / 13.2 / 11.2 / 10.0 / 9.0 with 1 / 2 / 3 / 4 / 6 / 8.
+int linear_split_ranks(int64_t tiles, int64_t blocks) {
+  if (tiles > 148) return 0;
+  int ranks = 8;
+  while (ranks > 1 && (ranks * 2 > blocks || tiles > clusters_of(ranks))) --ranks;
+  return ranks;
 }
 
 cudaError_t launch_linear_split(const LinearCall& c, int out_type, bool gelu, int ranks) {

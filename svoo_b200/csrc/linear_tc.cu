@@ -102,6 +102,11 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + C::kBars + C::BARS * 8 + 8);
   auto bar = [&](int i) { return bars + 8u * i; };
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  if (tid == 32) {
+    prefetch_map(&tm_a);
+    prefetch_map(&tm_b);
+    if (a.box_out) prefetch_map(&tm_out);
+  }
   if (tid == 0) {
     for (int i = 0; i < C::BARS; ++i)
       mbar_init(bar(i), i >= C::BIAS_EMPTY ? 8 : i >= C::BIAS_FULL ? 32 : i >= C::SC_EMPTY ? 8 : i >= C::SC_FULL ? 32 : i >= C::ACC_EMPTY ? 8 * CTAS : 1);
@@ -420,6 +425,7 @@ static cudaError_t launch_one(const LinearCall& c) {
   return launch_tiles<2, 256, OUT, kGelu, kRowScales>(c);
 }
 
+int linear_split_ranks(int64_t tiles, int64_t blocks);
 cudaError_t launch_linear_split(const LinearCall& c, int out_type, bool gelu, int ranks);
 
 cudaError_t launch_linear(const void* a, int64_t a_pitch, const float* sa, int64_t sa_pitch, const void* b, int64_t b_pitch, const float* sb,
@@ -430,12 +436,9 @@ cudaError_t launch_linear(const void* a, int64_t a_pitch, const float* sa, int64
   const LinearCall c{a, b, a_pitch, b_pitch,
                      {sa, sb, sa_pitch, sb_n, sb_k, bias, bias_type, out, out_pitch, out_scale, out_scale_pitch, (int)M, (int)N, (int)K, rows_status_word(), box_out}, st};
   if (!c.args.status) return cudaErrorInvalidDevice;
-  const int64_t small_tiles = ceil_div64(M, 128) * ceil_div64(N, 128), KB = ceil_div64(K, 128);
-  if (!row_scales && small_tiles <= 148) {
-    int64_t ranks = 148 / small_tiles;
-    ranks = ranks > 8 ? 8 : ranks;
-    ranks = ranks > KB ? KB : ranks;
-    return launch_linear_split(c, out_type, gelu, (int)ranks);
+  if (!row_scales) {
+    const int ranks = linear_split_ranks(ceil_div64(M, 128) * ceil_div64(N, 128), ceil_div64(K, 128));
+    if (ranks) return launch_linear_split(c, out_type, gelu, ranks);
   }
   if (row_scales) {
     switch (out_type) {
