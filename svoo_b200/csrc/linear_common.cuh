@@ -96,11 +96,51 @@ __device__ __forceinline__ uint64_t pack2(float a, float b) {
 }
 __device__ __forceinline__ float half_of(uint64_t v, int i) { return __uint_as_float((uint32_t)(i ? v >> 32 : v)); }
 
-// y / 2 (1 + tanh u) = y / (1 + exp(-2 u)), u = sqrt(2 / pi) (y + 0.044715 y^3)
-__device__ __forceinline__ float gelu_tanh(float y) {
-  const float u = 0.7978845608028654f * (y + 0.044715f * y * y * y);
-  return __fdividef(y, 1.f + fast_exp2(-2.f * 1.4426950408889634f * u));
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// GELU of two values: y / 2 (1 + tanh u) = y / (1 + exp(-2 u)), u = sqrt(2 / pi) (y + 0.044715 y^3).  The special-function unit is
+// what it costs most on: the two share a reciprocal (1 / d0 = d1 / (d0 d1)); exponents are cut at 60, where GELU is below 2^-57,
+// so that the product stays finite.
+__device__ __forceinline__ uint64_t gelu2(uint64_t y) {
+  constexpr float k = -2.f * 0.7978845608028654f * 1.4426950408889634f;
+  const uint64_t a = mul2(y, fma2(mul2(y, y), pack2(0.044715f * k, 0.044715f * k), pack2(k, k)));
+  const uint64_t d = add2(pack2(fast_exp2(fminf(half_of(a, 0), 60.f)), fast_exp2(fminf(half_of(a, 1), 60.f))), pack2(1.f, 1.f));
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(half_of(d, 0) * half_of(d, 1)));
+  return mul2(y, mul2(pack2(half_of(d, 1), half_of(d, 0)), pack2(r, r)));
+}
+// the largest of three magnitudes; NaN if one is
+__device__ __forceinline__ float max_magnitude(float top, uint64_t v) {
+  asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(fabsf(half_of(v, 0))), "f"(fabsf(half_of(v, 1))));
+  return top;
+}
+// x / s of values that are themselves rounded sums: one correction by the remainder, which leaves half a unit and 2^-22 of
+// one (BlockDivide makes it half a unit).  The scale as block_scale gives it.
+struct BlockDivideOnce {
+  uint64_t y, ns;
+  float up;
+  __device__ __forceinline__ explicit BlockDivideOnce(float s) {
+    const BlockDivide d(s);
+    y = pack2(d.y, d.y), ns = pack2(d.ns, d.ns), up = d.up;
+  }
+  __device__ __forceinline__ uint64_t quotient(uint64_t x) const {
+    if (up != 1.f) x = mul2(x, pack2(up, up));
+    const uint64_t q = mul2(x, y);
+    return fma2(fma2(q, ns, x), y, q);
+  }
+  __device__ __forceinline__ uint32_t e4m3x4(uint64_t a, uint64_t b) const {
+    a = quotient(a), b = quotient(b);
+    return e4m3x2(half_of(a, 0), half_of(a, 1)) | e4m3x2(half_of(b, 0), half_of(b, 1)) << 16;
+  }
+};
 
 __device__ __forceinline__ float load_bias(const LinearArgs& a, int n) {
   if (n >= a.N) return 0.f;

@@ -171,9 +171,13 @@ __global__ void __launch_bounds__(kSplitThreads, 1) linear_split_kernel(const __
     for (int k = 0; k < 8; ++k)
       if (k < ranks) v[0] += part[k].x, v[1] += part[k].y, v[2] += part[k].z, v[3] += part[k].w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] += bias[i];
-      if (kGelu) v[i] = gelu_tanh(v[i]);
+    for (int i = 0; i < 4; ++i) v[i] += bias[i];
+    if (kGelu) {
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        const uint64_t g = gelu2(pack2(v[i], v[i + 1]));
+        v[i] = half_of(g, 0), v[i + 1] = half_of(g, 1);
+      }
     }
     if constexpr (OUT == SVOO_TYPE_E4M3) {
       uint32_t top = max(max(magnitude(v[0]), magnitude(v[1])), max(magnitude(v[2]), magnitude(v[3])));
@@ -182,7 +186,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) linear_split_kernel(const __
       const float s = block_scale(top);
       if (lane == 0) a.out_scale[tn * a.out_scale_pitch + row0 + r] = s;
       if (n < ((a.N + 15) & ~15))
-        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + (int64_t)(row0 + r) * a.out_pitch + n) = BlockDivide(s).e4m3x4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + (int64_t)(row0 + r) * a.out_pitch + n) = BlockDivideOnce(s).e4m3x4(pack2(v[0], v[1]), pack2(v[2], v[3]));
     } else {
       typedef typename ElemOf<OUT>::T T;
       T* dst = static_cast<T*>(a.out) + (int64_t)(row0 + r) * a.out_pitch + n;

@@ -294,17 +294,17 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
       const bool skip = n0 >= a.N || row0 >= a.M;
       // four columns at a time
       auto finish4 = [&](int c) {
-        float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (has_bias)                                      // volatile: all of them at once would not fit the registers
-          asm volatile("ld.volatile.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(b.x), "=f"(b.y), "=f"(b.z), "=f"(b.w) : "r"(bias + c * 4));
-        float v[4] = {half_of(sum[c / 2], 0) + b.x, half_of(sum[c / 2], 1) + b.y, half_of(sum[c / 2 + 1], 0) + b.z, half_of(sum[c / 2 + 1], 1) + b.w};
-        if (kGelu) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = gelu_tanh(v[i]);
+        uint64_t u = sum[c / 2], v = sum[c / 2 + 1];
+        if (has_bias) {                                    // volatile: all of them at once would not fit the registers
+          uint64_t bu, bv;
+          asm volatile("ld.volatile.shared.v2.b64 {%0, %1}, [%2];" : "=l"(bu), "=l"(bv) : "r"(bias + c * 4));
+          u = add2(u, bu);
+          v = add2(v, bv);
         }
-        sum[c / 2] = pack2(v[0], v[1]);
-        sum[c / 2 + 1] = pack2(v[2], v[3]);
-        asm volatile("" : "+l"(sum[c / 2]), "+l"(sum[c / 2 + 1]));      // one after the other: together they would not fit the registers
+        if (kGelu) u = gelu2(u), v = gelu2(v);
+        sum[c / 2] = u;
+        sum[c / 2 + 1] = v;
+        asm volatile("" : "+l"(sum[c / 2]), "+l"(sum[c / 2 + 1]));      // one after the other: together they would not fit either
       };
       // a box is written again when the store before the last has read it
       auto begin_box = [&](int i) {
@@ -320,25 +320,22 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
       if constexpr (OUT == SVOO_TYPE_E4M3) {
         // the thread's 128 columns are one block of its row; columns behind N are zero
         static_assert(HC == 128);
-        uint32_t top = 0;
+        float top = 0.f;
 #pragma unroll
         for (int c = 0; c < HC; c += 4) {
           finish4(c);
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            top = max(top, max((uint32_t)sum[c / 2 + i] & 0x7fffffffu, (uint32_t)(sum[c / 2 + i] >> 32) & 0x7fffffffu));
+          top = max_magnitude(max_magnitude(top, sum[c / 2]), sum[c / 2 + 1]);
         }
-        const float s = block_scale(top);
+        const float s = block_scale(__float_as_uint(top) & 0x7fffffffu);
         if (row < a.M && !skip) a.out_scale[(n0 / 128) * a.out_scale_pitch + row] = s;
-        const BlockDivide by(s);
+        const BlockDivideOnce by(s);
         unsigned char* at = begin_box(n_tile);
 #pragma unroll
         for (int p = 0; p < 8; ++p) {
           uint32_t w[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint64_t u = sum[p * 8 + 2 * i], v = sum[p * 8 + 2 * i + 1];
-            w[i] = by.e4m3x4(half_of(u, 0), half_of(u, 1), half_of(v, 0), half_of(v, 1));
+            w[i] = by.e4m3x4(sum[p * 8 + 2 * i], sum[p * 8 + 2 * i + 1]);
           }
           *reinterpret_cast<uint4*>(at + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
