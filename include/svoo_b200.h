@@ -417,12 +417,16 @@ int svoo_b200_layer_norm_backward(const void* dy, int64_t dy_batch, int64_t dy_r
  *   rows:    blocks along K.  q [M, q_pitch], scale[kb * scale_pitch + m], kb < ceil(K / 128), scale_pitch >= M
  *   columns: blocks along M of the transpose.  q [K, q_pitch >= M], scale[mb * scale_pitch + k]; column_sums, if given, receives
  *            fp32 [ceil(M / 128), K] sums of each 128 rows, which svoo_b200_column_sum adds
+ *   both:    rows (q, scale) and columns (qt, scale_t, column_sums) from one reading of x
  *   blocks:  squares of 128 x 128.  q [M, q_pitch], scale [ceil(M / 128), ceil(K / 128)]; qt, if given, is the transpose of q,
  *            [K, qt_pitch >= M] */
 int svoo_b200_quantize_rows(const void* x, int32_t x_type, int64_t M, int64_t K, int64_t x_row, void* q, int64_t q_pitch, float* scale,
                             int64_t scale_pitch, void* stream);
 int svoo_b200_quantize_columns(const void* x, int32_t x_type, int64_t M, int64_t K, int64_t x_row, void* q, int64_t q_pitch,
                                float* scale, int64_t scale_pitch, float* column_sums, void* stream);
+int svoo_b200_quantize_both(const void* x, int32_t x_type, int64_t M, int64_t K, int64_t x_row, void* q, int64_t q_pitch, float* scale,
+                            int64_t scale_pitch, void* qt, int64_t qt_pitch, float* scale_t, int64_t scale_t_pitch,
+                            float* column_sums, void* stream);
 int svoo_b200_quantize_blocks(const void* x, int32_t x_type, int64_t M, int64_t K, int64_t x_row, void* q, int64_t q_pitch, void* qt,
                               int64_t qt_pitch, float* scale, void* stream);
 /* out[c] = sum over parts of partial[part][c] (fp32 [parts, C]), out of out_type. */

@@ -90,6 +90,8 @@ SIGNATURES = {
                                         c_void_p]),
     "svoo_b200_quantize_columns": (c_int, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64,
                                            c_void_p, c_void_p]),
+    "svoo_b200_quantize_both": (c_int, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                                        c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
     "svoo_b200_quantize_blocks": (c_int, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64,
                                           c_void_p, c_void_p]),
     "svoo_b200_column_sum": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int32, c_void_p]),

@@ -10,6 +10,9 @@ cudaError_t launch_quantize_rows(int type, const void* x, int64_t M, int64_t K, 
                                  int64_t scale_pitch, cudaStream_t st);
 cudaError_t launch_quantize_columns(int type, const void* x, int64_t M, int64_t K, int64_t row_stride, void* qt, int64_t qt_pitch,
                                     float* scale, int64_t scale_pitch, float* column_sum, cudaStream_t st);
+cudaError_t launch_quantize_both(int type, const void* x, int64_t M, int64_t K, int64_t row_stride, void* q, int64_t q_pitch, float* scale,
+                                 int64_t scale_pitch, void* qt, int64_t qt_pitch, float* scale_t, int64_t scale_t_pitch, float* column_sum,
+                                 cudaStream_t st);
 cudaError_t launch_quantize_blocks(int type, const void* w, int64_t N, int64_t K, int64_t row_stride, void* q, int64_t q_pitch, void* qt,
                                    int64_t qt_pitch, float* scale, cudaStream_t st);
 cudaError_t launch_linear(const void* a, int64_t a_pitch, const float* sa, int64_t sa_pitch, const void* b, int64_t b_pitch, const float* sb,
@@ -129,6 +132,7 @@ int svoo_b200_quantize_columns(const void* x, int32_t x_type, int64_t M, int64_t
                                float* scale, int64_t scale_pitch, float* column_sums, void* stream) {
   SVOO_TRY(check_quant(x, x_type, M, K, x_row, q, q_pitch, M, scale));
   if (scale_pitch < K || ceil_div64(M, 128) > 65535) return SVOO_ERR_SHAPE;
+  if (column_sums && !aligned(column_sums, 4)) return SVOO_ERR_ALIGN;
   if (M == 0) return SVOO_OK;
   return (int)launch_quantize_columns(x_type, x, M, K, x_row, q, q_pitch, scale, scale_pitch, column_sums, (cudaStream_t)stream);
 }
@@ -140,6 +144,18 @@ int svoo_b200_quantize_blocks(const void* x, int32_t x_type, int64_t M, int64_t 
   if (qt && !aligned(qt, 16)) return SVOO_ERR_ALIGN;
   if (M == 0) return SVOO_OK;
   return (int)launch_quantize_blocks(x_type, x, M, K, x_row, q, q_pitch, qt, qt_pitch, scale, (cudaStream_t)stream);
+}
+
+int svoo_b200_quantize_both(const void* x, int32_t x_type, int64_t M, int64_t K, int64_t x_row, void* q, int64_t q_pitch, float* scale,
+                            int64_t scale_pitch, void* qt, int64_t qt_pitch, float* scale_t, int64_t scale_t_pitch, float* column_sums,
+                            void* stream) {
+  SVOO_TRY(check_quant(x, x_type, M, K, x_row, q, q_pitch, K, scale));
+  SVOO_TRY(check_quant(x, x_type, M, K, x_row, qt, qt_pitch, M, scale_t));
+  if (scale_pitch < M || scale_t_pitch < K || ceil_div64(M, 128) > 65535) return SVOO_ERR_SHAPE;
+  if (column_sums && !aligned(column_sums, 4)) return SVOO_ERR_ALIGN;
+  if (M == 0) return SVOO_OK;
+  return (int)launch_quantize_both(x_type, x, M, K, x_row, q, q_pitch, scale, scale_pitch, qt, qt_pitch, scale_t, scale_t_pitch, column_sums,
+                                   (cudaStream_t)stream);
 }
 
 int svoo_b200_column_sum(const float* partial, int64_t parts, int64_t C, void* out, int32_t out_type, void* stream) {

@@ -111,11 +111,13 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 // so that the product stays finite.
 __device__ __forceinline__ uint64_t gelu2(uint64_t y) {
   constexpr float k = -2.f * 0.7978845608028654f * 1.4426950408889634f;
-  const uint64_t a = mul2(y, fma2(mul2(y, y), pack2(0.044715f * k, 0.044715f * k), pack2(k, k)));
-  const uint64_t d = add2(pack2(fast_exp2(fminf(half_of(a, 0), 60.f)), fast_exp2(fminf(half_of(a, 1), 60.f))), pack2(1.f, 1.f));
+  // constants in scalar operations: a pair of each would take registers that the epilogue does not have
+  const uint64_t z = mul2(y, y);
+  const uint64_t a = mul2(y, pack2(fmaf(half_of(z, 0), 0.044715f * k, k), fmaf(half_of(z, 1), 0.044715f * k, k)));
+  const float d[2] = {1.f + fast_exp2(fminf(half_of(a, 0), 60.f)), 1.f + fast_exp2(fminf(half_of(a, 1), 60.f))};
   float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(half_of(d, 0) * half_of(d, 1)));
-  return mul2(y, mul2(pack2(half_of(d, 1), half_of(d, 0)), pack2(r, r)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d[0] * d[1]));
+  return mul2(y, mul2(pack2(d[1], d[0]), pack2(r, r)));
 }
 // the largest of three magnitudes; NaN if one is
 __device__ __forceinline__ float max_magnitude(float top, uint64_t v) {

@@ -292,19 +292,20 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
       if (has_bias) ok = __all_sync(0xffffffffu, mbar_wait(bar(C::BIAS_FULL + (n_tile & 1)), (n_tile >> 1) & 1, abort_flag));
       if (!ok) break;
       const bool skip = n0 >= a.N || row0 >= a.M;
-      // four columns at a time
+      // four columns at a time, the bias of the next four on its way (volatile: all of it at once would not fit the registers)
+      uint64_t ahead[2] = {0, 0};
+      auto bias4 = [&](int c) {
+        if (has_bias && c < HC)
+          asm volatile("ld.volatile.shared.v2.b64 {%0, %1}, [%2];" : "=l"(ahead[0]), "=l"(ahead[1]) : "r"(bias + c * 4));
+      };
+      bias4(0);
       auto finish4 = [&](int c) {
-        uint64_t u = sum[c / 2], v = sum[c / 2 + 1];
-        if (has_bias) {                                    // volatile: all of them at once would not fit the registers
-          uint64_t bu, bv;
-          asm volatile("ld.volatile.shared.v2.b64 {%0, %1}, [%2];" : "=l"(bu), "=l"(bv) : "r"(bias + c * 4));
-          u = add2(u, bu);
-          v = add2(v, bv);
-        }
-        if (kGelu) u = gelu2(u), v = gelu2(v);
-        sum[c / 2] = u;
-        sum[c / 2 + 1] = v;
-        asm volatile("" : "+l"(sum[c / 2]), "+l"(sum[c / 2 + 1]));      // one after the other: together they would not fit either
+        uint64_t v[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) v[i] = has_bias ? add2(sum[c / 2 + i], ahead[i]) : sum[c / 2 + i];
+        bias4(c + 4);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) sum[c / 2 + i] = kGelu ? gelu2(v[i]) : v[i];
       };
       // a box is written again when the store before the last has read it
       auto begin_box = [&](int i) {
@@ -324,7 +325,8 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
 #pragma unroll
         for (int c = 0; c < HC; c += 4) {
           finish4(c);
-          top = max_magnitude(max_magnitude(top, sum[c / 2]), sum[c / 2 + 1]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) top = max_magnitude(top, sum[c / 2 + i]);
         }
         const float s = block_scale(__float_as_uint(top) & 0x7fffffffu);
         if (row < a.M && !skip) a.out_scale[(n0 / 128) * a.out_scale_pitch + row] = s;

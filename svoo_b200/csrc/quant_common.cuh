@@ -44,13 +44,26 @@ struct BlockDivide {
     up = s < 0x1p-90f ? 0x1p64f : 1.f;
     ns = s == INFINITY ? -1.f : -s * up;
   }
+  // Of x that are 16-bit numbers, as is the amax that s came from, q1 is enough: it is off the rounded quotient only
+  // where x / s lies within 2^-46 of the middle of two 32-bit numbers, and e4m3 tells that only beside its ties, 32-bit numbers t
+  // of five bits.  x = t s (1 +- 2^-24) has no solution in x of 11 bits but t = 2^-10, x a power of two and s one step
+  // below another, which no amax of 11 bits over 448 is.
+  template <bool kOnce = false>
   __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) const {
     if (up != 1.f) a *= up, b *= up, c *= up, d *= up;
-    pair(a, b);
-    pair(c, d);
+    pair<kOnce>(a, b);
+    pair<kOnce>(c, d);
     return e4m3x2(a, b) | e4m3x2(c, d) << 16;
   }
+  template <bool kOnce>
   __device__ __forceinline__ void pair(float& a, float& b) const {
+    if constexpr (kOnce) {
+      asm("{\n\t.reg .b64 x, ns, y, q, r;\n\t"
+          "mov.b64 x, {%0, %1};\n\tmov.b64 ns, {%2, %2};\n\tmov.b64 y, {%3, %3};\n\t"
+          "mul.rn.f32x2 q, x, y;\n\tfma.rn.f32x2 r, q, ns, x;\n\tfma.rn.f32x2 q, r, y, q;\n\t"
+          "mov.b64 {%0, %1}, q;\n\t}\n" : "+f"(a), "+f"(b) : "f"(ns), "f"(y));
+      return;
+    }
     asm("{\n\t.reg .b64 x, ns, y, q, r;\n\t"
         "mov.b64 x, {%0, %1};\n\tmov.b64 ns, {%2, %2};\n\tmov.b64 y, {%3, %3};\n\t"
         "mul.rn.f32x2 q, x, y;\n\t"

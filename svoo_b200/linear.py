@@ -25,39 +25,56 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
-        a = ops.quantize_rows(x)
-        if isinstance(weight, torch.Tensor):
-            w = ops.quantize_blocks(weight, transposed=ctx.needs_input_grad[0])
+        need_x, need_w, _ = ctx.needs_input_grad
+        trained = isinstance(weight, torch.Tensor)
+        if trained:
+            w = ops.quantize_blocks(weight, transposed=need_x)
             ctx.weight_dtype = weight.dtype
         else:
             w = weight
-            if ctx.needs_input_grad[0]:
-                w.transposed()
-        ctx.w = w
+            if need_x:
+                w.transposed()                              # raises without one
         ctx.bias_dtype = None if bias is None else bias.dtype
-        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None)
+        ctx.shape = w.shape
+        # what the gradients need: the weight's transpose, and x as its columns in e4m3
+        keep = [None] * 4
+        if need_w and x.shape[0]:
+            a, columns = ops.quantize_both(x)
+            keep[:2] = columns.q, columns.scale
+        else:
+            a = ops.quantize_rows(x)
+        if need_x:
+            keep[2:] = w.qt, w.scale
+        ctx.save_for_backward(*keep)
         return ops.mm_fp8(a, w, bias, None, x.dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         need_x, need_w, need_b = ctx.needs_input_grad
-        x, = ctx.saved_tensors
+        xt, xt_scale, wt, w_scale = ctx.saved_tensors
+        N, K = ctx.shape
         grad = _rows(grad)
-        M = grad.shape[0]
         dx = dw = db = None
-        if need_x:
-            dx = ops.mm_fp8(ops.quantize_rows(grad), ctx.w.transposed(), None, None, grad.dtype)
-        if M == 0:
-            N, K = ctx.w.shape
-            dw = torch.zeros(N, K, dtype=ctx.weight_dtype, device=grad.device) if need_w else None
-            db = torch.zeros(N, dtype=ctx.bias_dtype, device=grad.device) if need_b else None
-        elif need_w:
-            g = ops.quantize_columns(grad, ctx.bias_dtype if need_b else None)
-            g, db = g if need_b else (g, None)
-            dw = ops.mm_fp8(g, ops.quantize_columns(x), None, None, ctx.weight_dtype)
+        if grad.shape[0] == 0:
+            return (grad.new_zeros((0, K)) if need_x else None,
+                    grad.new_zeros((N, K), dtype=ctx.weight_dtype) if need_w else None,
+                    grad.new_zeros(N, dtype=ctx.bias_dtype) if need_b else None)
+        rows = columns = None
+        sums = ctx.bias_dtype if need_b else None
+        if need_x and (need_w or need_b):
+            rows, columns, *db = ops.quantize_both(grad, sums)
+            db = db[0] if db else None
+        elif need_x:
+            rows = ops.quantize_rows(grad)
         elif need_b:
-            db = ops.quantize_columns(grad, ctx.bias_dtype)[1]
+            columns, db = ops.quantize_columns(grad, sums)
+        else:
+            columns = ops.quantize_columns(grad)
+        if need_x:
+            dx = ops.mm_fp8(rows, Fp8Weight(wt, w_scale.t()), None, None, grad.dtype)
+        if need_w:
+            dw = ops.mm_fp8(columns, ops.Fp8Rows(xt, xt_scale), None, None, ctx.weight_dtype)
         return dx, dw, db
 
 

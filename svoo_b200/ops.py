@@ -787,6 +787,33 @@ def quantize_columns(x: torch.Tensor, column_sum_type: Optional[torch.dtype] = N
     return rows, sums
 
 
+def quantize_both(x: torch.Tensor, column_sum_type: Optional[torch.dtype] = None):
+    """(quantize_rows(x), quantize_columns(x)) from one reading of x [M, K], M >= 1; with column_sum_type also the sums of the
+    columns, as quantize_columns gives them."""
+    M, K, stride = _matrix(x, "x")
+    if M < 1:
+        raise ValueError("quantize_both needs at least one row")
+    if column_sum_type is not None and column_sum_type not in TYPES:
+        raise ValueError("column sums are bf16, fp16 or fp32")
+    index = _device(x)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return quantize_both(x, column_sum_type)
+    KB, MB, pitch = (K + 127) // 128, (M + 127) // 128, (K + 3) // 4 * 4
+    q, qt = _empty_e4m3(x, M, K), _empty_e4m3(x, K, M)
+    scale, scale_t = x.new_empty((KB, M), dtype=torch.float32), x.new_empty((MB, pitch), dtype=torch.float32)
+    part = None if column_sum_type is None else x.new_empty((MB, K), dtype=torch.float32)
+    stream = _raw_stream(index)
+    check(LIB.svoo_b200_quantize_both(x.data_ptr(), TYPES[x.dtype], M, K, stride, q.data_ptr(), _pad16(K), scale.data_ptr(), M, qt.data_ptr(),
+                                      _pad16(M), scale_t.data_ptr(), pitch, _ptr(part), stream), "quantize_both")
+    rows, columns = Fp8Rows(q, scale), Fp8Rows(qt, scale_t[:, :K])
+    if part is None:
+        return rows, columns
+    sums = x.new_empty(K, dtype=column_sum_type)
+    check(LIB.svoo_b200_column_sum(part.data_ptr(), MB, K, sums.data_ptr(), TYPES[column_sum_type], stream), "column_sum")
+    return rows, columns, sums
+
+
 def quantize_blocks(w: torch.Tensor, transposed: bool = False) -> Fp8Blocks:
     """w [N, K] in e4m3, one scale per 128 x 128 block; `transposed` keeps the transpose of the bytes too."""
     N, K, stride = _matrix(w, "w")

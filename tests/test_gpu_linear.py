@@ -44,8 +44,12 @@ def test_quantisers_bit_for_bit(dtype, M, K):
     b = ops.quantize_blocks(x, transposed=True)
     q, s = R.quantize(x, 128, 128)
     assert torch.equal(b.scale, s) and same_values(b.q, q) and same_values(b.qt, q.t())
+    r2, c2, sums2 = ops.quantize_both(x, torch.float32)
+    for one, two in ((r, r2), (c, c2)):
+        assert torch.equal(one.q.view(torch.uint8), two.q.view(torch.uint8)) and torch.equal(one.scale, two.scale)
+    assert ((sums2.double() - ref).abs() <= 100 * 2.0 ** -24 * x.double().abs().sum(0) + 1e-30).all()
     # what lies behind a row is zero up to the next multiple of 16
-    for t in (r.q, c.q, b.q, b.qt):
+    for t in (r.q, c.q, b.q, b.qt, r2.q, c2.q):
         whole = torch.as_strided(t.view(torch.uint8), (t.shape[0], t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16),
                                  (t.stride(0), 1))
         assert not whole[:, t.shape[1]:].any()
@@ -70,7 +74,7 @@ def test_quantise_strided():
     from svoo_b200 import ops
     wide = rand(70, 400, torch.bfloat16, 5)
     for x in (wide[:, :256], wide[:, 3:260], wide[::3, 8:136], wide[7:8, 1:2]):
-        for fn in (ops.quantize_rows, ops.quantize_columns, ops.quantize_blocks):
+        for fn in (ops.quantize_rows, ops.quantize_columns, ops.quantize_blocks, lambda t: ops.quantize_both(t)[0], lambda t: ops.quantize_both(t)[1]):
             a, b = fn(x), fn(x.contiguous())
             assert torch.equal(a.q.view(torch.uint8), b.q.view(torch.uint8)) and torch.equal(a.scale, b.scale)
 
@@ -231,7 +235,7 @@ def test_refusals():
     from svoo_b200 import linear, ops
     x, w = torch.randn(8, 64, device=DEV), torch.randn(40, 64, device=DEV)
     a, b = ops.quantize_rows(x), ops.quantize_blocks(w)
-    for fn in (ops.quantize_rows, ops.quantize_columns, ops.quantize_blocks):
+    for fn in (ops.quantize_rows, ops.quantize_columns, ops.quantize_blocks, ops.quantize_both):
         for t in (x.double(), x.t(), x[None], x.cpu(), x[:, :0]):
             with pytest.raises(ValueError):
                 fn(t)
