@@ -515,6 +515,8 @@ def run_dit_arm(args):
     if S % world:
         raise SystemExit(f"{S} tokens do not split evenly over {world} ranks")
     model = wan_dit.WanDiT(cfg).init_weights(seed=1).to(device=dev, dtype=torch.bfloat16).eval()
+    if args.token_kernels != "none":
+        model.use_token_kernels(fp8_linears=args.token_kernels == "fp8")
     steps_total = args.warmup + args.steps
     csv_path = os.path.join(tempfile.mkdtemp(), "density.csv")
     wan_dit.write_density_table(csv_path, steps_total, cfg.num_layers, H, *DIT_DENSITY, seed=1004)
@@ -600,10 +602,10 @@ def run_dit_arm(args):
         line = {
             "metric": "dit_denoising_step_ms", "value": step_ms, "unit": "ms", "n_gpus": world, "steps": args.steps,
             "warmup": args.warmup, "ms_per_step": step_ms, "higher_is_better": False, "scaling": "strong", "vs_baseline": None,
-            "dtype": "bf16", "data": "synthetic",
+            "dtype": "bf16" if args.token_kernels != "fp8" else "bf16, e4m3 linear layers", "data": "synthetic",
             "config": {"workload": "wan1.3b-dit-480p", "blocks": cfg.num_layers, "dim": cfg.dim, "heads": H, "tokens": S,
                        "q_clusters": 100, "k_clusters": 500, "kmeans_iters": 5, "density_floor_table": list(DIT_DENSITY),
-                       "parallelism": "one GPU" if world == 1 else f"sequence parallel x{world}, heads re-sharded by peer stores",
+                       "token_kernels": args.token_kernels, "parallelism": "one GPU" if world == 1 else f"sequence parallel x{world}, heads re-sharded by peer stores",
                        "l2": "activations of one block (100 MB per tensor) and 2.6 GB of weights exceed the L2; no flush"},
             "sparse_attention_ms_per_step": attn_ms, "sparse_attention_share": attn_ms / step_ms,
             "e2e": {"value": float(e2e_ms.item()), "unit": "ms", "ms_per_step": float(e2e_ms.item()),
@@ -654,6 +656,8 @@ def main():
     ap.add_argument("--impl", default="svoo_b200", choices=["svoo_b200", "reference"])
     ap.add_argument("--config", default="cfg2", choices=sorted(synth.CONFIGS) + ["cfg4"])
     ap.add_argument("--dit-layers", type=int, default=30, help="blocks of the cfg4 DiT (debugging)")
+    ap.add_argument("--token-kernels", default="none", choices=["none", "norms", "fp8"],
+                    help="cfg4: the blocks' layer norms, or norms and e4m3 linear layers, on this package's kernels")
     ap.add_argument("--heads", type=int, default=0, help="override the head count (debugging)")
     ap.add_argument("--top-p", type=float, default=None, help="override the config's top-p of the block selection")
     ap.add_argument("--pattern", default="svoo", choices=["svoo", "ear"],

@@ -9,6 +9,8 @@ loads libsvoo_b200.so and raises if it is missing -- there is no fallback):
   layer          sparse_attention_layer: the whole path as one kernel sequence
   processor      WanAttn_SAPAttn_Processor, Hunyuan_SAPAttn_Processor2_0
   parallel       head-sharded (Ulysses) execution: peer-store re-shard, head partition, host-shard pipeline
+  norm           layer norm, affine or modulated, with its gradient
+  linear         linear layers in e4m3 with block scales: linear_fp8 and its gradients, mlp_fp8, Fp8Linear, Fp8FeedForward
   wan_dit        a plain-torch DiT with the Wan block structure around the processor (in-situ runs)
   ops            one torch wrapper per C-ABI entry point
   synth          seeded synthetic workloads

@@ -107,3 +107,72 @@ def mlp_fp8(x: torch.Tensor, w1: Fp8Weight, bias1: Optional[torch.Tensor], w2: F
     h = ops.linear_fp8(_rows(x), w1, bias1, "gelu", ops.E4M3)
     y = ops.mm_fp8(h, w2, bias2, None, x.dtype)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[1])
+
+
+class Fp8Linear(nn.Module):
+    """An nn.Linear for inference whose weight is held in e4m3, one byte per number: forward is linear_fp8 with the bias and
+    type of the input.  The bytes and scales are kept as uint8 buffers, which follow the module to a device and through a
+    state dict, and which a cast of the module's floating-point type leaves alone."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, input_grad: bool = False, device=None,
+                 dtype: Optional[torch.dtype] = None):
+        super().__init__()
+        self.in_features, self.out_features = in_features, out_features
+        blocks = ((out_features + 127) // 128, (in_features + 127) // 128)
+
+        def buffer(rows, columns):
+            return torch.zeros(rows, columns, dtype=torch.uint8, device=device)
+
+        self.register_buffer("weight_q", buffer(out_features, ops._pad16(in_features)))
+        self.register_buffer("weight_scale", buffer(blocks[0], 4 * blocks[1]))
+        self.register_buffer("weight_qt", buffer(in_features, ops._pad16(out_features)) if input_grad else None)
+        self.bias = nn.Parameter(torch.zeros(out_features, device=device, dtype=dtype), requires_grad=False) if bias else None
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear, input_grad: bool = False) -> "Fp8Linear":
+        """Quantises the weight of a linear layer on its GPU.  input_grad keeps the transpose too, for the gradient of the input."""
+        w = linear.weight.detach()
+        m = cls(linear.in_features, linear.out_features, linear.bias is not None, input_grad, w.device, w.dtype)
+        m.set_weight(ops.quantize_blocks(w, transposed=input_grad))
+        if linear.bias is not None:
+            m.bias.data.copy_(linear.bias.detach())
+        return m.train(linear.training)
+
+    @torch.no_grad()
+    def set_weight(self, w: Fp8Weight) -> None:
+        N, K = w.shape
+        if (N, K) != (self.out_features, self.in_features):
+            raise ValueError(f"expected a weight [{self.out_features}, {self.in_features}], got {[N, K]}")
+        self.weight_q[:, :K].copy_(w.q.view(torch.uint8))
+        self.weight_scale.copy_(w.scale.contiguous().view(torch.uint8))
+        if self.weight_qt is not None:
+            self.weight_qt[:, :N].copy_(w.transposed().q.view(torch.uint8))
+
+    @property
+    def weight(self) -> Fp8Weight:
+        qt = None if self.weight_qt is None else self.weight_qt.view(ops.E4M3)[:, :self.out_features]
+        return Fp8Weight(self.weight_q.view(ops.E4M3)[:, :self.in_features], self.weight_scale.view(torch.float32), qt)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return linear_fp8(x, self.weight, self.bias)
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
+
+
+class Fp8FeedForward(nn.Module):
+    """Linear, GELU (tanh formula), Linear on e4m3 weights, for inference: forward is mlp_fp8."""
+
+    def __init__(self, first: Fp8Linear, second: Fp8Linear):
+        super().__init__()
+        self.first, self.second = first, second
+
+    @classmethod
+    def from_sequential(cls, seq: nn.Sequential) -> "Fp8FeedForward":
+        if len(seq) != 3 or not isinstance(seq[0], nn.Linear) or not isinstance(seq[2], nn.Linear) or \
+                not isinstance(seq[1], nn.GELU) or seq[1].approximate != "tanh":
+            raise ValueError("expected Linear, GELU(approximate='tanh'), Linear")
+        return cls(Fp8Linear.from_linear(seq[0]), Fp8Linear.from_linear(seq[2]))
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return mlp_fp8(x, self.first.weight, self.first.bias, self.second.weight, self.second.bias)

@@ -2,7 +2,8 @@
 processor in situ: every block's self-attention goes through `WanAttn_SAPAttn_Processor`
 (the path this package implements); everything else -- patch embedding, condition embedder,
 layer norms, AdaLN modulation, cross attention to the text context, feed-forward, output
-projection -- is ordinary torch and outside the path.
+projection -- is ordinary torch and outside the path, unless `WanDiT.use_token_kernels` puts the norms and
+the linear layers of the blocks on this package's kernels as well.
 
 The block dataflow follows the reference's patched forward (svoo/models/wan/custom_models.py:
 22-108 block, :116-197 model), which threads `timestep` into `attn1` (:63).  Weights are
@@ -23,6 +24,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import linear as fp8
+from . import norm
 from .layer import sparse_attention_layer
 from .processor import WanAttn_SAPAttn_Processor
 
@@ -101,21 +104,25 @@ class WanBlock(nn.Module):
         self.norm3 = nn.LayerNorm(d, cfg.eps, elementwise_affine=False)
         self.ffn = nn.Sequential(nn.Linear(d, cfg.ffn_dim), nn.GELU(approximate="tanh"), nn.Linear(cfg.ffn_dim, d))
         self.scale_shift_table = nn.Parameter(torch.zeros(1, 6, d))
+        self.fused_norms = False
 
-    @staticmethod
-    def _ln(norm: nn.LayerNorm, x):
-        w = None if norm.weight is None else norm.weight.float()
-        b = None if norm.bias is None else norm.bias.float()
-        return F.layer_norm(x.float(), norm.normalized_shape, w, b, norm.eps)
+    def _norm(self, ln: nn.LayerNorm, x, scale=None, shift=None):
+        """fp32 layer norm of x, modulated where scale and shift are given, in x's type."""
+        if self.fused_norms:
+            return norm.layer_norm(x, ln.weight, ln.bias, scale, shift, ln.eps)
+        w = None if ln.weight is None else ln.weight.float()
+        b = None if ln.bias is None else ln.bias.float()
+        y = F.layer_norm(x.float(), ln.normalized_shape, w, b, ln.eps)
+        return (y if scale is None else y * (1 + scale) + shift).type_as(x)
 
     def forward(self, hidden_states, encoder_hidden_states, temb, rotary_emb, timestep=0):
         shift, scale, gate, c_shift, c_scale, c_gate = (self.scale_shift_table.float() + temb.float()).chunk(6, dim=1)
-        x = (self._ln(self.norm1, hidden_states) * (1 + scale) + shift).type_as(hidden_states)
+        x = self._norm(self.norm1, hidden_states, scale, shift)
         attn = self.attn1(hidden_states=x, rotary_emb=rotary_emb, timestep=timestep)
         hidden_states = (hidden_states.float() + attn * gate).type_as(hidden_states)
-        x = self._ln(self.norm2, hidden_states).type_as(hidden_states)
+        x = self._norm(self.norm2, hidden_states)
         hidden_states = hidden_states + self.attn2(hidden_states=x, encoder_hidden_states=encoder_hidden_states)
-        x = (self._ln(self.norm3, hidden_states) * (1 + c_scale) + c_shift).type_as(hidden_states)
+        x = self._norm(self.norm3, hidden_states, c_scale, c_shift)
         ff = self.ffn(x)
         return (hidden_states.float() + ff.float() * c_gate).type_as(hidden_states)
 
@@ -164,6 +171,20 @@ class WanDiT(nn.Module):
                 p.zero_()
             elif "norm_q" in name or "norm_k" in name:
                 p.copy_(1.0 + 0.1 * torch.randn(p.shape, generator=g))
+        return self
+
+    def use_token_kernels(self, norms: bool = True, fp8_linears: bool = True) -> "WanDiT":
+        """Puts the token-wise half of every block on this package's kernels: layer norms with their modulation in one pass,
+        and (inference only) the projections and the feed-forward in e4m3, their weights quantised here.  The model has to be on
+        its GPU.  Embedders, the output projection and the per-step embeddings stay as they are."""
+        for block in self.blocks:
+            block.fused_norms = norms
+            if fp8_linears:
+                for attn in (block.attn1, block.attn2):
+                    for name in ("to_q", "to_k", "to_v"):
+                        setattr(attn, name, fp8.Fp8Linear.from_linear(getattr(attn, name)))
+                    attn.to_out[0] = fp8.Fp8Linear.from_linear(attn.to_out[0])
+                block.ffn = fp8.Fp8FeedForward.from_sequential(block.ffn)
         return self
 
     def _timestep_embedding(self, timestep):
