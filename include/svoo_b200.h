@@ -443,8 +443,10 @@ int svoo_b200_mm_fp8(const void* a, int64_t a_pitch, const float* a_scale, int64
                      int32_t bias_type, int64_t M, int64_t N, int64_t K, int32_t activation, void* out, int32_t out_type,
                      int64_t out_pitch, float* out_scale, int64_t out_scale_pitch, void* stream);
 /* svoo_b200_quantize_rows of x [M, K] (x_type, rows x_row apart) into the workspace and svoo_b200_mm_fp8 with b [N, K] and its
- * block scales: a linear layer on unquantised rows in one call, with the same result as the two. */
-int svoo_b200_linear_fp8_workspace_bytes(int64_t M, int64_t K, int64_t* bytes_out);
+ * block scales: a linear layer on unquantised rows in one call.  Where it needs no workspace (at most 8 rows, or 16 rows of up to
+ * 4,096 columns; not with an e4m3 output) it is one launch whose sums run in an order of their own; otherwise the result is that
+ * of the two calls. */
+int svoo_b200_linear_fp8_workspace_bytes(int64_t M, int64_t K, int32_t out_type, int64_t* bytes_out);
 int svoo_b200_linear_fp8(const void* x, int32_t x_type, int64_t M, int64_t K, int64_t x_row, const void* b, int64_t b_pitch,
                          const float* b_scale, int64_t b_scale_n, int64_t b_scale_k, const void* bias, int32_t bias_type, int64_t N,
                          int32_t activation, void* out, int32_t out_type, int64_t out_pitch, float* out_scale,

@@ -98,7 +98,7 @@ SIGNATURES = {
     "svoo_b200_mm_fp8": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int32,
                                  c_void_p, c_int32, c_int64, c_int64, c_int64, c_int32, c_void_p, c_int32, c_int64, c_void_p,
                                  c_int64, c_void_p]),
-    "svoo_b200_linear_fp8_workspace_bytes": (c_int, [c_int64, c_int64, _I64P]),
+    "svoo_b200_linear_fp8_workspace_bytes": (c_int, [c_int64, c_int64, c_int32, _I64P]),
     "svoo_b200_linear_fp8": (c_int, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64,
                                      c_void_p, c_int32, c_int64, c_int32, c_void_p, c_int32, c_int64, c_void_p, c_int64, c_void_p,
                                      c_int64, c_void_p]),

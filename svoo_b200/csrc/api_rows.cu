@@ -18,6 +18,10 @@ cudaError_t launch_quantize_blocks(int type, const void* w, int64_t N, int64_t K
 cudaError_t launch_linear(const void* a, int64_t a_pitch, const float* sa, int64_t sa_pitch, const void* b, int64_t b_pitch, const float* sb,
                              int64_t sb_n, int64_t sb_k, bool row_scales, const void* bias, int bias_type, int64_t M, int64_t N, int64_t K,
                              bool gelu, int out_type, void* out, int64_t out_pitch, float* out_scale, int64_t out_scale_pitch, cudaStream_t st);
+bool linear_few_rows(int64_t M, int64_t K, int out_type);
+cudaError_t launch_linear_few_rows(int x_type, const void* x, int64_t x_row, const void* b, int64_t b_pitch, const float* sb, int64_t sb_n,
+                                   int64_t sb_k, const void* bias, int bias_type, int64_t M, int64_t N, int64_t K, bool gelu, int out_type,
+                                   void* out, int64_t out_pitch, cudaStream_t st);
 cudaError_t read_linear_status(int32_t* out, cudaStream_t st);
 }  // namespace svoo
 
@@ -178,10 +182,10 @@ int svoo_b200_mm_fp8(const void* a, int64_t a_pitch, const float* a_scale, int64
                             (cudaStream_t)stream);
 }
 
-int svoo_b200_linear_fp8_workspace_bytes(int64_t M, int64_t K, int64_t* bytes_out) {
+int svoo_b200_linear_fp8_workspace_bytes(int64_t M, int64_t K, int32_t out_type, int64_t* bytes_out) {
   if (!bytes_out) return SVOO_ERR_NULL;
   if (M < 0 || K < 1 || M > kMaxRows || K > kMaxRows) return SVOO_ERR_SHAPE;
-  *bytes_out = align_up(M * align_up(K, 16), 256) + ceil_div64(K, 128) * M * 4;
+  *bytes_out = linear_few_rows(M, K, out_type) ? 0 : align_up(M * align_up(K, 16), 256) + ceil_div64(K, 128) * M * 4;
   return SVOO_OK;
 }
 
@@ -190,21 +194,27 @@ int svoo_b200_linear_fp8(const void* x, int32_t x_type, int64_t M, int64_t K, in
                          int32_t activation, void* out, int32_t out_type, int64_t out_pitch, float* out_scale,
                          int64_t out_scale_pitch, void* workspace, int64_t workspace_bytes, void* stream) {
   int64_t need = 0;
-  SVOO_TRY(svoo_b200_linear_fp8_workspace_bytes(M, K, &need));
-  if (M > 0 && !workspace) return SVOO_ERR_NULL;
+  SVOO_TRY(svoo_b200_linear_fp8_workspace_bytes(M, K, out_type, &need));
+  if (need && !workspace) return SVOO_ERR_NULL;
   if (workspace_bytes < need) return SVOO_ERR_WORKSPACE;
   if (!aligned(workspace, 16)) return SVOO_ERR_ALIGN;
   const int64_t pitch = align_up(K, 16);
-  float* scale = reinterpret_cast<float*>(static_cast<char*>(workspace) + align_up(M * pitch, 256));
-  // the product's arguments are checked before anything is launched
-  SVOO_TRY(check_quant(x, x_type, M, K, x_row, workspace, pitch, K, scale));
-  SVOO_TRY(check_mm(workspace, pitch, scale, M, b, b_pitch, b_scale, b_scale_n, b_scale_k, 0, bias, bias_type, M, N, K, activation, out,
+  // the product's arguments are checked before anything is launched; without a workspace b stands in for the rows in it
+  const void* rows = need ? workspace : b;
+  float* scale = need ? reinterpret_cast<float*>(static_cast<char*>(workspace) + align_up(M * pitch, 256)) : nullptr;
+  const float* any_scale = need ? scale : b_scale;
+  SVOO_TRY(check_quant(x, x_type, M, K, x_row, rows, pitch, K, any_scale));
+  SVOO_TRY(check_mm(rows, pitch, any_scale, M, b, b_pitch, b_scale, b_scale_n, b_scale_k, 0, bias, bias_type, M, N, K, activation, out,
                     out_type, out_pitch, out_scale, out_scale_pitch));
   if (M == 0) return SVOO_OK;
+  const bool gelu = activation == SVOO_ACT_GELU_TANH;
+  if (!need)
+    return (int)launch_linear_few_rows(x_type, x, x_row, b, b_pitch, b_scale, b_scale_n, b_scale_k, bias, bias_type, M, N, K, gelu, out_type,
+                                       out, out_pitch, (cudaStream_t)stream);
   const cudaError_t e = launch_quantize_rows(x_type, x, M, K, x_row, workspace, pitch, scale, M, (cudaStream_t)stream);
   if (e != cudaSuccess) return (int)e;
-  return (int)launch_linear(workspace, pitch, scale, M, b, b_pitch, b_scale, b_scale_n, b_scale_k, false, bias, bias_type, M, N, K,
-                            activation == SVOO_ACT_GELU_TANH, out_type, out, out_pitch, out_scale, out_scale_pitch, (cudaStream_t)stream);
+  return (int)launch_linear(workspace, pitch, scale, M, b, b_pitch, b_scale, b_scale_n, b_scale_k, false, bias, bias_type, M, N, K, gelu,
+                            out_type, out, out_pitch, out_scale, out_scale_pitch, (cudaStream_t)stream);
 }
 
 int svoo_b200_linear_status(int32_t* status, void* stream) {

@@ -144,11 +144,12 @@ struct BlockDivideOnce {
   }
 };
 
+// Plain loads: the 16-bit forms of __ldg are assembly that the compiler may move in front of the condition on a.bias.
 __device__ __forceinline__ float load_bias(const LinearArgs& a, int n) {
-  if (n >= a.N) return 0.f;
-  if (a.bias_type == SVOO_TYPE_FP32) return __ldg(static_cast<const float*>(a.bias) + n);
-  if (a.bias_type == SVOO_TYPE_BF16) return to_f32(__ldg(static_cast<const __nv_bfloat16*>(a.bias) + n));
-  return to_f32(__ldg(static_cast<const __half*>(a.bias) + n));
+  if (!a.bias || n >= a.N) return 0.f;
+  if (a.bias_type == SVOO_TYPE_FP32) return static_cast<const float*>(a.bias)[n];
+  if (a.bias_type == SVOO_TYPE_BF16) return to_f32(static_cast<const __nv_bfloat16*>(a.bias)[n]);
+  return to_f32(static_cast<const __half*>(a.bias)[n]);
 }
 
 }  // namespace tc

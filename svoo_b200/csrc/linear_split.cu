@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) linear_split_kernel(const __
   const int n = n0 + lane * 4;
   float bias[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) bias[i] = a.bias ? load_bias(a, n + i) : 0.f;
+  for (int i = 0; i < 4; ++i) bias[i] = load_bias(a, n + i);
   const int r1 = rows * (rank + 1) / ranks;
   for (int r = rows * rank / ranks + warp; r < r1; r += kSplitThreads / 32) {
     const uint32_t at = base + r * kSplitN * 4 + ((lane ^ (r & 31)) << 4);
@@ -202,6 +202,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) linear_split_kernel(const __
       }
     }
   }
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");   // nobody reads this CTA's sums any more
   if (tid == 0 && *abort_flag) atomicExch(a.status, 1);
   if (warp == 1) {

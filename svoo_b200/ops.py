@@ -891,8 +891,8 @@ def mm_fp8(a: Fp8Rows, b, bias: Optional[torch.Tensor] = None, activation: Optio
 
 def linear_fp8(x: torch.Tensor, w: Fp8Blocks, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
                out_dtype: Optional[torch.dtype] = None):
-    """mm_fp8(quantize_rows(x), w, bias, activation, out_dtype or x's type) in one call, with the same result: x [M, K] (bf16, fp16,
-    fp32; dense rows)."""
+    """mm_fp8(quantize_rows(x), w, bias, activation, out_dtype or x's type) in one call: x [M, K] (bf16, fp16, fp32; dense
+    rows).  Few rows (8, or 16 of up to 4,096 columns) are one launch, whose 32-bit sums run in another order than mm_fp8's."""
     M, K, stride = _matrix(x, "x")
     q, scale = w.q, w.scale
     N = q.shape[0]
@@ -905,12 +905,13 @@ def linear_fp8(x: torch.Tensor, w: Fp8Blocks, bias: Optional[torch.Tensor] = Non
         with torch.cuda.device(index):
             return linear_fp8(x, w, bias, activation, out_dtype)
     out, out_scale, pitch, kind = _product_output(x, M, N, bias, activation, out_dtype or x.dtype)
-    ws_bytes = (M * _pad16(K) + 255) // 256 * 256 + KB * M * 4
-    ws = x.new_empty(ws_bytes, dtype=torch.uint8)
+    ws, ws_bytes = None, 0                                  # as svoo_b200_linear_fp8_workspace_bytes
+    if M > 16 or (M > 8 and K > 4096) or out_scale is not None:
+        ws_bytes = (M * _pad16(K) + 255) // 256 * 256 + KB * M * 4
+        ws = x.new_empty(ws_bytes, dtype=torch.uint8)
     check(LIB.svoo_b200_linear_fp8(x.data_ptr(), TYPES[x.dtype], M, K, stride, q.data_ptr(), wp, scale.data_ptr(), scale.stride(0),
                                    scale.stride(1), _ptr(bias), 0 if bias is None else TYPES[bias.dtype], N, _ACTIVATIONS[activation],
-                                   out.data_ptr(), kind, pitch, _ptr(out_scale), M, ws.data_ptr(), ws_bytes, _raw_stream(index)),
-          "linear_fp8")
+                                   out.data_ptr(), kind, pitch, _ptr(out_scale), M, _ptr(ws), ws_bytes, _raw_stream(index)), "linear_fp8")
     return out if out_scale is None else Fp8Rows(out, out_scale)
 
 

@@ -110,6 +110,40 @@ def test_product_with_blocks(dtype, M, N, K):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 5, 16), (2, 130, 300), (3, 777, 1001), (7, 4800, 130), (8, 33, 2048), (9, 40, 257), (15, 5000, 640), (16, 5120, 1300), (9, 64, 4100),
+                                   (16, 129, 1000), (17, 129, 1000)])
+def test_linear_of_few_rows(dtype, M, N, K):
+    """One launch up to 16 rows: quantised, multiplied, bias and GELU; weights with bytes behind their rows, rows of a wider tensor."""
+    from svoo_b200 import ops
+    wide = rand(M, K + 24, dtype, M + K)
+    w = rand(N, K, dtype, N + K, 0.05)
+    bias = rand(1, N, [torch.float32, dtype][M % 2], N)[0]
+    b = ops.quantize_blocks(w)
+    if K % 16:
+        torch.as_strided(b.q.view(torch.uint8), (N, -K % 16), (b.q.stride(0) if N > 1 else (K + 15) // 16 * 16, 1), K).fill_(0x7f)   # NaN
+    bd = R.dequantize(w, 128, 128)
+    for x in (wide[:, :K].contiguous(), wide[:, 8:K + 8], wide[:, 3:K + 3]):
+        ad = R.dequantize(x.contiguous(), 1, 128)
+        want = ad @ bd.t() + bias.double()
+        tol = R.product_bound(ad, bd, torch.float32, want) + 2.0 ** -22 * bias.double().abs()
+        y = ops.linear_fp8(x, b, bias, None, torch.float32)
+        assert ((y.double() - want).abs() <= tol).all()
+        y = ops.linear_fp8(x, b, None, None, torch.float32)
+        plain = ad @ bd.t()
+        assert ((y.double() - plain).abs() <= R.product_bound(ad, bd, torch.float32, plain)).all()
+        y = ops.linear_fp8(x, b, bias, "gelu")
+        g = R.gelu(want)
+        assert y.dtype == dtype
+        assert ((y.double() - g).abs() <= 1.13 * tol + 2.0 ** -19 * want.abs() + R.half_step(dtype) * g.abs() + torch.finfo(dtype).tiny).all()
+        h, q = ops.linear_fp8(x, b, bias, None, ops.E4M3), ops.mm_fp8(ops.quantize_rows(x), b, bias, None, ops.E4M3)
+        assert torch.equal(h.q.view(torch.uint8), q.q.view(torch.uint8)) and torch.equal(h.scale, q.scale)
+    x = wide[:, :K].contiguous()
+    x[0, K // 2] = float("nan")
+    y = ops.linear_fp8(x, b, bias)
+    assert torch.isnan(y[0]).all() and torch.isfinite(y[1:]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M,N,K", SIZES)
 def test_product_with_rows(dtype, M, N, K):
     """Both operands with 1 x 128 scales: the gradient of a weight."""

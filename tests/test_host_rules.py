@@ -123,3 +123,12 @@ def test_token_wise_entry_points_check_their_arguments():
     assert mm(act=2) == -8 and mm(ot=4) == -8 and mm(bias=p, bt=3) == -8
     assert mm(a=p + 8) == -5 and mm(rows=1, sk=16, sb=p + 4) == -5
     assert L.svoo_b200_linear_status(None, None) == -1
+    assert L.svoo_b200_linear_fp8_workspace_bytes(16, 100, 0, ctypes.byref(out)) == 0 and out.value == 0
+    assert L.svoo_b200_linear_fp8_workspace_bytes(16, 100, 3, ctypes.byref(out)) == 0 and out.value >= 16 * 112 + 64
+    assert L.svoo_b200_linear_fp8_workspace_bytes(17, 100, 0, ctypes.byref(out)) == 0 and out.value >= 17 * 112 + 68
+    assert L.svoo_b200_linear_fp8_workspace_bytes(9, 5000, 0, ctypes.byref(out)) == 0 and out.value >= 9 * 5008
+    few = dict(x=p, t=0, M=4, K=64, xr=64, b=p, bp=64, sb=p, sn=1, sk=1, bias=None, bt=0, N=16, act=0, out=p, ot=0, op=16, os=None, osp=4, ws=None,
+               wb=0, st=None)
+    lin = lambda **k: L.svoo_b200_linear_fp8(*{**few, **k}.values())                      # noqa: E731
+    assert lin(M=0) == 0 and lin(x=None) == -1 and lin(b=None) == -1 and lin(out=None) == -1 and lin(bp=72) == -2 and lin(t=3) == -8
+    assert lin(M=17) == -1 and lin(M=17, ws=p, wb=16) == -4 and lin(ot=3) == -1 and lin(K=0) == -2 and lin(b=p + 8) == -5
