@@ -2,7 +2,7 @@
 #include "rows_common.cuh"
 
 namespace svoo {
-int64_t norm_backward_bytes(int64_t rows, int groups, int C);
+int64_t norm_backward_bytes(int64_t batch, int64_t rows, int groups, int C);
 cudaError_t launch_layer_norm(int type, const NormArgs& a, cudaStream_t st);
 cudaError_t launch_layer_norm_backward(int type, const NormArgs& a, int groups, void* dgain, void* doffset, cudaStream_t st);
 cudaError_t launch_column_sum(const float* partial, int64_t parts, int64_t C, void* out, int out_type, cudaStream_t st);
@@ -67,6 +67,10 @@ int check_mm(const void* a, int64_t a_pitch, const float* a_scale, int64_t a_sca
     return SVOO_ERR_ALIGN;
   return SVOO_OK;
 }
+// the byte behind the last element of a tensor [batch, rows, C]
+const void* end_of(const void* p, int64_t batch, int64_t rows, int64_t C, int64_t batch_stride, int64_t row_stride, int e) {
+  return static_cast<const char*>(p) + ((batch - 1) * batch_stride + (rows - 1) * row_stride + C) * e;
+}
 int64_t norm_groups(int64_t batch, int32_t per_sample) { return per_sample && batch > 1 ? batch : 1; }
 #define SVOO_TRY(expr) do { int _rc = (expr); if (_rc != SVOO_OK) return _rc; } while (0)
 }  // namespace
@@ -86,6 +90,7 @@ int svoo_b200_layer_norm(const void* x, int32_t x_type, int64_t batch, int64_t r
   a.x = x, a.y = y, a.gain = gain, a.offset = offset, a.mean = mean, a.rstd = rstd;
   a.x_batch = batch == 1 ? 0 : x_batch, a.x_row = x_row, a.gain_batch = gain_batch, a.offset_batch = offset_batch;
   a.batch = batch, a.rows = rows, a.C = (int)C, a.params_fp32 = param_type == SVOO_TYPE_FP32, a.plus_one = gain_plus_one != 0, a.eps = eps;
+  a.x_end = end_of(x, batch, rows, C, a.x_batch, x_row, e);
   if (!(a.status = rows_status_word())) return (int)cudaErrorInvalidDevice;
   return (int)launch_layer_norm(x_type, a, (cudaStream_t)stream);
 }
@@ -94,7 +99,7 @@ int svoo_b200_layer_norm_workspace_bytes(int64_t batch, int64_t rows, int64_t C,
   if (!bytes_out) return SVOO_ERR_NULL;
   SVOO_TRY(check_norm(SVOO_TYPE_FP32, batch, rows, C, 0, 0, SVOO_TYPE_FP32, per_sample != 0));
   const int64_t groups = norm_groups(batch, per_sample);
-  *bytes_out = norm_backward_bytes(groups > 1 ? rows : batch * rows, (int)groups, (int)C);
+  *bytes_out = norm_backward_bytes(batch, rows, (int)groups, (int)C);
   return SVOO_OK;
 }
 
@@ -114,12 +119,14 @@ int svoo_b200_layer_norm_backward(const void* dy, int64_t dy_batch, int64_t dy_r
       !aligned(workspace, 4) || !aligned(mean, 4) || !aligned(rstd, 4))
     return SVOO_ERR_ALIGN;
   const int64_t groups = norm_groups(batch, per_sample);
-  if (dgain && workspace_bytes < norm_backward_bytes(groups > 1 ? rows : batch * rows, (int)groups, (int)C)) return SVOO_ERR_WORKSPACE;
+  if (dgain && workspace_bytes < norm_backward_bytes(batch, rows, (int)groups, (int)C)) return SVOO_ERR_WORKSPACE;
   NormArgs a = {};
   a.x = x, a.dy = dy, a.dx = dx, a.gain = gain, a.mean_in = mean, a.rstd_in = rstd, a.partial = dgain ? (float*)workspace : nullptr;
   a.x_batch = batch == 1 ? 0 : x_batch, a.x_row = x_row, a.dy_batch = batch == 1 ? 0 : dy_batch, a.dy_row = dy_row;
   a.gain_batch = groups > 1 ? gain_batch : 0;
   a.batch = batch, a.rows = rows, a.C = (int)C, a.params_fp32 = param_type == SVOO_TYPE_FP32, a.plus_one = gain_plus_one != 0;
+  a.x_end = end_of(x, batch, rows, C, a.x_batch, x_row, e);
+  a.dy_end = end_of(dy, batch, rows, C, a.dy_batch, dy_row, e);
   if (!(a.status = rows_status_word())) return (int)cudaErrorInvalidDevice;
   return (int)launch_layer_norm_backward(x_type, a, (int)groups, dgain, doffset, (cudaStream_t)stream);
 }

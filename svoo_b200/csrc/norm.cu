@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(TPR) layer_norm_backward_kernel(const NormArgs
   }
 }
 
-// ---- rows of whole 16-byte pieces: fetched ahead into shared memory -----------------------------------------------------
+// ---- rows fetched ahead into shared memory -----------------------------------------------------------------------------
 //
 // A group of TPR threads walks rows; cp.async.bulk brings the next kStages rows of every group while one is worked on, so that what is
 // in flight does not depend on registers or on where the group is in its arithmetic.  Gain and offset lie in shared memory in 32
@@ -229,12 +229,17 @@ constexpr int kRingThreads = 256;
 constexpr int kForwardStages = 1;                  // the row is in registers at once, so its place is free again: three cost 15 %
 constexpr int kBackwardStages = 3;                 // the row is read twice
 
+// kAligned: every row starts on 16 bytes and is whole 16-byte pieces.  Other rows are fetched with the bytes that share their first and
+// last 16 (their neighbours', inside the tensor), read at a shift that is the same for the whole row, and written back
+// the same way: staged in shared memory and stored as aligned pieces, single elements at both ends.
 struct RingLayout {
-  int row, ring, bars, total;                     // bytes of a row; offsets
-  __host__ __device__ RingLayout(int C, int e, int param_rows, int row_tensors, int groups, int stages) {
-    row = C * e;
-    ring = param_rows * C * 4;
-    bars = ring + groups * stages * row_tensors * row;
+  int columns, row, ring, out, bars, total;       // columns rounded up to whole pieces, bytes of a row's place; offsets
+  __host__ __device__ RingLayout(int C, int e, int param_rows, int row_tensors, int groups, int stages, bool aligned) {
+    columns = (C + 7) & ~7;
+    row = aligned ? C * e : ((C * e + 15) & ~15) + 16;
+    ring = param_rows * columns * 4;
+    out = ring + groups * stages * row_tensors * row;
+    bars = out + (aligned ? 0 : groups * row);
     total = bars + groups * stages * 8 + 16;
   }
 };
@@ -323,6 +328,78 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
+// 16 bytes at `shift` (0 .. 15) bytes behind piece c of a row
+__device__ __forceinline__ uint4 shifted_piece(const unsigned char* row, int c, int shift) {
+  const uint4 u = reinterpret_cast<const uint4*>(row)[c], v = reinterpret_cast<const uint4*>(row)[c + 1];
+  uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+  if (shift & 8) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  }
+  if (shift & 4) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  }
+  const int bits = 8 * (shift & 3);
+  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
+                    __funnelshift_r(w[3], w[4], bits));
+}
+// What a bulk copy brings of a row, to `at` bytes behind its place in shared memory.
+struct RowCopy {
+  const void* src;
+  uint32_t bytes, at;
+};
+// The copy for a row whose first byte is to lie where it lies in its 16 bytes.  [lo, hi) is the tensor: where the row's outer 16
+// bytes reach beyond it, its elements in them are copied here, one by one (the first and the last row of all).
+template <typename T, bool kAligned>
+__device__ __forceinline__ RowCopy plan_row(unsigned char* place, const T* src, int C, const void* lo, const void* hi) {
+  if (kAligned) return {src, (uint32_t)(C * sizeof(T)), 0};
+  const uintptr_t first = (uintptr_t)src, last = first + C * sizeof(T);
+  uintptr_t from = first & ~(uintptr_t)15, to = (last + 15) & ~(uintptr_t)15;
+  const uintptr_t base = from;
+  if (from < (uintptr_t)lo) {
+    from += 16;
+    for (uintptr_t p = first; p < last && p < from; p += sizeof(T)) *reinterpret_cast<T*>(place + (p - base)) = *reinterpret_cast<const T*>(p);
+  }
+  if (to > (uintptr_t)hi && to > from) {
+    to -= 16;
+    for (uintptr_t p = first > to ? first : to; p < last; p += sizeof(T)) *reinterpret_cast<T*>(place + (p - base)) = *reinterpret_cast<const T*>(p);
+  }
+  return {(const void*)from, (uint32_t)(to - from), (uint32_t)(from - base)};
+}
+__device__ __forceinline__ void start_copy(unsigned char* place, const RowCopy& c, uint32_t bar) {
+  if (c.bytes) bulk_load(smem_u32(place) + c.at, c.src, c.bytes, bar);
+}
+// piece c of a row that lies at `shift` in its place
+template <bool kAligned>
+__device__ __forceinline__ uint4 row_piece(const unsigned char* place, int c, int shift) {
+  return kAligned ? reinterpret_cast<const uint4*>(place)[c] : shifted_piece(place, c, shift);
+}
+template <typename T>
+__device__ __forceinline__ int shift_of(const T* row) { return (int)((uintptr_t)row & 15); }
+// Zeroes the elements from `valid` on.
+template <int P>
+__device__ __forceinline__ void cut(uint64_t (&d)[P], int valid) {
+#pragma unroll
+  for (int k = 0; k < P; ++k) {
+    if (2 * k >= valid) d[k] = 0;
+    else if (2 * k + 1 >= valid) d[k] &= 0xffffffffull;
+  }
+}
+// A row staged in shared memory (first byte at `staged`) to global memory at any address: aligned 16-byte pieces by all threads of the
+// group, single elements at the ends.
+template <typename T, int TPR>
+__device__ __forceinline__ void store_row(T* dst, const unsigned char* staged, int C, int t) {
+  const int shift = (int)((uintptr_t)dst & 15), bytes = C * (int)sizeof(T);
+  const int head = shift ? 16 - shift : 0;                  // bytes in front of the first aligned piece
+  const int pieces = bytes > head ? (bytes - head) / 16 : 0;
+  unsigned char* out = reinterpret_cast<unsigned char*>(dst);
+  for (int k = t; k < pieces; k += TPR) *reinterpret_cast<uint4*>(out + head + k * 16) = shifted_piece(staged, k, head);
+  const int edge = (head < bytes ? head : bytes) / (int)sizeof(T), tail = bytes > head ? (bytes - head - pieces * 16) / (int)sizeof(T) : 0;
+  if (t < edge) dst[t] = reinterpret_cast<const T*>(staged)[t];
+  if (t < tail) dst[C - tail + t] = reinterpret_cast<const T*>(staged)[C - tail + t];
+}
+
 // Row r of the walk of sample `sample` (per_sample) or of all samples: pointer offset in a tensor of these strides
 __device__ __forceinline__ int64_t row_offset(const NormArgs& a, bool per_sample, int sample, int r, int64_t batch_stride, int64_t row_stride) {
   if (per_sample) return sample * batch_stride + r * row_stride;
@@ -331,12 +408,12 @@ __device__ __forceinline__ int64_t row_offset(const NormArgs& a, bool per_sample
   return b * batch_stride + (r - b * a.rows) * row_stride;
 }
 
-// gain (1 + gain, 1) and offset (0) of a sample to shared memory, 32 bits
+// gain (1 + gain, 1) and offset (0) of a sample to shared memory, 32 bits; whole pieces, with `none` behind the last column
 template <typename T>
-__device__ __forceinline__ void stage_param(const NormArgs& a, const void* p, int64_t at, float add, float none, float* dst) {
-  for (int c = threadIdx.x; c < a.C; c += kRingThreads) {
+__device__ __forceinline__ void stage_param(const NormArgs& a, int columns, const void* p, int64_t at, float add, float none, float* dst) {
+  for (int c = threadIdx.x; c < columns; c += kRingThreads) {
     float v = none;
-    if (p) v = add + (a.params_fp32 ? static_cast<const float*>(p)[at + c] : to_f32(static_cast<const T*>(p)[at + c]));
+    if (p && c < a.C) v = add + (a.params_fp32 ? static_cast<const float*>(p)[at + c] : to_f32(static_cast<const T*>(p)[at + c]));
     dst[c] = v;
   }
 }
@@ -351,17 +428,18 @@ __device__ __forceinline__ void leave(uint32_t bars, int stages, int issued, int
   __syncthreads();
 }
 
-template <typename T, int NV, int TPR>
+template <typename T, int NV, int TPR, bool kAligned>
 __global__ void __launch_bounds__(kRingThreads) layer_norm_ring_kernel(const NormArgs a) {
   constexpr int P = 8 / (int)sizeof(T), V = 2 * P, G = kRingThreads / TPR;    // pairs and elements of a piece, groups
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ float slots[2][G][TPR / 32][1];
   const int stages = a.stages;
-  const RingLayout lay(a.C, sizeof(T), 2, 1, G, stages);
+  const RingLayout lay(a.C, sizeof(T), 2, 1, G, stages, kAligned);
   float* gain = reinterpret_cast<float*>(smem);
-  float* off = gain + a.C;
+  float* off = gain + lay.columns;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + lay.bars + G * stages * 8);
-  const int group = threadIdx.x / TPR, t = threadIdx.x % TPR, nvec = a.C / V;
+  const int group = threadIdx.x / TPR, t = threadIdx.x % TPR, nvec = (a.C + V - 1) / V;
+  const int last = kAligned ? -1 : nvec - 1, valid = a.C - (nvec - 1) * V;    // the piece that may be cut
   const bool per_sample = gridDim.y > 1;
   const int n = (int)(per_sample ? a.rows : a.batch * a.rows), step = gridDim.x * G, first = blockIdx.x * G + group;
   unsigned char* ring = smem + lay.ring + group * stages * lay.row;
@@ -373,16 +451,17 @@ __global__ void __launch_bounds__(kRingThreads) layer_norm_ring_kernel(const Nor
   }
   pdl_trigger();
   pdl_wait();
+  auto row_of = [&](int r) { return static_cast<const T*>(a.x) + row_offset(a, per_sample, blockIdx.y, r, a.x_batch, a.x_row); };
   auto fetch = [&](int r, int s) {
-    tc::mbar_expect_tx(bars + 8 * s, lay.row);
-    bulk_load(smem_u32(ring + s * lay.row), static_cast<const T*>(a.x) + row_offset(a, per_sample, blockIdx.y, r, a.x_batch, a.x_row), lay.row,
-              bars + 8 * s);
+    const RowCopy c = plan_row<T, kAligned>(ring + s * lay.row, row_of(r), a.C, a.x, a.x_end);
+    tc::mbar_expect_tx(bars + 8 * s, c.bytes);
+    start_copy(ring + s * lay.row, c, bars + 8 * s);
   };
   int ahead = first, issued = 0;                           // the next row to fetch, fetches so far (thread 0 of the group)
   if (t == 0)
     for (; issued < stages && ahead < n; ++issued, ahead += step) fetch(ahead, issued);
-  stage_param<T>(a, a.gain, blockIdx.y * a.gain_batch, a.plus_one ? 1.f : 0.f, 1.f, gain);
-  stage_param<T>(a, a.offset, blockIdx.y * a.offset_batch, 0.f, 0.f, off);
+  stage_param<T>(a, lay.columns, a.gain, blockIdx.y * a.gain_batch, a.plus_one ? 1.f : 0.f, 1.f, gain);
+  stage_param<T>(a, lay.columns, a.offset, blockIdx.y * a.offset_batch, 0.f, 0.f, off);
   __syncthreads();
   const float inv_c = 1.f / a.C;
   int s = 0, phase = 0;
@@ -391,11 +470,13 @@ __global__ void __launch_bounds__(kRingThreads) layer_norm_ring_kernel(const Nor
     // a wait that expires ends the stores and the fetches, not the walk: every thread meets every barrier
     ok = tc::mbar_wait(bars + 8 * s, phase, abort_flag) && ok;
     uint64_t d[NV][P], sum = 0;
+    const int shift = kAligned ? 0 : shift_of(row_of(r));
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = i * TPR + t;
       if (c < nvec) {
-        unpack<T>(reinterpret_cast<const uint4*>(ring + s * lay.row)[c], d[i]);
+        unpack<T>(row_piece<kAligned>(ring + s * lay.row, c, shift), d[i]);
+        if (!kAligned && c == last) cut(d[i], valid);
 #pragma unroll
         for (int k = 0; k < P; ++k) sum = add2(sum, d[i][k]);
       }
@@ -416,10 +497,10 @@ __global__ void __launch_bounds__(kRingThreads) layer_norm_ring_kernel(const Nor
     for (int i = 0; i < NV; ++i) {
       if (i * TPR + t < nvec) {
 #pragma unroll
-        for (int k = 0; k < P; ++k) {
-          d[i][k] = add2(d[i][k], minus);
-          sum = fma2(d[i][k], d[i][k], sum);
-        }
+        for (int k = 0; k < P; ++k) d[i][k] = add2(d[i][k], minus);
+        if (!kAligned && i * TPR + t == last) cut(d[i], valid);
+#pragma unroll
+        for (int k = 0; k < P; ++k) sum = fma2(d[i][k], d[i][k], sum);
       }
     }
     one[0] = lo2(sum) + hi2(sum);
@@ -431,7 +512,9 @@ __global__ void __launch_bounds__(kRingThreads) layer_norm_ring_kernel(const Nor
       a.rstd[row] = rstd;
     }
     const uint64_t rs = f2(rstd, rstd);
-    uint4* y = reinterpret_cast<uint4*>(static_cast<T*>(a.y) + row * a.C);
+    T* y = static_cast<T*>(a.y) + row * a.C;
+    unsigned char* staged = smem + lay.out + group * lay.row;
+    uint4* to = kAligned ? reinterpret_cast<uint4*>(y) : reinterpret_cast<uint4*>(staged);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = i * TPR + t;
@@ -444,8 +527,13 @@ __global__ void __launch_bounds__(kRingThreads) layer_norm_ring_kernel(const Nor
           d[i][k] = fma2(mul2(d[i][k], rs), gv.x, ov.x);
           d[i][k + 1] = fma2(mul2(d[i][k + 1], rs), gv.y, ov.y);
         }
-        if (ok) y[c] = pack<T>(d[i]);
+        if (ok || !kAligned) to[c] = pack<T>(d[i]);
       }
+    }
+    if (!kAligned) {
+      group_sync<TPR>(group);
+      if (ok) store_row<T, TPR>(y, staged, a.C, t);
+      if (TPR == 32) __syncwarp();                         // other groups meet two barriers before the next row is staged
     }
     if (++s == stages) s = 0, phase ^= 1;
   }
@@ -453,16 +541,17 @@ __global__ void __launch_bounds__(kRingThreads) layer_norm_ring_kernel(const Nor
 }
 
 // x and dy rows come in together.  A thread's columns are the same in every row: their sums stay in its registers.
-template <typename T, int NV, int TPR>
+template <typename T, int NV, int TPR, bool kAligned>
 __global__ void __launch_bounds__(kRingThreads < TPR ? TPR : kRingThreads) layer_norm_backward_ring_kernel(const NormArgs a) {
   constexpr int P = 8 / (int)sizeof(T), V = 2 * P, G = kRingThreads / TPR;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ float slots[2][G][TPR / 32][2];
   const int stages = a.stages;
-  const RingLayout lay(a.C, sizeof(T), 1, 2, G, stages);
+  const RingLayout lay(a.C, sizeof(T), 1, 2, G, stages, kAligned);
   float* gain = reinterpret_cast<float*>(smem);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + lay.bars + G * stages * 8);
-  const int group = threadIdx.x / TPR, t = threadIdx.x % TPR, nvec = a.C / V;
+  const int group = threadIdx.x / TPR, t = threadIdx.x % TPR, nvec = (a.C + V - 1) / V;
+  const int last = kAligned ? -1 : nvec - 1, valid = a.C - (nvec - 1) * V;
   const bool per_sample = gridDim.y > 1;
   const int n = (int)(per_sample ? a.rows : a.batch * a.rows), step = gridDim.x * G, first = blockIdx.x * G + group;
   unsigned char* ring = smem + lay.ring + group * stages * 2 * lay.row;
@@ -474,16 +563,19 @@ __global__ void __launch_bounds__(kRingThreads < TPR ? TPR : kRingThreads) layer
   }
   pdl_trigger();
   pdl_wait();
+  auto x_of = [&](int r) { return static_cast<const T*>(a.x) + row_offset(a, per_sample, blockIdx.y, r, a.x_batch, a.x_row); };
+  auto dy_of = [&](int r) { return static_cast<const T*>(a.dy) + row_offset(a, per_sample, blockIdx.y, r, a.dy_batch, a.dy_row); };
   auto fetch = [&](int r, int s) {
-    const uint32_t dst = smem_u32(ring + s * 2 * lay.row);
-    tc::mbar_expect_tx(bars + 8 * s, 2 * lay.row);
-    bulk_load(dst, static_cast<const T*>(a.x) + row_offset(a, per_sample, blockIdx.y, r, a.x_batch, a.x_row), lay.row, bars + 8 * s);
-    bulk_load(dst + lay.row, static_cast<const T*>(a.dy) + row_offset(a, per_sample, blockIdx.y, r, a.dy_batch, a.dy_row), lay.row, bars + 8 * s);
+    unsigned char *px = ring + s * 2 * lay.row, *pd = px + lay.row;
+    const RowCopy cx = plan_row<T, kAligned>(px, x_of(r), a.C, a.x, a.x_end), cd = plan_row<T, kAligned>(pd, dy_of(r), a.C, a.dy, a.dy_end);
+    tc::mbar_expect_tx(bars + 8 * s, cx.bytes + cd.bytes);
+    start_copy(px, cx, bars + 8 * s);
+    start_copy(pd, cd, bars + 8 * s);
   };
   int ahead = first, issued = 0;
   if (t == 0)
     for (; issued < stages && ahead < n; ++issued, ahead += step) fetch(ahead, issued);
-  stage_param<T>(a, a.gain, blockIdx.y * a.gain_batch, a.plus_one ? 1.f : 0.f, 1.f, gain);
+  stage_param<T>(a, lay.columns, a.gain, blockIdx.y * a.gain_batch, a.plus_one ? 1.f : 0.f, 1.f, gain);
   __syncthreads();
   const float inv_c = 1.f / a.C;
   uint64_t dg[NV][P], dof[NV][P];
@@ -499,8 +591,8 @@ __global__ void __launch_bounds__(kRingThreads < TPR ? TPR : kRingThreads) layer
   for (int r = first, turn = 0; r < n; r += step, turn ^= 1) {
     // a wait that expires ends the stores and the fetches, not the walk: every thread meets every barrier
     ok = tc::mbar_wait(bars + 8 * s, phase, abort_flag) && ok;
-    const uint4* xs = reinterpret_cast<const uint4*>(ring + s * 2 * lay.row);
-    const uint4* ds = reinterpret_cast<const uint4*>(ring + (s * 2 + 1) * lay.row);
+    const unsigned char *xs = ring + s * 2 * lay.row, *ds = xs + lay.row;
+    const int x_shift = kAligned ? 0 : shift_of(x_of(r)), d_shift = kAligned ? 0 : shift_of(dy_of(r));
     const uint64_t rs = f2(rstd, rstd), shift = f2(-mean * rstd, -mean * rstd);       // xhat = x rstd - mean rstd
     uint64_t s1 = 0, s2 = 0;
 #pragma unroll
@@ -508,8 +600,9 @@ __global__ void __launch_bounds__(kRingThreads < TPR ? TPR : kRingThreads) layer
       const int c = i * TPR + t;
       if (c < nvec) {
         uint64_t x[P], d[P];
-        unpack<T>(xs[c], x);
-        unpack<T>(ds[c], d);
+        unpack<T>(row_piece<kAligned>(xs, c, x_shift), x);
+        unpack<T>(row_piece<kAligned>(ds, c, d_shift), d);
+        if (!kAligned && c == last) cut(x, valid), cut(d, valid);
         const ulonglong2* g = reinterpret_cast<const ulonglong2*>(gain + c * V);
 #pragma unroll
         for (int k = 0; k < P; ++k) {
@@ -527,14 +620,17 @@ __global__ void __launch_bounds__(kRingThreads < TPR ? TPR : kRingThreads) layer
     // dx = w rstd - (s1 + xhat s2) rstd = d g rstd + (x (-s2 rstd rstd) + (mean rstd s2 - s1) rstd)
     const float m1 = sums[0] * inv_c, m2 = sums[1] * inv_c;
     const uint64_t a2 = f2(-m2, -m2), a1 = f2(-m1, -m1);
-    uint4* dx = reinterpret_cast<uint4*>(static_cast<T*>(a.dx) + (sample_row + r) * a.C);
+    T* dx = static_cast<T*>(a.dx) + (sample_row + r) * a.C;
+    unsigned char* staged = smem + lay.out + group * lay.row;
+    uint4* to = kAligned ? reinterpret_cast<uint4*>(dx) : reinterpret_cast<uint4*>(staged);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = i * TPR + t;
       if (c < nvec) {
         uint64_t x[P], d[P];
-        unpack<T>(xs[c], x);
-        unpack<T>(ds[c], d);
+        unpack<T>(row_piece<kAligned>(xs, c, x_shift), x);
+        unpack<T>(row_piece<kAligned>(ds, c, d_shift), d);
+        if (!kAligned && c == last) cut(x, valid), cut(d, valid);
         const ulonglong2* g = reinterpret_cast<const ulonglong2*>(gain + c * V);
 #pragma unroll
         for (int k = 0; k < P; ++k) {
@@ -542,10 +638,12 @@ __global__ void __launch_bounds__(kRingThreads < TPR ? TPR : kRingThreads) layer
           const uint64_t h = fma2(x[k], rs, shift);
           d[k] = mul2(fma2(h, a2, fma2(d[k], k & 1 ? gv.y : gv.x, a1)), rs);
         }
-        if (ok) dx[c] = pack<T>(d);
+        if (ok || !kAligned) to[c] = pack<T>(d);
       }
     }
     group_sync<TPR>(group);                                // the row has been read: its place takes another
+    if (!kAligned && ok) store_row<T, TPR>(dx, staged, a.C, t);
+    if (!kAligned && TPR == 32) __syncwarp();
     if (t == 0 && ahead < n && ok) {
       fetch(ahead, s);
       ahead += step;
@@ -557,7 +655,7 @@ __global__ void __launch_bounds__(kRingThreads < TPR ? TPR : kRingThreads) layer
   if (a.partial) {
     // the groups of the CTA are added in shared memory, in order
     __syncthreads();
-    float* acc = reinterpret_cast<float*>(smem + lay.ring);                            // [dg, do][C]: fits the ring
+    float* acc = reinterpret_cast<float*>(smem + lay.ring);                            // [dg, do][columns]: fits the ring
     for (int k = 0; k < G; ++k) {
       if (k == group) {
 #pragma unroll
@@ -565,7 +663,7 @@ __global__ void __launch_bounds__(kRingThreads < TPR ? TPR : kRingThreads) layer
           const int c = i * TPR + t;
           if (c < nvec) {
             ulonglong2* p = reinterpret_cast<ulonglong2*>(acc + c * V);
-            ulonglong2* q = reinterpret_cast<ulonglong2*>(acc + a.C + c * V);
+            ulonglong2* q = reinterpret_cast<ulonglong2*>(acc + lay.columns + c * V);
 #pragma unroll
             for (int j = 0; j < P; j += 2) {
               ulonglong2 u = make_ulonglong2(dg[i][j], dg[i][j + 1]), w = make_ulonglong2(dof[i][j], dof[i][j + 1]);
@@ -583,7 +681,7 @@ __global__ void __launch_bounds__(kRingThreads < TPR ? TPR : kRingThreads) layer
       __syncthreads();
     }
     float* out = a.partial + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 * a.C;
-    for (int c = threadIdx.x; c < 2 * a.C; c += kRingThreads) out[c] = acc[c];
+    for (int c = threadIdx.x; c < 2 * a.C; c += kRingThreads) out[c] = acc[c < a.C ? c : c - a.C + lay.columns];
   }
   leave(bars, stages, issued, t, abort_flag, a.status);
 }
@@ -675,16 +773,17 @@ cudaError_t backward_v(const NormArgs& a, int groups, int parts, cudaStream_t st
 }
 
 // Threads per row of the ring kernels: at most 80 elements a thread forward (75,600 x 5,120: 128 threads 306 us, 64 threads
-// 284), 40 backward (with two sums each).
+// 284); backward 80 bytes a thread and tensor (40 elements with two sums each; 32-bit rows take twice the place in the ring, and
+// twice the threads keep two CTAs on an SM: 2 x 4,097 x 1,001 54 us with one).
 constexpr int kRingColumns = 8192;
 int ring_threads_forward(int C) { return C <= 32 * 64 ? 32 : C <= 64 * 80 ? 64 : 128; }
-int ring_threads_backward(int C) { return C <= 32 * 40 ? 32 : C <= 64 * 40 ? 64 : C <= 128 * 40 ? 128 : 256; }
+int ring_threads_backward(int C, int e) { return C * e <= 32 * 80 ? 32 : C * e <= 64 * 80 ? 64 : C * e <= 128 * 80 ? 128 : 256; }
 // Stages of the backward ring: three where two CTAs of them still fit an SM, else two.
-int backward_stages(int C, int e, int groups) {
-  return 2 * (RingLayout(C, e, 1, 2, groups, kBackwardStages).total + 1536) <= 232448 ? kBackwardStages : 2;
+int backward_stages(int C, int e, int groups, bool aligned) {
+  return 2 * (RingLayout(C, e, 1, 2, groups, kBackwardStages, aligned).total + 1536) <= 232448 ? kBackwardStages : 2;
 }
 // CTAs of a kernel that the SMs hold at this much shared memory; the answer for the last size is kept.
-constexpr int kRingSmem = 200 * 1024;
+constexpr int kRingSmem = 230000;                  // above what any layout needs (205,000: forward, fp32, 5,120 unaligned columns)
 template <typename Kernel>
 cudaError_t resident(Kernel* kernel, int smem, int64_t& kept, int& ctas) {
   const int64_t known = __atomic_load_n(&kept, __ATOMIC_RELAXED);
@@ -705,58 +804,59 @@ cudaError_t launch_ring(Kernel* kernel, const NormArgs& a, int64_t ctas, int gro
   count_launches(1);
   return launch_pdl(kernel, dim3((unsigned)ctas, (unsigned)groups), dim3(kRingThreads), smem, st, a);
 }
-template <typename T, int NV, int TPR>
+template <typename T, bool kAligned, int NV, int TPR>
 cudaError_t forward_ring(NormArgs a, cudaStream_t st) {
   constexpr int G = kRingThreads / TPR;
   static int64_t kept;
   const int samples = a.gain_batch || a.offset_batch ? (int)a.batch : 1;
   a.stages = kForwardStages;
-  const int smem = RingLayout(a.C, sizeof(T), 2, 1, G, a.stages).total;
+  const int smem = RingLayout(a.C, sizeof(T), 2, 1, G, a.stages, kAligned).total;
   int fit = 0;
   static uint64_t done;
-  cudaError_t e = allow_smem(&layer_norm_ring_kernel<T, NV, TPR>, kRingSmem, done);
-  if (e == cudaSuccess) e = resident(&layer_norm_ring_kernel<T, NV, TPR>, smem, kept, fit);
+  cudaError_t e = allow_smem(&layer_norm_ring_kernel<T, NV, TPR, kAligned>, kRingSmem, done);
+  if (e == cudaSuccess) e = resident(&layer_norm_ring_kernel<T, NV, TPR, kAligned>, smem, kept, fit);
   if (e != cudaSuccess) return e;
   const int64_t jobs = ceil_div64(samples > 1 ? a.rows : a.batch * a.rows, G), ctas = ceil_div64(fit, samples);
-  return launch_ring(&layer_norm_ring_kernel<T, NV, TPR>, a, jobs < ctas ? jobs : ctas, samples, smem, st);
+  return launch_ring(&layer_norm_ring_kernel<T, NV, TPR, kAligned>, a, jobs < ctas ? jobs : ctas, samples, smem, st);
 }
-template <typename T>
+template <typename T, bool kAligned>
 cudaError_t forward_ring_t(const NormArgs& a, cudaStream_t st) {
   constexpr int V = 16 / (int)sizeof(T), Q = 8 / V;          // pieces per 8 elements
-  const int tpr = ring_threads_forward(a.C), nv = ceil_div(a.C / V, tpr);
+  const int tpr = ring_threads_forward(a.C), nv = ceil_div(ceil_div(a.C, V), tpr);
   if (tpr == 32) {
-    if (nv <= 2 * Q) return forward_ring<T, 2 * Q, 32>(a, st);
-    if (nv <= 4 * Q) return forward_ring<T, 4 * Q, 32>(a, st);
-    if (nv <= 6 * Q) return forward_ring<T, 6 * Q, 32>(a, st);
-    return forward_ring<T, 8 * Q, 32>(a, st);
+    if (nv <= 2 * Q) return forward_ring<T, kAligned, 2 * Q, 32>(a, st);
+    if (nv <= 4 * Q) return forward_ring<T, kAligned, 4 * Q, 32>(a, st);
+    if (nv <= 6 * Q) return forward_ring<T, kAligned, 6 * Q, 32>(a, st);
+    return forward_ring<T, kAligned, 8 * Q, 32>(a, st);
   }
-  if (tpr == 64) return nv <= 6 * Q ? forward_ring<T, 6 * Q, 64>(a, st) : forward_ring<T, 10 * Q, 64>(a, st);
-  return forward_ring<T, 8 * Q, 128>(a, st);
+  if (tpr == 64) return nv <= 6 * Q ? forward_ring<T, kAligned, 6 * Q, 64>(a, st) : forward_ring<T, kAligned, 10 * Q, 64>(a, st);
+  return forward_ring<T, kAligned, 8 * Q, 128>(a, st);
 }
-template <typename T, int NV, int TPR>
+template <typename T, bool kAligned, int NV, int TPR>
 cudaError_t backward_ring(NormArgs a, int groups, int parts, cudaStream_t st) {
   constexpr int G = kRingThreads / TPR;
-  a.stages = backward_stages(a.C, sizeof(T), G);
+  a.stages = backward_stages(a.C, sizeof(T), G, kAligned);
   static uint64_t done;
-  const cudaError_t e = allow_smem(&layer_norm_backward_ring_kernel<T, NV, TPR>, kRingSmem, done);
+  const cudaError_t e = allow_smem(&layer_norm_backward_ring_kernel<T, NV, TPR, kAligned>, kRingSmem, done);
   if (e != cudaSuccess) return e;
-  return launch_ring(&layer_norm_backward_ring_kernel<T, NV, TPR>, a, parts, groups, RingLayout(a.C, sizeof(T), 1, 2, G, a.stages).total, st);
+  return launch_ring(&layer_norm_backward_ring_kernel<T, NV, TPR, kAligned>, a, parts, groups, RingLayout(a.C, sizeof(T), 1, 2, G, a.stages, kAligned).total, st);
 }
-template <typename T>
+template <typename T, bool kAligned>
 cudaError_t backward_ring_t(const NormArgs& a, int groups, int parts, cudaStream_t st) {
   constexpr int V = 16 / (int)sizeof(T), Q = 8 / V;
-  const int tpr = ring_threads_backward(a.C);
-  const bool few = ceil_div(a.C / V, tpr) <= 3 * Q;
+  const int tpr = ring_threads_backward(a.C, sizeof(T));
+  const bool few = ceil_div(ceil_div(a.C, V), tpr) <= 3 * Q;
   switch (tpr) {
-    case 32: return few ? backward_ring<T, 3 * Q, 32>(a, groups, parts, st) : backward_ring<T, 5 * Q, 32>(a, groups, parts, st);
-    case 64: return few ? backward_ring<T, 3 * Q, 64>(a, groups, parts, st) : backward_ring<T, 5 * Q, 64>(a, groups, parts, st);
-    case 128: return few ? backward_ring<T, 3 * Q, 128>(a, groups, parts, st) : backward_ring<T, 5 * Q, 128>(a, groups, parts, st);
-    default: return few ? backward_ring<T, 3 * Q, 256>(a, groups, parts, st) : backward_ring<T, 5 * Q, 256>(a, groups, parts, st);
+    case 32: return few ? backward_ring<T, kAligned, 3 * Q, 32>(a, groups, parts, st) : backward_ring<T, kAligned, 5 * Q, 32>(a, groups, parts, st);
+    case 64: return few ? backward_ring<T, kAligned, 3 * Q, 64>(a, groups, parts, st) : backward_ring<T, kAligned, 5 * Q, 64>(a, groups, parts, st);
+    case 128: return few ? backward_ring<T, kAligned, 3 * Q, 128>(a, groups, parts, st) : backward_ring<T, kAligned, 5 * Q, 128>(a, groups, parts, st);
+    default: return few ? backward_ring<T, kAligned, 3 * Q, 256>(a, groups, parts, st) : backward_ring<T, kAligned, 5 * Q, 256>(a, groups, parts, st);
   }
 }
-// Rows that the ring can fetch: whole 16-byte pieces, everywhere.  (The strides of parameters do not matter to it.)
-bool ring_rows(const NormArgs& a, int e) {
-  if (a.C > kRingColumns || a.batch * a.rows > INT32_MAX - (1 << 20)) return false;
+// Whether the ring kernels take these rows, and whether all of them are whole 16-byte pieces.  (The strides of parameters do not
+// matter to them.)
+bool ring_fits(int64_t batch, int64_t rows, int C) { return C <= kRingColumns && batch * rows <= INT32_MAX - (1 << 20); }
+bool ring_aligned(const NormArgs& a, int e) {
   for (int64_t stride : {(int64_t)a.C, a.x_batch, a.x_row, a.dy_batch, a.dy_row})
     if (stride * e % 16) return false;
   for (const void* p : {a.x, a.dy, (const void*)a.y, (const void*)a.dx})
@@ -768,36 +868,38 @@ bool ring_rows(const NormArgs& a, int e) {
   (type == SVOO_TYPE_BF16 ? (v == 8 ? fn<__nv_bfloat16, 8>(__VA_ARGS__) : v == 2 ? fn<__nv_bfloat16, 2>(__VA_ARGS__) : fn<__nv_bfloat16, 1>(__VA_ARGS__)) \
    : type == SVOO_TYPE_FP16 ? (v == 8 ? fn<__half, 8>(__VA_ARGS__) : v == 2 ? fn<__half, 2>(__VA_ARGS__) : fn<__half, 1>(__VA_ARGS__))                    \
                             : (v == 4 ? fn<float, 4>(__VA_ARGS__) : fn<float, 1>(__VA_ARGS__)))
-#define SVOO_RING(fn, ...) \
-  (type == SVOO_TYPE_BF16 ? fn<__nv_bfloat16>(__VA_ARGS__) : type == SVOO_TYPE_FP16 ? fn<__half>(__VA_ARGS__) : fn<float>(__VA_ARGS__))
+#define SVOO_RING(fn, aligned, ...) \
+  (type == SVOO_TYPE_BF16 ? (aligned ? fn<__nv_bfloat16, true>(__VA_ARGS__) : fn<__nv_bfloat16, false>(__VA_ARGS__)) \
+   : type == SVOO_TYPE_FP16 ? (aligned ? fn<__half, true>(__VA_ARGS__) : fn<__half, false>(__VA_ARGS__))             \
+                            : (aligned ? fn<float, true>(__VA_ARGS__) : fn<float, false>(__VA_ARGS__)))
 }  // namespace
 
-// CTAs per group of the backward kernels: what the SMs hold at once, at most one per row (ring: per row of every group).
+// CTAs per group of the backward kernels: what the SMs hold at once, at most one per row (ring: per row of every group, as many
+// as for 32-bit rows whatever the type, so that the workspace does not depend on it).
 int norm_backward_parts(int64_t rows, int groups, int C, bool ring) {
   const int t = backward_threads(C);
   const int per_sm = ring ? 2 : t >= 1024 ? 1 : 1024 / t > 16 ? 16 : 1024 / t;
-  int64_t parts = (int64_t)148 * per_sm / groups, jobs = ring ? ceil_div64(rows, kRingThreads / ring_threads_backward(C)) : rows;
+  int64_t parts = (int64_t)148 * per_sm / groups, jobs = ring ? ceil_div64(rows, kRingThreads / ring_threads_backward(C, 4)) : rows;
   if (parts > jobs) parts = jobs;
   return parts < 1 ? 1 : (int)parts;
 }
-// The workspace holds what either kernel leaves, so that its size does not depend on alignment.
-int64_t norm_backward_bytes(int64_t rows, int groups, int C) {
-  const int a = norm_backward_parts(rows, groups, C, false), b = norm_backward_parts(rows, groups, C, true);
-  return (int64_t)groups * (a > b ? a : b) * 2 * C * 4;
+int64_t norm_backward_bytes(int64_t batch, int64_t rows, int groups, int C) {
+  const bool ring = ring_fits(batch, rows, C);
+  return (int64_t)groups * norm_backward_parts(groups > 1 ? rows : batch * rows, groups, C, ring) * 2 * C * 4;
 }
 
 cudaError_t launch_layer_norm(int type, const NormArgs& a, cudaStream_t st) {
   const int e = elem_bytes(type);
-  if (ring_rows(a, e)) return SVOO_RING(forward_ring_t, a, st);
+  if (ring_fits(a.batch, a.rows, a.C)) return SVOO_RING(forward_ring_t, ring_aligned(a, e), a, st);
   const int v = norm_vector(a, e);
   return SVOO_NORM(forward_v, a, st);
 }
 
 cudaError_t launch_layer_norm_backward(int type, const NormArgs& a, int groups, void* dgain, void* doffset, cudaStream_t st) {
   const int elem = elem_bytes(type), v = norm_vector(a, elem);
-  const bool ring = ring_rows(a, elem);
+  const bool ring = ring_fits(a.batch, a.rows, a.C), aligned = ring_aligned(a, elem);
   const int parts = norm_backward_parts(groups > 1 ? a.rows : a.batch * a.rows, groups, a.C, ring);
-  const cudaError_t e = ring ? SVOO_RING(backward_ring_t, a, groups, parts, st) : SVOO_NORM(backward_v, a, groups, parts, st);
+  const cudaError_t e = ring ? SVOO_RING(backward_ring_t, aligned, a, groups, parts, st) : SVOO_NORM(backward_v, a, groups, parts, st);
   if (e != cudaSuccess || !a.partial) return e;
   const dim3 grid((unsigned)ceil_div(a.C, 32), (unsigned)groups, 2);
   const bool f32 = a.params_fp32 || type == SVOO_TYPE_FP32;

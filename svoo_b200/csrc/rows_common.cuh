@@ -11,6 +11,7 @@ namespace svoo {
 // Layer norm and its gradient (norm.cu)
 struct NormArgs {
   const void *x, *dy, *gain, *offset;
+  const void *x_end, *dy_end;                   // the byte behind the last element
   const float *mean_in, *rstd_in;
   void *y, *dx;
   float *mean, *rstd, *partial;
