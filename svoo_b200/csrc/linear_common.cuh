@@ -125,31 +125,39 @@ __device__ __forceinline__ float max_magnitude(float top, uint64_t v) {
   return top;
 }
 // x / s of values that are themselves rounded sums: one correction by the remainder, which leaves half a unit and 2^-22 of
-// one (BlockDivide makes it half a unit).  The scale as block_scale gives it.
+// one (BlockDivide makes it half a unit).  s >= 2^-90, as BlockDivide wants it; the scale as block_scale gives it.
 struct BlockDivideOnce {
-  uint64_t y, ns;
-  float up;
-  __device__ __forceinline__ explicit BlockDivideOnce(float s) {
-    const BlockDivide d(s);
-    y = pack2(d.y, d.y), ns = pack2(d.ns, d.ns), up = d.up;
-  }
-  __device__ __forceinline__ uint64_t quotient(uint64_t x) const {
-    if (up != 1.f) x = mul2(x, pack2(up, up));
-    const uint64_t q = mul2(x, y);
-    return fma2(fma2(q, ns, x), y, q);
+  float y, ns;
+  __device__ __forceinline__ explicit BlockDivideOnce(float s) : y(BlockDivide::reciprocal(s)), ns(s == INFINITY ? -1.f : -s) {}
+  __device__ __forceinline__ float quotient(float x) const {
+    const float q = x * y;
+    return fmaf(fmaf(q, ns, x), y, q);
   }
   __device__ __forceinline__ uint32_t e4m3x4(uint64_t a, uint64_t b) const {
-    a = quotient(a), b = quotient(b);
-    return e4m3x2(half_of(a, 0), half_of(a, 1)) | e4m3x2(half_of(b, 0), half_of(b, 1)) << 16;
+    return e4m3x2(quotient(half_of(a, 0)), quotient(half_of(a, 1))) | e4m3x2(quotient(half_of(b, 0)), quotient(half_of(b, 1))) << 16;
   }
 };
 
-// Plain loads: the 16-bit forms of __ldg are assembly that the compiler may move in front of the condition on a.bias.
-__device__ __forceinline__ float load_bias(const LinearArgs& a, int n) {
-  if (!a.bias || n >= a.N) return 0.f;
-  if (a.bias_type == SVOO_TYPE_FP32) return static_cast<const float*>(a.bias)[n];
-  if (a.bias_type == SVOO_TYPE_BF16) return to_f32(static_cast<const __nv_bfloat16*>(a.bias)[n]);
-  return to_f32(static_cast<const __half*>(a.bias)[n]);
+// bias of columns n, n + step, ..., zero where there is none; the loads go out together.  Plain loads: the 16-bit forms of __ldg are
+// assembly that the compiler may move in front of the condition on a.bias.
+template <typename T, int COUNT>
+__device__ __forceinline__ void bias_columns_of(const LinearArgs& a, int n, int step, float (&v)[COUNT]) {
+  const T* p = static_cast<const T*>(a.bias);
+  T raw[COUNT];
+#pragma unroll
+  for (int i = 0; i < COUNT; ++i)
+    if (n + i * step < a.N) raw[i] = p[n + i * step];
+#pragma unroll
+  for (int i = 0; i < COUNT; ++i) v[i] = n + i * step < a.N ? to_f32(raw[i]) : 0.f;
+}
+template <int COUNT>
+__device__ __forceinline__ void bias_columns(const LinearArgs& a, int n, int step, float (&v)[COUNT]) {
+#pragma unroll
+  for (int i = 0; i < COUNT; ++i) v[i] = 0.f;
+  if (!a.bias) return;
+  if (a.bias_type == SVOO_TYPE_FP32) bias_columns_of<float>(a, n, step, v);
+  else if (a.bias_type == SVOO_TYPE_BF16) bias_columns_of<__nv_bfloat16>(a, n, step, v);
+  else bias_columns_of<__half>(a, n, step, v);
 }
 
 }  // namespace tc

@@ -129,7 +129,9 @@ __global__ void __launch_bounds__(kFewWarps * 32) linear_few_kernel(const T* __r
     float v = 0.f;
 #pragma unroll
     for (int i = 0; i < kFewWarps; ++i) v += part[i][r][o % NW];
-    v += tc::load_bias(a, n);
+    float bias[1];
+    tc::bias_columns(a, n, 1, bias);
+    v += bias[0];
     if (gelu) v = tc::half_of(tc::gelu2(tc::pack2(v, v)), 0);
     const int64_t at = r * a.out_pitch + n;
     if (out_type == SVOO_TYPE_FP32) static_cast<float*>(a.out)[at] = v;

@@ -157,8 +157,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) linear_split_kernel(const __
   const int rows = a.M - row0 < kSplitM ? a.M - row0 : kSplitM;
   const int n = n0 + lane * 4;
   float bias[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) bias[i] = load_bias(a, n + i);
+  bias_columns(a, n, 1, bias);
   const int r1 = rows * (rank + 1) / ranks;
   for (int r = rows * rank / ranks + warp; r < r1; r += kSplitThreads / 32) {
     const uint32_t at = base + r * kSplitN * 4 + ((lane ^ (r & 31)) << 4);
@@ -186,7 +185,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) linear_split_kernel(const __
       const float s = block_scale(top);
       if (lane == 0) a.out_scale[tn * a.out_scale_pitch + row0 + r] = s;
       if (n < ((a.N + 15) & ~15))
-        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + (int64_t)(row0 + r) * a.out_pitch + n) = BlockDivideOnce(s).e4m3x4(pack2(v[0], v[1]), pack2(v[2], v[3]));
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + (int64_t)(row0 + r) * a.out_pitch + n) = BlockDivide(s).e4m3x4(v[0], v[1], v[2], v[3]);
     } else {
       typedef typename ElemOf<OUT>::T T;
       T* dst = static_cast<T*>(a.out) + (int64_t)(row0 + r) * a.out_pitch + n;

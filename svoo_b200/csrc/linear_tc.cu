@@ -216,13 +216,15 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
       int i = 0;
       for (int t = worker; t < tiles; t += workers, ++i) {
         const LinTile tile(t, tiles_m, tiles_n);
-        float v[TN / 32];
-#pragma unroll
-        for (int k = 0; k < TN / 32; ++k) v[k] = load_bias(a, tile.tn * TN + k * 32 + lane);
         if (!__all_sync(0xffffffffu, mbar_wait(bar(C::BIAS_EMPTY + (i & 1)), ((i >> 1) & 1) ^ 1, abort_flag))) break;
-        float* dst = reinterpret_cast<float*>(gen + C::kBias) + (i & 1) * TN;
+        float* dst = reinterpret_cast<float*>(gen + C::kBias) + (i & 1) * TN + lane;
+#pragma unroll 1
+        for (int k = 0; k < TN; k += 128) {                // four loads at a time: these warps have few registers
+          float v[4];
+          bias_columns(a, tile.tn * TN + k + lane, 32, v);
 #pragma unroll
-        for (int k = 0; k < TN / 32; ++k) dst[k * 32 + lane] = v[k];
+          for (int j = 0; j < 4; ++j) dst[k + j * 32] = v[j];
+        }
         mbar_arrive(bar(C::BIAS_FULL + (i & 1)));
       }
     }
@@ -330,7 +332,12 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
         }
         const float s = block_scale(__float_as_uint(top) & 0x7fffffffu);
         if (row < a.M && !skip) a.out_scale[(n0 / 128) * a.out_scale_pitch + row] = s;
-        const BlockDivideOnce by(s);
+        const bool tiny = s < 0x1p-90f;
+        if (tiny) {
+#pragma unroll
+          for (int i = 0; i < HC / 2; ++i) sum[i] = mul2(sum[i], pack2(0x1p64f, 0x1p64f));
+        }
+        const BlockDivideOnce by(tiny ? s * 0x1p64f : s);
         unsigned char* at = begin_box(n_tile);
 #pragma unroll
         for (int p = 0; p < 8; ++p) {

@@ -132,3 +132,20 @@ def test_token_wise_entry_points_check_their_arguments():
     lin = lambda **k: L.svoo_b200_linear_fp8(*{**few, **k}.values())                      # noqa: E731
     assert lin(M=0) == 0 and lin(x=None) == -1 and lin(b=None) == -1 and lin(out=None) == -1 and lin(bp=72) == -2 and lin(t=3) == -8
     assert lin(M=17) == -1 and lin(M=17, ws=p, wb=16) == -4 and lin(ot=3) == -1 and lin(K=0) == -2 and lin(b=p + 8) == -5
+
+
+def test_product_kernels_do_not_spill():
+    """tcgen05.ld fills registers behind the instruction stream: code that issues it must not spill (a register could be saved
+    before it is filled).  The register shares that setmaxnreg deals out add up to a launch at 168 registers a thread."""
+    import os
+    import re
+    import subprocess
+    from svoo_b200 import build
+    for src, kernels in (("linear_tc.cu", 11), ("linear_split.cu", 8)):
+        res = subprocess.run([build._nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-Xptxas", "-v", "-c",
+                              os.path.join(build.CSRC, src), "-o", os.devnull], capture_output=True, text=True)
+        assert res.returncode == 0, res.stderr
+        spills = re.findall(r"(\d+) bytes spill stores, (\d+) bytes spill loads", res.stderr)
+        assert len(spills) >= kernels and all(s == ("0", "0") for s in spills), res.stderr
+        if src == "linear_tc.cu":
+            assert set(re.findall(r"Used (\d+) registers", res.stderr)) == {"168"}
