@@ -395,15 +395,16 @@ int svoo_b200_peer_barrier(void* const* peer_flags, int32_t world, int32_t rank,
 /* y = (x - mean) rstd g + o over the last dimension, rstd = 1 / sqrt(var + eps), var around the mean / C; statistics in
  * 32 bits.  x: [batch, rows, C] of x_type, last dimension dense, rows x_row and samples x_batch apart; y: dense, x_type.
  * gain, offset: C values of param_type (SVOO_TYPE_FP32 or x_type) per sample, gain_batch / offset_batch apart (0: one row for
- * all); null: 1 and 0.  gain_plus_one: g = 1 + gain (AdaLN).  mean, rstd: fp32 [batch * rows], both or none.  C <= 16384.
+ * all); null: 1 and 0.  gain_plus_one: g = 1 + gain (AdaLN).  mean, rstd: fp32 [batch * rows], both or none.  C <= 16384;
+ * at most 65,535 samples with parameters of their own.
  * (fp32 layer norm and modulation of the block, svoo/models/wan/custom_models.py:22-108) */
 int svoo_b200_layer_norm(const void* x, int32_t x_type, int64_t batch, int64_t rows, int64_t C, int64_t x_batch, int64_t x_row,
                          const void* gain, int64_t gain_batch, const void* offset, int64_t offset_batch, int32_t param_type,
                          int32_t gain_plus_one, float eps, void* y, float* mean, float* rstd, void* stream);
 /* Its gradient: dx (dense, x_type) from dy [batch, rows, C] (x_type, last dimension dense), x and the statistics of the
  * forward call.  dgain, doffset (param_type; both or none): sums over the rows of each sample, [batch, C], where
- * per_sample != 0, otherwise over all rows, [C].  The sums run in a fixed order.  workspace: layer_norm_workspace_bytes,
- * needed with dgain. */
+ * per_sample != 0, otherwise over all rows, [C].  The sums run in a fixed order; with batch 0 nothing is written.
+ * workspace: layer_norm_workspace_bytes, needed with dgain. */
 int svoo_b200_layer_norm_workspace_bytes(int64_t batch, int64_t rows, int64_t C, int32_t per_sample, int64_t* bytes_out);
 int svoo_b200_layer_norm_backward(const void* dy, int64_t dy_batch, int64_t dy_row, const void* x, int32_t x_type, int64_t batch,
                                   int64_t rows, int64_t C, int64_t x_batch, int64_t x_row, const float* mean, const float* rstd,

@@ -35,13 +35,13 @@ bool element(int type) { return type == SVOO_TYPE_BF16 || type == SVOO_TYPE_FP16
 int check_norm(int32_t x_type, int64_t batch, int64_t rows, int64_t C, int64_t x_batch, int64_t x_row, int32_t param_type, bool per_sample) {
   if (!element(x_type) || (param_type != SVOO_TYPE_FP32 && param_type != x_type)) return SVOO_ERR_TYPE;
   if (batch < 0 || rows < 0 || C < 1 || C > SVOO_MAX_NORM_COLUMNS || x_batch < 0 || x_row < 0) return SVOO_ERR_SHAPE;
-  if (rows > kMaxRows || batch > kMaxRows || batch * rows > (int64_t)INT32_MAX || (per_sample && batch > 65535)) return SVOO_ERR_SHAPE;
+  if (rows > kMaxRows || batch > kMaxRows || batch * rows > (int64_t)INT32_MAX - (1 << 20) || (per_sample && batch > 65535)) return SVOO_ERR_SHAPE;
   return SVOO_OK;
 }
 int check_quant(const void* x, int32_t type, int64_t M, int64_t K, int64_t x_row, const void* q, int64_t q_pitch, int64_t q_cols, const float* scale) {
   if (!element(type)) return SVOO_ERR_TYPE;
   if (M < 0 || K < 1 || M > kMaxRows || K > kMaxRows || x_row < 0 || q_pitch < q_cols || q_pitch % 16) return SVOO_ERR_SHAPE;
-  if (M * ceil_div64(K, 128) > (int64_t)INT32_MAX - 16) return SVOO_ERR_SHAPE;
+  if (M * ceil_div64(K, 128) > (int64_t)INT32_MAX - 1024) return SVOO_ERR_SHAPE;     // blocks are counted in 32 bits
   if (M == 0) return SVOO_OK;
   if (!x || !q || !scale) return SVOO_ERR_NULL;
   if (!aligned(q, 16) || !aligned(x, elem_bytes(type)) || !aligned(scale, 4)) return SVOO_ERR_ALIGN;
@@ -80,7 +80,7 @@ extern "C" {
 int svoo_b200_layer_norm(const void* x, int32_t x_type, int64_t batch, int64_t rows, int64_t C, int64_t x_batch, int64_t x_row,
                          const void* gain, int64_t gain_batch, const void* offset, int64_t offset_batch, int32_t param_type,
                          int32_t gain_plus_one, float eps, void* y, float* mean, float* rstd, void* stream) {
-  SVOO_TRY(check_norm(x_type, batch, rows, C, x_batch, x_row, param_type, false));
+  SVOO_TRY(check_norm(x_type, batch, rows, C, x_batch, x_row, param_type, gain_batch != 0 || offset_batch != 0));
   if (batch * rows == 0) return SVOO_OK;
   if (!x || !y || !mean != !rstd) return SVOO_ERR_NULL;
   if (gain_batch < 0 || offset_batch < 0) return SVOO_ERR_SHAPE;

@@ -34,7 +34,6 @@ __device__ __forceinline__ void load_param(const void* p, bool fp32, int64_t at,
 template <int TPR>
 __device__ __forceinline__ float row_sum(float s, float* slot, int t) {
   s = warp_sum(s);
-  if (TPR == 32) return s;
   if (t % 32 == 0) slot[t / 32] = s;
   __syncthreads();
   s = 0.f;
@@ -43,16 +42,19 @@ __device__ __forceinline__ float row_sum(float s, float* slot, int t) {
   return s;
 }
 
-// TPR threads hold one row, NV vectors of V elements each, vector i of thread t at (i * TPR + t) * V.
-template <typename T, int V, int NV, int TPR>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) layer_norm_kernel(const NormArgs a) {
-  constexpr int G = TPR < 128 ? 128 / TPR : 1;
-  __shared__ float slots[2][G][TPR / 32];
+// ---- rows of more than 8,192 columns: a CTA per row, straight from global memory ------------------------------------------
+//
+// Vector i of thread t, of NV with V elements each, lies at (i * threads + t) * V.
+constexpr int kWideThreads = 256, kWideColumns = 64;               // 16,384 columns
+constexpr int kWideBackwardThreads = 1024, kWideBackwardColumns = 16;
+template <typename T, int V, int NV>
+__global__ void __launch_bounds__(kWideThreads) layer_norm_kernel(const NormArgs a) {
+  constexpr int TPR = kWideThreads;
+  __shared__ float slots[2][TPR / 32];
   pdl_trigger();
   pdl_wait();
-  const int g = threadIdx.x / TPR, t = threadIdx.x % TPR;
-  const int64_t row = (int64_t)blockIdx.x * G + g;
-  if (G > 1 && row >= a.batch * a.rows) return;          // whole warps: a row is one warp there
+  const int t = threadIdx.x;
+  const int64_t row = blockIdx.x;
   const int64_t b = a.batch == 1 ? 0 : row / a.rows;
   const T* x = static_cast<const T*>(a.x) + b * a.x_batch + (row - b * a.rows) * a.x_row;
   const int nvec = a.C / V;
@@ -75,7 +77,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) layer_norm_kernel(const
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int k = 0; k < V; ++k) s += v[i][k];
-  const float mean = row_sum<TPR>(s, slots[0][g], t) / a.C;
+  const float mean = row_sum<TPR>(s, slots[0], t) / a.C;
   float q = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -87,7 +89,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) layer_norm_kernel(const
       }
     }
   }
-  const float rstd = 1.f / sqrtf(row_sum<TPR>(q, slots[1][g], t) / a.C + a.eps);
+  const float rstd = 1.f / sqrtf(row_sum<TPR>(q, slots[1], t) / a.C + a.eps);
   if (t == 0 && a.mean) {
     a.mean[row] = mean;
     a.rstd[row] = rstd;
@@ -114,12 +116,13 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) layer_norm_kernel(const
   }
 }
 
-// One CTA of TPR threads walks the rows blockIdx.x, + gridDim.x, ... of group blockIdx.y (a sample where the modulation is
+// A CTA walks the rows blockIdx.x, + gridDim.x, ... of group blockIdx.y (a sample where the modulation is
 // per sample, otherwise all rows) and keeps the column sums of its rows in registers; they go to `partial`
 // [group][CTA][dg, do][C], which column_sum_kernel adds in a fixed order.  The next row is fetched before this one's two
 // sums are joined.
-template <typename T, int V, int NV, int TPR>
-__global__ void __launch_bounds__(TPR) layer_norm_backward_kernel(const NormArgs a) {
+template <typename T, int V, int NV>
+__global__ void __launch_bounds__(kWideBackwardThreads) layer_norm_backward_kernel(const NormArgs a) {
+  constexpr int TPR = kWideBackwardThreads;
   __shared__ float slots[2][2][TPR / 32];
   pdl_trigger();
   pdl_wait();
@@ -184,13 +187,11 @@ __global__ void __launch_bounds__(TPR) layer_norm_backward_kernel(const NormArgs
     if (r + gridDim.x < n) fetch(r + gridDim.x);
     s1 = warp_sum(s1);
     s2 = warp_sum(s2);
-    if (TPR > 32) {
-      if (t % 32 == 0) slots[buf][0][t / 32] = s1, slots[buf][1][t / 32] = s2;
-      __syncthreads();                                   // the other buffer is written only after the next row's barrier
-      s1 = s2 = 0.f;
+    if (t % 32 == 0) slots[buf][0][t / 32] = s1, slots[buf][1][t / 32] = s2;
+    __syncthreads();                                     // the other buffer is written only after the next row's barrier
+    s1 = s2 = 0.f;
 #pragma unroll
-      for (int k = 0; k < TPR / 32; ++k) s1 += slots[buf][0][k], s2 += slots[buf][1][k];
-    }
+    for (int k = 0; k < TPR / 32; ++k) s1 += slots[buf][0][k], s2 += slots[buf][1][k];
     s1 /= a.C;
     s2 /= a.C;
     T* dx = static_cast<T*>(a.dx) + (per_sample ? blockIdx.y * a.rows + r : r) * a.C;
@@ -734,42 +735,16 @@ int norm_vector(const NormArgs& a, int e) {
   return 1;
 }
 
-template <typename T, int V, int NF, int TPR>
-cudaError_t forward(const NormArgs& a, cudaStream_t st) {
-  constexpr int G = TPR < 128 ? 128 / TPR : 1;
-  count_launches(1);
-  return launch_pdl(layer_norm_kernel<T, V, NF / V, TPR>, dim3((unsigned)ceil_div64(a.batch * a.rows, G)), dim3(TPR < 128 ? 128 : TPR), 0, st, a);
-}
 template <typename T, int V>
 cudaError_t forward_v(const NormArgs& a, cudaStream_t st) {
-  if (a.C <= 32 * 16) return forward<T, V, 16, 32>(a, st);
-  if (a.C <= 32 * 32) return forward<T, V, 32, 32>(a, st);
-  if (a.C <= 32 * 64) return forward<T, V, 64, 32>(a, st);
-  if (a.C <= 128 * 64) return forward<T, V, 64, 128>(a, st);
-  return forward<T, V, 64, 256>(a, st);
-}
-
-constexpr int kBwdCols = 16;                       // columns per thread of the simple backward kernel
-int backward_threads(int C) {
-  int t = 32;
-  while (t * kBwdCols < C) t *= 2;
-  return t;
-}
-template <typename T, int V, int TPR>
-cudaError_t backward(const NormArgs& a, int groups, int parts, cudaStream_t st) {
   count_launches(1);
-  return launch_pdl(layer_norm_backward_kernel<T, V, kBwdCols / V, TPR>, dim3((unsigned)parts, (unsigned)groups), dim3(TPR), 0, st, a);
+  return launch_pdl(layer_norm_kernel<T, V, kWideColumns / V>, dim3((unsigned)(a.batch * a.rows)), dim3(kWideThreads), 0, st, a);
 }
 template <typename T, int V>
 cudaError_t backward_v(const NormArgs& a, int groups, int parts, cudaStream_t st) {
-  switch (backward_threads(a.C)) {
-    case 32: return backward<T, V, 32>(a, groups, parts, st);
-    case 64: return backward<T, V, 64>(a, groups, parts, st);
-    case 128: return backward<T, V, 128>(a, groups, parts, st);
-    case 256: return backward<T, V, 256>(a, groups, parts, st);
-    case 512: return backward<T, V, 512>(a, groups, parts, st);
-    default: return backward<T, V, 1024>(a, groups, parts, st);
-  }
+  count_launches(1);
+  return launch_pdl(layer_norm_backward_kernel<T, V, kWideBackwardColumns / V>, dim3((unsigned)parts, (unsigned)groups), dim3(kWideBackwardThreads), 0,
+                    st, a);
 }
 
 // Threads per row of the ring kernels: at most 80 elements a thread forward (75,600 x 5,120: 128 threads 306 us, 64 threads
@@ -853,9 +828,7 @@ cudaError_t backward_ring_t(const NormArgs& a, int groups, int parts, cudaStream
     default: return few ? backward_ring<T, kAligned, 3 * Q, 256>(a, groups, parts, st) : backward_ring<T, kAligned, 5 * Q, 256>(a, groups, parts, st);
   }
 }
-// Whether the ring kernels take these rows, and whether all of them are whole 16-byte pieces.  (The strides of parameters do not
-// matter to them.)
-bool ring_fits(int64_t batch, int64_t rows, int C) { return C <= kRingColumns && batch * rows <= INT32_MAX - (1 << 20); }
+// Whether all rows are whole 16-byte pieces.  (The strides of parameters do not matter to the ring kernels.)
 bool ring_aligned(const NormArgs& a, int e) {
   for (int64_t stride : {(int64_t)a.C, a.x_batch, a.x_row, a.dy_batch, a.dy_row})
     if (stride * e % 16) return false;
@@ -876,29 +849,27 @@ bool ring_aligned(const NormArgs& a, int e) {
 
 // CTAs per group of the backward kernels: what the SMs hold at once, at most one per row (ring: per row of every group, as many
 // as for 32-bit rows whatever the type, so that the workspace does not depend on it).
-int norm_backward_parts(int64_t rows, int groups, int C, bool ring) {
-  const int t = backward_threads(C);
-  const int per_sm = ring ? 2 : t >= 1024 ? 1 : 1024 / t > 16 ? 16 : 1024 / t;
-  int64_t parts = (int64_t)148 * per_sm / groups, jobs = ring ? ceil_div64(rows, kRingThreads / ring_threads_backward(C, 4)) : rows;
+int norm_backward_parts(int64_t rows, int groups, int C) {
+  const bool ring = C <= kRingColumns;
+  int64_t parts = (int64_t)148 * (ring ? 2 : 1) / groups, jobs = ring ? ceil_div64(rows, kRingThreads / ring_threads_backward(C, 4)) : rows;
   if (parts > jobs) parts = jobs;
   return parts < 1 ? 1 : (int)parts;
 }
 int64_t norm_backward_bytes(int64_t batch, int64_t rows, int groups, int C) {
-  const bool ring = ring_fits(batch, rows, C);
-  return (int64_t)groups * norm_backward_parts(groups > 1 ? rows : batch * rows, groups, C, ring) * 2 * C * 4;
+  return (int64_t)groups * norm_backward_parts(groups > 1 ? rows : batch * rows, groups, C) * 2 * C * 4;
 }
 
 cudaError_t launch_layer_norm(int type, const NormArgs& a, cudaStream_t st) {
   const int e = elem_bytes(type);
-  if (ring_fits(a.batch, a.rows, a.C)) return SVOO_RING(forward_ring_t, ring_aligned(a, e), a, st);
+  if (a.C <= kRingColumns) return SVOO_RING(forward_ring_t, ring_aligned(a, e), a, st);
   const int v = norm_vector(a, e);
   return SVOO_NORM(forward_v, a, st);
 }
 
 cudaError_t launch_layer_norm_backward(int type, const NormArgs& a, int groups, void* dgain, void* doffset, cudaStream_t st) {
   const int elem = elem_bytes(type), v = norm_vector(a, elem);
-  const bool ring = ring_fits(a.batch, a.rows, a.C), aligned = ring_aligned(a, elem);
-  const int parts = norm_backward_parts(groups > 1 ? a.rows : a.batch * a.rows, groups, a.C, ring);
+  const bool ring = a.C <= kRingColumns, aligned = ring_aligned(a, elem);
+  const int parts = norm_backward_parts(groups > 1 ? a.rows : a.batch * a.rows, groups, a.C);
   const cudaError_t e = ring ? SVOO_RING(backward_ring_t, aligned, a, groups, parts, st) : SVOO_NORM(backward_v, a, groups, parts, st);
   if (e != cudaSuccess || !a.partial) return e;
   const dim3 grid((unsigned)ceil_div(a.C, 32), (unsigned)groups, 2);

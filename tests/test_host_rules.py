@@ -95,6 +95,7 @@ def test_token_wise_entry_points_check_their_arguments():
     assert norm(r=0) == 0 and norm(b=0) == 0
     assert norm(x=None) == -1 and norm(y=None) == -1 and norm(m=p) == -1
     assert norm(C=0) == -2 and norm(C=16385) == -2 and norm(r=-1) == -2 and norm(xr=-1) == -2 and norm(b=1 << 20, r=1 << 20) == -2
+    assert norm(b=70000, r=1, gb=64) == -2 and norm(b=1 << 11, r=1 << 20) == -2
     assert norm(t=3) == -8 and norm(t=0, pt=1) == -8
     assert norm(x=p + 1) == -5 and norm(g=p + 2) == -5
     out = ctypes.c_int64(0)
