@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(kWideBackwardThreads) layer_norm_backward_kern
 // a time, parameters in registers: 243 instructions per 16 bytes, 2.9 TB/s at 32,760 x 5,120.)
 constexpr int kRingThreads = 256;
 constexpr int kForwardStages = 1;                  // the row is in registers at once, so its place is free again: three cost 15 %
-constexpr int kBackwardStages = 3;                 // the row is read twice
+constexpr int kBackwardStages = 2;                 // the row is read twice; three or four are no faster
 
 // kAligned: every row starts on 16 bytes and is whole 16-byte pieces.  Other rows are fetched with the bytes that share their first and
 // last 16 (their neighbours', inside the tensor), read at a shift that is the same for the whole row, and written back
@@ -753,10 +753,6 @@ cudaError_t backward_v(const NormArgs& a, int groups, int parts, cudaStream_t st
 constexpr int kRingColumns = 8192;
 int ring_threads_forward(int C) { return C <= 32 * 64 ? 32 : C <= 64 * 80 ? 64 : 128; }
 int ring_threads_backward(int C, int e) { return C * e <= 32 * 80 ? 32 : C * e <= 64 * 80 ? 64 : C * e <= 128 * 80 ? 128 : 256; }
-// Stages of the backward ring: three where two CTAs of them still fit an SM, else two.
-int backward_stages(int C, int e, int groups, bool aligned) {
-  return 2 * (RingLayout(C, e, 1, 2, groups, kBackwardStages, aligned).total + 1536) <= 232448 ? kBackwardStages : 2;
-}
 // CTAs of a kernel that the SMs hold at this much shared memory; the answer for the last size is kept.
 constexpr int kRingSmem = 230000;                  // above what any layout needs (205,000: forward, fp32, 5,120 unaligned columns)
 template <typename Kernel>
@@ -810,7 +806,7 @@ cudaError_t forward_ring_t(const NormArgs& a, cudaStream_t st) {
 template <typename T, bool kAligned, int NV, int TPR>
 cudaError_t backward_ring(NormArgs a, int groups, int parts, cudaStream_t st) {
   constexpr int G = kRingThreads / TPR;
-  a.stages = backward_stages(a.C, sizeof(T), G, kAligned);
+  a.stages = kBackwardStages;
   static uint64_t done;
   const cudaError_t e = allow_smem(&layer_norm_backward_ring_kernel<T, NV, TPR, kAligned>, kRingSmem, done);
   if (e != cudaSuccess) return e;
