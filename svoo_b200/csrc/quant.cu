@@ -81,9 +81,10 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
     const BlockDivide by(s, __shfl_sync(0xffffffffu, reciprocal, u, 16));
     const int k = kb[u] * kBlock + lane * 8;
     if (lane == u) scale[kb[u] * scale_pitch + row[u]] = s;
-    uint2 out;
-    out.x = by.e4m3x4<sizeof(T) == 2>(to_f32(raw[u].v[0]), to_f32(raw[u].v[1]), to_f32(raw[u].v[2]), to_f32(raw[u].v[3]));
-    out.y = by.e4m3x4<sizeof(T) == 2>(to_f32(raw[u].v[4]), to_f32(raw[u].v[5]), to_f32(raw[u].v[6]), to_f32(raw[u].v[7]));
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f32(raw[u].v[i]);
+    const uint2 out = by.e4m3x8<sizeof(T) == 2>(v);
     if (k < q_pitch) *reinterpret_cast<uint2*>(q + row[u] * q_pitch + k) = out;      // zeros behind the row
   }
 }
@@ -217,9 +218,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quantize_tile_ker
         const BlockDivide by(s, __shfl_sync(0xffffffffu, reciprocal, u, 16));
         if (m >= M) continue;
         if (lane == u) scale[kb * scale_pitch + m] = s;
-        uint2 out;
-        out.x = by.e4m3x4<sizeof(T) == 2>(to_f32(raw[u].v[0]), to_f32(raw[u].v[1]), to_f32(raw[u].v[2]), to_f32(raw[u].v[3]));
-        out.y = by.e4m3x4<sizeof(T) == 2>(to_f32(raw[u].v[4]), to_f32(raw[u].v[5]), to_f32(raw[u].v[6]), to_f32(raw[u].v[7]));
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f32(raw[u].v[i]);
+        const uint2 out = by.e4m3x8<sizeof(T) == 2>(v);
         if (k < q_pitch) *reinterpret_cast<uint2*>(q + (int64_t)m * q_pitch + k) = out;
       }
     }

@@ -50,10 +50,21 @@ struct BlockDivide {
   // below another, which no amax of 11 bits over 448 is.
   template <bool kOnce = false>
   __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) const {
-    if (up != 1.f) a *= up, b *= up, c *= up, d *= up;
+    if (__builtin_expect(up != 1.f, 0)) a *= up, b *= up, c *= up, d *= up;
     pair<kOnce>(a, b);
     pair<kOnce>(c, d);
     return e4m3x2(a, b) | e4m3x2(c, d) << 16;
+  }
+  // eight values, in one branch
+  template <bool kOnce>
+  __device__ __forceinline__ uint2 e4m3x8(float (&v)[8]) const {
+    if (__builtin_expect(up != 1.f, 0)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= up;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) pair<kOnce>(v[i], v[i + 1]);
+    return make_uint2(e4m3x2(v[0], v[1]) | e4m3x2(v[2], v[3]) << 16, e4m3x2(v[4], v[5]) | e4m3x2(v[6], v[7]) << 16);
   }
   template <bool kOnce>
   __device__ __forceinline__ void pair(float& a, float& b) const {
