@@ -452,6 +452,21 @@ int svoo_b200_linear_fp8(const void* x, int32_t x_type, int64_t M, int64_t K, in
                          const float* b_scale, int64_t b_scale_n, int64_t b_scale_k, const void* bias, int32_t bias_type, int64_t N,
                          int32_t activation, void* out, int32_t out_type, int64_t out_pitch, float* out_scale,
                          int64_t out_scale_pitch, void* workspace, int64_t workspace_bytes, void* stream);
+/* A linear layer that is being trained, x [M, K] and w [N, K] unquantised, M >= 1.  forward: y [M, N] (dense, x_type) =
+ * quantize_rows(x) quantize_blocks(w)^T + bias; `saved` receives what the gradients need: with keep_x_grad the transpose of w's
+ * bytes, with keep_w_grad the quantised columns of x.  backward: from dy [M, N] (x_type) and saved, each of dx [M, K] (dense, x_type) =
+ * quantize_rows(dy) w, dw [N, K] (dense, w_type) = quantize_columns(dy) quantize_columns(x)^T and db [N] (bias_type, column sums of dy)
+ * that is not null; dx wants keep_x_grad, dw keep_w_grad.  Results are those of the separate calls.
+ * bytes_out[3]: saved, scratch of forward, scratch of backward. */
+int svoo_b200_linear_train_bytes(int64_t M, int64_t N, int64_t K, int32_t keep_x_grad, int32_t keep_w_grad, int64_t* bytes_out);
+int svoo_b200_linear_train_forward(const void* x, int32_t x_type, int64_t M, int64_t K, int64_t x_row, const void* w, int32_t w_type,
+                                   int64_t N, int64_t w_row, const void* bias, int32_t bias_type, int32_t keep_x_grad,
+                                   int32_t keep_w_grad, void* y, void* saved, int64_t saved_bytes, void* scratch,
+                                   int64_t scratch_bytes, void* stream);
+int svoo_b200_linear_train_backward(const void* dy, int32_t x_type, int64_t M, int64_t N, int64_t K, int64_t dy_row, const void* saved,
+                                    int64_t saved_bytes, int32_t keep_x_grad, int32_t keep_w_grad, void* dx, void* dw,
+                                    int32_t w_type, void* db, int32_t bias_type, void* scratch, int64_t scratch_bytes,
+                                    void* stream);
 /* Copies the product's status word of the current device to *status (device int32): 0, or 1 after a kernel gave up on a
  * bounded wait and left rows unwritten. */
 int svoo_b200_linear_status(int32_t* status, void* stream);

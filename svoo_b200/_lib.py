@@ -102,6 +102,13 @@ SIGNATURES = {
     "svoo_b200_linear_fp8": (c_int, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64,
                                      c_void_p, c_int32, c_int64, c_int32, c_void_p, c_int32, c_int64, c_void_p, c_int64, c_void_p,
                                      c_int64, c_void_p]),
+    "svoo_b200_linear_train_bytes": (c_int, [c_int64, c_int64, c_int64, c_int32, c_int32, _I64P]),
+    "svoo_b200_linear_train_forward": (c_int, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int32, c_int64, c_int64,
+                                               c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
+                                               c_void_p]),
+    "svoo_b200_linear_train_backward": (c_int, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int32,
+                                                c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_int32, c_void_p, c_int64,
+                                                c_void_p]),
     "svoo_b200_linear_status": (c_int, [c_void_p, c_void_p]),
     "svoo_b200_push_seq": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int64, c_int64, c_int64, c_void_p]),
 }

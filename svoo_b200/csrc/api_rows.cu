@@ -72,6 +72,34 @@ const void* end_of(const void* p, int64_t batch, int64_t rows, int64_t C, int64_
   return static_cast<const char*>(p) + ((batch - 1) * batch_stride + (rows - 1) * row_stride + C) * e;
 }
 int64_t norm_groups(int64_t batch, int32_t per_sample) { return per_sample && batch > 1 ? batch : 1; }
+// Where a training step keeps things: offsets in `saved`, in forward's and in backward's scratch.
+struct TrainLayout {
+  int64_t mp, np, kp, mb, nb, kb, xs, ys;        // rows in bytes, blocks, pitches of the column scales
+  int64_t wt, w_scale, xt, xt_scale, saved;
+  int64_t w_q, x_q, x_scale, forward;
+  int64_t g_q, g_scale, gt, gt_scale, part, backward;
+  TrainLayout(int64_t M, int64_t N, int64_t K, bool keep_x, bool keep_w) {
+    mp = align_up(M, 16), np = align_up(N, 16), kp = align_up(K, 16);
+    mb = ceil_div64(M, 128), nb = ceil_div64(N, 128), kb = ceil_div64(K, 128), xs = align_up(K, 4), ys = align_up(N, 4);
+    int64_t at = 0;
+    auto take = [&at](int64_t bytes) { const int64_t here = at; at += align_up(bytes, 256); return here; };
+    wt = take(keep_x ? K * np : 0), w_scale = take(nb * kb * 4), xt = take(keep_w ? K * mp : 0), xt_scale = take(keep_w ? mb * xs * 4 : 0);
+    saved = at, at = 0;
+    w_q = take(N * kp), x_q = take(M * kp), x_scale = take(kb * M * 4);
+    forward = at, at = 0;
+    g_q = take(M * np), g_scale = take(nb * M * 4), gt = take(N * mp), gt_scale = take(mb * ys * 4), part = take(mb * N * 4);
+    backward = at;
+  }
+};
+int check_train(int64_t M, int64_t N, int64_t K) {
+  if (M < 1 || N < 1 || K < 1 || M > kMaxRows || N > kMaxRows || K > kMaxRows) return SVOO_ERR_SHAPE;
+  const int64_t mb = ceil_div64(M, 128), nb = ceil_div64(N, 128), kb = ceil_div64(K, 128);
+  if (mb > 65535 || nb > 65535 || M * kb > (int64_t)INT32_MAX - 1024 || M * nb > (int64_t)INT32_MAX - 1024 || mb * nb > INT32_MAX / 2 ||
+      mb * kb > INT32_MAX / 2 || nb * kb > INT32_MAX / 2)
+    return SVOO_ERR_SHAPE;
+  return SVOO_OK;
+}
+#define SVOO_CUDA(expr) do { cudaError_t _e = (expr); if (_e != cudaSuccess) return (int)_e; } while (0)
 #define SVOO_TRY(expr) do { int _rc = (expr); if (_rc != SVOO_OK) return _rc; } while (0)
 }  // namespace
 
@@ -222,6 +250,74 @@ int svoo_b200_linear_fp8(const void* x, int32_t x_type, int64_t M, int64_t K, in
   if (e != cudaSuccess) return (int)e;
   return (int)launch_linear(workspace, pitch, scale, M, b, b_pitch, b_scale, b_scale_n, b_scale_k, false, bias, bias_type, M, N, K, gelu,
                             out_type, out, out_pitch, out_scale, out_scale_pitch, (cudaStream_t)stream);
+}
+
+int svoo_b200_linear_train_bytes(int64_t M, int64_t N, int64_t K, int32_t keep_x_grad, int32_t keep_w_grad, int64_t* bytes_out) {
+  if (!bytes_out) return SVOO_ERR_NULL;
+  SVOO_TRY(check_train(M, N, K));
+  const TrainLayout l(M, N, K, keep_x_grad != 0, keep_w_grad != 0);
+  bytes_out[0] = l.saved, bytes_out[1] = l.forward, bytes_out[2] = l.backward;
+  return SVOO_OK;
+}
+
+int svoo_b200_linear_train_forward(const void* x, int32_t x_type, int64_t M, int64_t K, int64_t x_row, const void* w, int32_t w_type,
+                                   int64_t N, int64_t w_row, const void* bias, int32_t bias_type, int32_t keep_x_grad,
+                                   int32_t keep_w_grad, void* y, void* saved, int64_t saved_bytes, void* scratch,
+                                   int64_t scratch_bytes, void* stream) {
+  if (!element(x_type) || !element(w_type) || (bias && !element(bias_type))) return SVOO_ERR_TYPE;
+  SVOO_TRY(check_train(M, N, K));
+  if (x_row < 0 || w_row < 0) return SVOO_ERR_SHAPE;
+  if (!x || !w || !y || !saved || !scratch) return SVOO_ERR_NULL;
+  const TrainLayout l(M, N, K, keep_x_grad != 0, keep_w_grad != 0);
+  if (saved_bytes < l.saved || scratch_bytes < l.forward) return SVOO_ERR_WORKSPACE;
+  if (!aligned(x, elem_bytes(x_type)) || !aligned(w, elem_bytes(w_type)) || !aligned(y, elem_bytes(x_type)) || !aligned(saved, 16) ||
+      !aligned(scratch, 16) || (bias && !aligned(bias, elem_bytes(bias_type))))
+    return SVOO_ERR_ALIGN;
+  char *k = static_cast<char*>(saved), *t = static_cast<char*>(scratch);
+  float *w_scale = (float*)(k + l.w_scale), *x_scale = (float*)(t + l.x_scale);
+  const cudaStream_t st = (cudaStream_t)stream;
+  SVOO_CUDA(launch_quantize_blocks(w_type, w, N, K, w_row, t + l.w_q, l.kp, keep_x_grad ? k + l.wt : nullptr, l.np, w_scale, st));
+  if (keep_w_grad)
+    SVOO_CUDA(launch_quantize_both(x_type, x, M, K, x_row, t + l.x_q, l.kp, x_scale, M, k + l.xt, l.mp, (float*)(k + l.xt_scale), l.xs, nullptr, st));
+  else
+    SVOO_CUDA(launch_quantize_rows(x_type, x, M, K, x_row, t + l.x_q, l.kp, x_scale, M, st));
+  return (int)launch_linear(t + l.x_q, l.kp, x_scale, M, t + l.w_q, l.kp, w_scale, l.kb, 1, false, bias, bias_type, M, N, K, false, x_type, y, N,
+                            nullptr, 0, st);
+}
+
+int svoo_b200_linear_train_backward(const void* dy, int32_t x_type, int64_t M, int64_t N, int64_t K, int64_t dy_row, const void* saved,
+                                    int64_t saved_bytes, int32_t keep_x_grad, int32_t keep_w_grad, void* dx, void* dw,
+                                    int32_t w_type, void* db, int32_t bias_type, void* scratch, int64_t scratch_bytes,
+                                    void* stream) {
+  if (!element(x_type) || (dw && !element(w_type)) || (db && !element(bias_type))) return SVOO_ERR_TYPE;
+  SVOO_TRY(check_train(M, N, K));
+  if (dy_row < 0) return SVOO_ERR_SHAPE;
+  if (!dy || !saved || !scratch || (dx && !keep_x_grad) || (dw && !keep_w_grad)) return SVOO_ERR_NULL;
+  if (!dx && !dw && !db) return SVOO_OK;
+  const TrainLayout l(M, N, K, keep_x_grad != 0, keep_w_grad != 0);
+  if (saved_bytes < l.saved || scratch_bytes < l.backward) return SVOO_ERR_WORKSPACE;
+  if (!aligned(dy, elem_bytes(x_type)) || !aligned(saved, 16) || !aligned(scratch, 16) || !aligned(dx, elem_bytes(x_type)) ||
+      (dw && !aligned(dw, elem_bytes(w_type))) || (db && !aligned(db, elem_bytes(bias_type))))
+    return SVOO_ERR_ALIGN;
+  const char* k = static_cast<const char*>(saved);
+  char* t = static_cast<char*>(scratch);
+  const float* w_scale = (const float*)(k + l.w_scale);
+  float *g_scale = (float*)(t + l.g_scale), *gt_scale = (float*)(t + l.gt_scale), *part = db ? (float*)(t + l.part) : nullptr;
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (dx && (dw || db))
+    SVOO_CUDA(launch_quantize_both(x_type, dy, M, N, dy_row, t + l.g_q, l.np, g_scale, M, t + l.gt, l.mp, gt_scale, l.ys, part, st));
+  else if (dx)
+    SVOO_CUDA(launch_quantize_rows(x_type, dy, M, N, dy_row, t + l.g_q, l.np, g_scale, M, st));
+  else
+    SVOO_CUDA(launch_quantize_columns(x_type, dy, M, N, dy_row, t + l.gt, l.mp, gt_scale, l.ys, part, st));
+  if (db) SVOO_CUDA(launch_column_sum(part, l.mb, N, db, bias_type, st));
+  if (dx)
+    SVOO_CUDA(launch_linear(t + l.g_q, l.np, g_scale, M, k + l.wt, l.np, w_scale, 1, l.kb, false, nullptr, 0, M, K, N, false, x_type, dx, K, nullptr,
+                            0, st));
+  if (dw)
+    SVOO_CUDA(launch_linear(t + l.gt, l.mp, gt_scale, l.ys, k + l.xt, l.mp, (const float*)(k + l.xt_scale), 1, l.xs, true, nullptr, 0, N, K, M,
+                            false, w_type, dw, K, nullptr, 0, st));
+  return SVOO_OK;
 }
 
 int svoo_b200_linear_status(int32_t* status, void* stream) {

@@ -22,60 +22,62 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return x if x.shape[1] == 1 or x.stride(1) == 1 else x.contiguous()
 
 
-class _Linear(torch.autograd.Function):
+class _Trained(torch.autograd.Function):
+    """A weight that is quantised in the call: one call of the library forward, one backward."""
+
     @staticmethod
     def forward(ctx, x, weight, bias):
-        need_x, need_w, _ = ctx.needs_input_grad
-        trained = isinstance(weight, torch.Tensor)
-        if trained:
-            w = ops.quantize_blocks(weight, transposed=need_x)
-            ctx.weight_dtype = weight.dtype
-        else:
-            w = weight
-            if need_x:
-                w.transposed()                              # raises without one
-        ctx.bias_dtype = None if bias is None else bias.dtype
-        ctx.shape = w.shape
-        # what the gradients need: the weight's transpose, and x as its columns in e4m3
-        keep = [None] * 4
-        if need_w and x.shape[0]:
-            a, columns = ops.quantize_both(x)
-            keep[:2] = columns.q, columns.scale
-        else:
-            a = ops.quantize_rows(x)
-        if need_x:
-            keep[2:] = w.qt, w.scale
-        ctx.save_for_backward(*keep)
-        return ops.mm_fp8(a, w, bias, None, x.dtype)
+        ctx.kept = ctx.needs_input_grad[:2]
+        ctx.dtypes = weight.dtype, None if bias is None else bias.dtype
+        ctx.shape = weight.shape
+        y, saved = ops.linear_train_forward(x, weight, bias, *ctx.kept)
+        ctx.save_for_backward(saved)
+        return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         need_x, need_w, need_b = ctx.needs_input_grad
-        xt, xt_scale, wt, w_scale = ctx.saved_tensors
-        N, K = ctx.shape
+        saved, = ctx.saved_tensors
+        return ops.linear_train_backward(_rows(grad), saved, ctx.shape[1], *ctx.kept, need_x, ctx.dtypes[0] if need_w else None,
+                                         ctx.dtypes[1] if need_b else None)
+
+
+class _Stored(torch.autograd.Function):
+    """A weight that is a constant."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        if ctx.needs_input_grad[0]:
+            w = weight.transposed()                         # raises without one
+            ctx.save_for_backward(w.q, w.scale)
+        return ops.mm_fp8(ops.quantize_rows(x), weight, bias, None, x.dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
         grad = _rows(grad)
-        dx = dw = db = None
-        if grad.shape[0] == 0:
-            return (grad.new_zeros((0, K)) if need_x else None,
-                    grad.new_zeros((N, K), dtype=ctx.weight_dtype) if need_w else None,
-                    grad.new_zeros(N, dtype=ctx.bias_dtype) if need_b else None)
-        rows = columns = None
-        sums = ctx.bias_dtype if need_b else None
-        if need_x and (need_w or need_b):
-            rows, columns, *db = ops.quantize_both(grad, sums)
-            db = db[0] if db else None
-        elif need_x:
-            rows = ops.quantize_rows(grad)
-        elif need_b:
-            columns, db = ops.quantize_columns(grad, sums)
-        else:
-            columns = ops.quantize_columns(grad)
-        if need_x:
-            dx = ops.mm_fp8(rows, Fp8Weight(wt, w_scale.t()), None, None, grad.dtype)
-        if need_w:
-            dw = ops.mm_fp8(columns, ops.Fp8Rows(xt, xt_scale), None, None, ctx.weight_dtype)
-        return dx, dw, db
+        dx = db = None
+        if ctx.needs_input_grad[0]:
+            dx = ops.mm_fp8(ops.quantize_rows(grad), Fp8Weight(*ctx.saved_tensors), None, None, grad.dtype)
+        if ctx.needs_input_grad[2]:
+            db = ops.quantize_columns(grad, ctx.bias_dtype)[1] if grad.shape[0] else grad.new_zeros(grad.shape[1], dtype=ctx.bias_dtype)
+        return dx, None, db
+
+
+class _NoRows(torch.autograd.Function):
+    """A trained layer without rows: an empty result, gradients of zeros."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        ctx.like = [None if t is None else (t.shape, t.dtype) for t in (x, weight, bias)]
+        return x.new_empty((0, weight.shape[0]))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        return tuple(grad.new_zeros(like[0], dtype=like[1]) if need else None for like, need in zip(ctx.like, ctx.needs_input_grad))
 
 
 def linear_fp8(x: torch.Tensor, weight: Union[torch.Tensor, Fp8Weight], bias: Optional[torch.Tensor] = None,
@@ -91,7 +93,8 @@ def linear_fp8(x: torch.Tensor, weight: Union[torch.Tensor, Fp8Weight], bias: Op
     if training:
         if activation is not None:
             raise ValueError("linear_fp8 has no gradient through an activation: apply it to the result")
-        y = _Linear.apply(m, weight, bias)
+        trained = isinstance(weight, torch.Tensor)
+        y = (_Stored if not trained else _Trained if m.shape[0] else _NoRows).apply(m, weight, bias)
     else:
         w = ops.quantize_blocks(weight) if isinstance(weight, torch.Tensor) else weight
         y = ops.linear_fp8(m, w, bias, activation)

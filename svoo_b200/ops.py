@@ -915,6 +915,63 @@ def linear_fp8(x: torch.Tensor, w: Fp8Blocks, bias: Optional[torch.Tensor] = Non
     return out if out_scale is None else Fp8Rows(out, out_scale)
 
 
+@functools.lru_cache(maxsize=1024)
+def _train_bytes(M: int, N: int, K: int, keep_x: bool, keep_w: bool) -> Tuple[int, int, int]:
+    need = (ctypes.c_int64 * 3)()
+    check(LIB.svoo_b200_linear_train_bytes(M, N, K, keep_x, keep_w, need), "linear_train")
+    return tuple(need)
+
+
+def linear_train_forward(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, keep_x_grad: bool = True,
+                         keep_w_grad: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(x w^T + bias, saved) of a layer in training: x [M, K], M >= 1, and w [N, K], both quantised in the call (quantize_rows,
+    quantize_blocks), results as mm_fp8 gives them; `saved`, bytes, is what linear_train_backward needs for the gradient of x and of w."""
+    M, K, x_row = _matrix(x, "x")
+    N, KW, w_row = _matrix(w, "w")
+    if K != KW or M < 1 or N < 1:
+        raise ValueError(f"x {[M, K]} and w {[N, KW]} do not sum over the same length, or have no rows")
+    if bias is not None and (bias.dtype not in TYPES or bias.dim() != 1 or bias.shape[0] != N or (N > 1 and bias.stride(0) != 1)):
+        raise ValueError(f"bias must be a dense [{N}] of bf16, fp16 or fp32")
+    index = _device(x, w, bias)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return linear_train_forward(x, w, bias, keep_x_grad, keep_w_grad)
+    saved_bytes, scratch_bytes, _ = _train_bytes(M, N, K, keep_x_grad, keep_w_grad)
+    y = x.new_empty((M, N))
+    saved, scratch = x.new_empty(saved_bytes, dtype=torch.uint8), x.new_empty(scratch_bytes, dtype=torch.uint8)
+    check(LIB.svoo_b200_linear_train_forward(x.data_ptr(), TYPES[x.dtype], M, K, x_row, w.data_ptr(), TYPES[w.dtype], N, w_row, _ptr(bias),
+                                             0 if bias is None else TYPES[bias.dtype], keep_x_grad, keep_w_grad, y.data_ptr(),
+                                             saved.data_ptr(), saved_bytes, scratch.data_ptr(), scratch_bytes, _raw_stream(index)),
+          "linear_train_forward")
+    return y, saved
+
+
+def linear_train_backward(grad: torch.Tensor, saved: torch.Tensor, K: int, keep_x_grad: bool = True, keep_w_grad: bool = True,
+                          x_grad: bool = True, w_dtype: Optional[torch.dtype] = None, bias_dtype: Optional[torch.dtype] = None):
+    """(dx or None, dw or None, db or None) of linear_train_forward at grad [M, N] (the type of its result): dx with x_grad, dw and db
+    of w_dtype and bias_dtype where those are given.  K and the keep flags as in the forward call."""
+    M, N, row = _matrix(grad, "the gradient")
+    if (x_grad and not keep_x_grad) or (w_dtype is not None and not keep_w_grad):
+        raise ValueError("the forward call did not keep what this gradient needs")
+    if not all(t is None or t in TYPES for t in (w_dtype, bias_dtype)):
+        raise ValueError("gradients are bf16, fp16 or fp32")
+    saved_bytes, _, scratch_bytes = _train_bytes(M, N, K, keep_x_grad, keep_w_grad)
+    if saved.dtype is not torch.uint8 or saved.dim() != 1 or saved.shape[0] != saved_bytes:
+        raise ValueError("saved is not of a forward call with these sizes")
+    index = _device(grad, saved)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return linear_train_backward(grad, saved, K, keep_x_grad, keep_w_grad, x_grad, w_dtype, bias_dtype)
+    dx = grad.new_empty((M, K)) if x_grad else None
+    dw = None if w_dtype is None else grad.new_empty((N, K), dtype=w_dtype)
+    db = None if bias_dtype is None else grad.new_empty(N, dtype=bias_dtype)
+    scratch = grad.new_empty(scratch_bytes, dtype=torch.uint8)
+    check(LIB.svoo_b200_linear_train_backward(grad.data_ptr(), TYPES[grad.dtype], M, N, K, row, saved.data_ptr(), saved_bytes, keep_x_grad,
+                                              keep_w_grad, _ptr(dx), _ptr(dw), TYPES.get(w_dtype, 0), _ptr(db), TYPES.get(bias_dtype, 0),
+                                              scratch.data_ptr(), scratch_bytes, _raw_stream(index)), "linear_train_backward")
+    return dx, dw, db
+
+
 def linear_status(device: torch.device) -> int:
     """Status word of the 8-bit products on this device (synchronises): 0, or 1 after a kernel gave up on a bounded wait and
     left rows unwritten."""

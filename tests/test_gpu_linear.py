@@ -183,6 +183,41 @@ def test_linear_with_gradients(dtype, M, N, K, bias):
                 + torch.finfo(dtype).tiny).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (70, 130, 260), (300, 200, 129)])
+def test_training_calls_are_the_separate_calls(dtype, M, N, K):
+    """Bit for bit, for every subset of gradients, with rows of wider tensors."""
+    from svoo_b200 import linear, ops
+    x, w, g = rand(M, K + 5, dtype, 1)[:, 5:], rand(N, K + 3, dtype, 2, 0.05)[:, :K], rand(M, N + 1, dtype, 3)[:, 1:]
+    b = rand(1, N, torch.float32, 4)[0]
+    y, saved = ops.linear_train_forward(x, w, b)
+    q = ops.quantize_blocks(w, transposed=True)
+    assert torch.equal(y, ops.mm_fp8(ops.quantize_rows(x), q, b, None, dtype))
+    dx, dw, db = ops.linear_train_backward(g, saved, K, w_dtype=torch.float32, bias_dtype=torch.float32)
+    assert torch.equal(dx, ops.mm_fp8(ops.quantize_rows(g), q.transposed(), None, None, dtype))
+    gt, sums = ops.quantize_columns(g, torch.float32)
+    dw_t = ops.mm_fp8(gt, ops.quantize_columns(x), None, None, dtype)
+    assert torch.equal(dw, ops.mm_fp8(gt, ops.quantize_columns(x), None, None, torch.float32)) and torch.equal(db, sums)
+    for need in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 0), (1, 0, 1), (0, 1, 1)):
+        leaves = [t.detach().requires_grad_(bool(n)) for t, n in zip((x, w, b), need)]
+        got = torch.autograd.grad(linear.linear_fp8(*leaves), [t for t, n in zip(leaves, need) if n], g)
+        for t, ref in zip(got, [r for r, n in zip((dx, dw_t, db), need) if n]):
+            assert torch.equal(t, ref)
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    part, = torch.autograd.grad(linear.linear_fp8(*leaves), leaves[1:2], g)              # kept for all, asked for one
+    assert torch.equal(part, dw_t)
+    for bad in (dict(saved=saved[:-1]), dict(K=K + 1), dict(keep_w_grad=False, w_dtype=torch.float32), dict(w_dtype=torch.float64)):
+        kw = dict(dict(saved=saved, K=K), **bad)
+        if kw["K"] == K + 1 and kw["saved"].shape[0] == ops._train_bytes(M, N, K + 1, True, True)[0]:
+            continue
+        with pytest.raises(ValueError):
+            ops.linear_train_backward(g, **kw)
+    with pytest.raises(ValueError):
+        ops.linear_train_forward(x, w[:, 1:], b)
+    with pytest.raises(ValueError):
+        ops.linear_train_forward(x[:0], w, b)
+
+
 def test_gradients_are_those_of_a_linear_layer():
     """Against the unquantised layer: e4m3 rounds each operand by up to 2^-4, about 2.6 % of its norm, so a product of two
     is within 5 % of the true one in the 2-norm."""

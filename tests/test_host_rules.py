@@ -133,6 +133,20 @@ def test_token_wise_entry_points_check_their_arguments():
     lin = lambda **k: L.svoo_b200_linear_fp8(*{**few, **k}.values())                      # noqa: E731
     assert lin(M=0) == 0 and lin(x=None) == -1 and lin(b=None) == -1 and lin(out=None) == -1 and lin(bp=72) == -2 and lin(t=3) == -8
     assert lin(M=17) == -1 and lin(M=17, ws=p, wb=16) == -4 and lin(ot=3) == -1 and lin(K=0) == -2 and lin(b=p + 8) == -5
+    three = (ctypes.c_int64 * 3)()
+    assert L.svoo_b200_linear_train_bytes(100, 200, 300, 1, 1, three) == 0 and all(v > 0 for v in three)
+    whole = list(three)
+    assert L.svoo_b200_linear_train_bytes(100, 200, 300, 0, 0, three) == 0 and three[0] < whole[0] and list(three)[1:] == whole[1:]
+    assert L.svoo_b200_linear_train_bytes(0, 200, 300, 1, 1, three) == -2 and L.svoo_b200_linear_train_bytes(1, 1, 1, 1, 1, None) == -1
+    fw = dict(x=p, t=0, M=4, K=64, xr=64, w=p, wt=0, N=16, wr=64, bias=None, bt=0, kx=1, kw=1, y=p, sv=p, sb=1 << 20, ws=p, wb=1 << 20, st=None)
+    forward = lambda **k: L.svoo_b200_linear_train_forward(*{**fw, **k}.values())         # noqa: E731
+    assert forward(x=None) == -1 and forward(sv=None) == -1 and forward(t=3) == -8 and forward(wt=4) == -8 and forward(M=0) == -2
+    assert forward(sb=64) == -4 and forward(wb=64) == -4 and forward(sv=p + 8) == -5 and forward(bias=p, bt=3) == -8 and forward(xr=-1) == -2
+    bwd = dict(dy=p, t=0, M=4, N=16, K=64, r=16, sv=p, sb=1 << 20, kx=1, kw=1, dx=p, dw=p, wt=0, db=p, bt=0, ws=p, wb=1 << 20, st=None)
+    backward = lambda **k: L.svoo_b200_linear_train_backward(*{**bwd, **k}.values())      # noqa: E731
+    assert backward(dx=None, dw=None, db=None) == 0
+    assert backward(dy=None) == -1 and backward(kx=0) == -1 and backward(kw=0) == -1 and backward(wt=3) == -8 and backward(bt=3) == -8
+    assert backward(sb=64) == -4 and backward(wb=64) == -4 and backward(dy=p + 1) == -5 and backward(N=0) == -2
 
 
 def test_product_kernels_do_not_spill():
