@@ -38,14 +38,10 @@ __device__ __forceinline__ void umma_e4m3(uint32_t d, uint64_t a, uint64_t b, ui
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n"
         ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
-// Arrives at the barrier (at this place in every CTA of the pair) when the issued MMAs have completed.
-template <int CTAS>
-__device__ __forceinline__ void commit_all(uint32_t bar) {
-  if constexpr (CTAS == 2)
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                 ::"r"(bar), "h"((uint16_t)3) : "memory");
-  else
-    tc_commit(bar);
+// Arrives at the barrier, in both CTAs of the pair, when the issued MMAs have completed.
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
 // TMA load into this CTA's shared memory that signals a barrier of the pair's first CTA.
 __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t first_bar) {

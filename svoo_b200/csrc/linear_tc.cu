@@ -9,16 +9,16 @@
 // TMEM); a scale that changes from block to block cannot be applied there, so every block starts a fresh accumulator and
 // the epilogue threads add it to their running sums in registers, times sa sb.  Two accumulators alternate.
 //
-// A tile is 128 CTAS rows x TN columns, CTAS = 2: a pair of SMs (cta_group::2), each with its half of a's and of b's rows in
+// A tile is 256 rows x 256 columns and belongs to a pair of SMs (cta_group::2), each with its half of a's and of b's rows in
 // shared memory, so that a byte that was fetched feeds twice the products.
 //
-//   warp 0       TMA producer: 128 x 128 bytes of a, TN / CTAS x 128 of b per stage (128-byte swizzle)
-//   warp 1       MMA issuer (of the pair's first CTA): M 128 CTAS, N TN, K 32
+//   warp 0       TMA producer: 128 x 128 bytes of a, 128 x 128 of b per stage (128-byte swizzle)
+//   warp 1       MMA issuer (of the pair's first CTA): M 256, N 256, K 32
 //   warp 2       copies the scales of a block of k into a ring of their own (cp.async)
 //   warp 3       brings the bias of a tile's columns to 32 bits
-//   warps 4-11   thread r of each group of four warps owns row r (TMEM lane r) and TN / 2 columns, which lie in one scale block
-//                of b: the factor sa sb is one number per thread and block.  The sums (TN / 2 registers) are moved
-//                between warpgroups by setmaxnreg.  Rows leave by TMA (boxes of 32 rows x 128 bytes) while the next tile runs.
+//   warps 4-11   thread r of each group of four warps owns row r (TMEM lane r) and 128 columns, which are one scale block
+//                of b: the factor sa sb is one number per thread and block.  The registers for the 128 sums come from the
+//                other warps (setmaxnreg).  Rows leave by TMA (boxes of 32 rows x 128 bytes) while the next tile runs.
 //
 // Every mbarrier wait is bounded; on expiry the CTA sets the status word of the device and leaves.
 #include "linear_common.cuh"
@@ -27,13 +27,14 @@ namespace svoo {
 namespace tc {
 
 constexpr int kLinThreads = 384;
-constexpr int kLinM = 128;                                    // rows of a CTA
+constexpr int kLinM = 128, TM = 2 * kLinM, TN = 256;          // rows of a CTA; a pair's tile
+constexpr int HC = TN / 2;                                    // columns of a warpgroup of sums
 constexpr int kLinBox = 32 * 128;                             // rows leave in boxes of 32 rows x 128 bytes, two per warp in flight
 constexpr int kLinScales = 8;                                 // scale blocks in flight
 
-template <int CTAS, int TN, bool kRowScales>
+template <bool kRowScales>
 struct LinCfg {
-  static constexpr int kABytes = kLinM * 128, kBRows = TN / CTAS, kBBytes = kBRows * 128, kStageBytes = kABytes + kBBytes;
+  static constexpr int kABytes = kLinM * 128, kBRows = TN / 2, kBBytes = kBRows * 128, kStageBytes = kABytes + kBBytes;
   static constexpr int kScaleFloats = kLinM + (kRowScales ? TN : 4);       // sa of the rows, sb of the columns (or of two blocks)
   static constexpr int kFixed = 16 * kLinBox + kLinScales * kScaleFloats * 4 + 2 * TN * 4 + 512 + 1024;
   static constexpr int kStages = (232448 - kFixed) / kStageBytes < 8 ? (232448 - kFixed) / kStageBytes : 8;
@@ -86,15 +87,14 @@ __device__ __forceinline__ void store_ragged(const unsigned char* box, const Lin
 }
 
 // OUT: SVOO_TYPE_* of the output, SVOO_TYPE_E4M3 with scales
-template <int CTAS, int TN, int OUT, bool kGelu, bool kRowScales>
+template <int OUT, bool kGelu, bool kRowScales>
 __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                                                                    const __grid_constant__ CUtensorMap tm_out, const LinearArgs a) {
-  using C = LinCfg<CTAS, TN, kRowScales>;
-  constexpr int TM = kLinM * CTAS, HC = TN / 2;                  // rows of a tile, columns of a warpgroup
+  using C = LinCfg<kRowScales>;
   extern __shared__ unsigned char smem_raw[];
   const int tiles_m = (a.M + TM - 1) / TM, tiles_n = (a.N + TN - 1) / TN, tiles = tiles_m * tiles_n;
   const int KB = (a.K + 127) / 128;
-  const int rank = CTAS == 2 ? (int)(blockIdx.x & 1) : 0, worker = blockIdx.x / CTAS, workers = gridDim.x / CTAS;
+  const int rank = (int)(blockIdx.x & 1), worker = blockIdx.x / 2, workers = gridDim.x / 2;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* gen = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t bars = base + C::kBars;
@@ -109,23 +109,18 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
   }
   if (tid == 0) {
     for (int i = 0; i < C::BARS; ++i)
-      mbar_init(bar(i), i >= C::BIAS_EMPTY ? 8 : i >= C::BIAS_FULL ? 32 : i >= C::SC_EMPTY ? 8 : i >= C::SC_FULL ? 32 : i >= C::ACC_EMPTY ? 8 * CTAS : 1);
+      mbar_init(bar(i), i >= C::BIAS_EMPTY ? 8 : i >= C::BIAS_FULL ? 32 : i >= C::SC_EMPTY ? 8 : i >= C::SC_FULL ? 32 : i >= C::ACC_EMPTY ? 16 : 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    if constexpr (CTAS == 2) {
-      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(C::kTmemColumns) : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    } else {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(C::kTmemColumns) : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(C::kTmemColumns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   pdl_trigger();
   tc_fence_before();
   __syncthreads();
-  if (CTAS == 2) pair_sync();                              // the other CTA's barriers are set up before they are signalled
+  pair_sync();                                             // the other CTA's barriers are set up before they are signalled
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
@@ -143,16 +138,10 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
           const int s = it % C::kStages;
           if (!(ok = mbar_wait(bar(C::EMPTY + s), ((it / C::kStages) & 1) ^ 1, abort_flag))) break;
           const uint32_t dst = base + s * C::kStageBytes;
-          if constexpr (CTAS == 2) {
-            if (rank == 0) mbar_expect_tx(bar(C::FULL + s), 2 * C::kStageBytes);
-            const uint32_t full = at_cta(bar(C::FULL + s), 0);
-            tma_load_pair(dst, &tm_a, kb * 128, tile.tm * TM + rank * kLinM, full);
-            tma_load_pair(dst + C::kABytes, &tm_b, kb * 128, tile.tn * TN + rank * C::kBRows, full);
-          } else {
-            mbar_expect_tx(bar(C::FULL + s), C::kStageBytes);
-            tma_load_2d(dst, &tm_a, kb * 128, tile.tm * TM, bar(C::FULL + s));
-            tma_load_2d(dst + C::kABytes, &tm_b, kb * 128, tile.tn * TN, bar(C::FULL + s));
-          }
+          if (rank == 0) mbar_expect_tx(bar(C::FULL + s), 2 * C::kStageBytes);
+          const uint32_t full = at_cta(bar(C::FULL + s), 0);
+          tma_load_pair(dst, &tm_a, kb * 128, tile.tm * TM + rank * kLinM, full);
+          tma_load_pair(dst + C::kABytes, &tm_b, kb * 128, tile.tn * TN + rank * C::kBRows, full);
         }
       }
       // copies in flight land before the CTA ends (the pair leaves together)
@@ -172,10 +161,10 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
           const uint32_t as = base + s * C::kStageBytes, bs = as + C::kABytes;
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)
-            umma_e4m3<CTAS>(tmem + b * TN, smem_desc_sw128(as + ks * 32, 16, 1024), smem_desc_sw128(bs + ks * 32, 16, 1024),
+            umma_e4m3<2>(tmem + b * TN, smem_desc_sw128(as + ks * 32, 16, 1024), smem_desc_sw128(bs + ks * 32, 16, 1024),
                             idesc_e4m3(TM, TN), ks > 0);
-          commit_all<CTAS>(bar(C::EMPTY + s));
-          commit_all<CTAS>(bar(C::ACC_FULL + b));
+          commit_pair(bar(C::EMPTY + s));
+          commit_pair(bar(C::ACC_FULL + b));
         }
       }
     } else if (warp == 2) {
@@ -237,7 +226,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
     unsigned char* box = gen + C::kOut + (warp - 4) * 2 * kLinBox;
     const bool has_bias = !kRowScales && a.bias;
     int n_tile = 0;
-    const uint32_t acc_empty = CTAS == 2 ? at_cta(bar(C::ACC_EMPTY), 0) : bar(C::ACC_EMPTY);
+    const uint32_t acc_empty = at_cta(bar(C::ACC_EMPTY), 0);
     int it = 0;
     bool ok = true;
     for (int t = worker; t < tiles && ok; t += workers, ++n_tile) {
@@ -265,10 +254,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
           } else {                                         // all columns are here: the next block may be summed over them
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) {
-              if (CTAS == 2) arrive_cluster(acc_empty + 8 * b);
-              else mbar_arrive(acc_empty + 8 * b);
-            }
+            if (lane == 0) arrive_cluster(acc_empty + 8 * b);
           }
           const uint32_t(&v)[16] = r[ch & 1];
           if (kRowScales) {
@@ -382,35 +368,31 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
   }
   tc_fence_before();
   __syncthreads();
-  if (CTAS == 2) pair_sync();
+  pair_sync();
   if (tid == 0 && *abort_flag) atomicExch(a.status, 1);
   if (warp == 1) {
     tc_fence_after();
-    if constexpr (CTAS == 2)
-      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemColumns) : "memory");
-    else
-      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemColumns) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemColumns) : "memory");
   }
 }
 
 }  // namespace tc
 
-template <int CTAS, int TN, int OUT, bool kGelu, bool kRowScales>
-static cudaError_t launch_tiles(const LinearCall& c) {
-  using C = tc::LinCfg<CTAS, TN, kRowScales>;
+template <int OUT, bool kGelu, bool kRowScales>
+static cudaError_t launch_one(const LinearCall& c) {
+  using C = tc::LinCfg<kRowScales>;
   alignas(64) CUtensorMap ma, mb, mo = {};
   if (!tc::make_byte_tensor_map(&ma, c.a, c.args.M, c.args.K, c.a_pitch, tc::kLinM) ||
       !tc::make_byte_tensor_map(&mb, c.b, c.args.N, c.args.K, c.b_pitch, C::kBRows) ||
       (c.args.box_out && !tc::make_out_tensor_map(&mo, OUT, c.args.out, c.args.M, c.args.N, c.args.out_pitch)))
     return cudaErrorInvalidValue;
-  auto* kernel = &tc::linear_tc_kernel<CTAS, TN, OUT, kGelu, kRowScales>;
+  auto* kernel = &tc::linear_tc_kernel<OUT, kGelu, kRowScales>;
   static uint64_t done;
   const cudaError_t e = allow_smem(kernel, C::kSmemBytes, done);
   if (e != cudaSuccess) return e;
-  constexpr int sms = 148;
-  const int64_t tiles = ceil_div64(c.args.M, tc::kLinM * CTAS) * ceil_div64(c.args.N, TN);
+  const int64_t tiles = ceil_div64(c.args.M, tc::TM) * ceil_div64(c.args.N, tc::TN);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles < sms / CTAS ? tiles : sms / CTAS) * CTAS);
+  cfg.gridDim = dim3(2 * (unsigned)(tiles < 74 ? tiles : 74));      // a pair per two SMs
   cfg.blockDim = dim3(tc::kLinThreads);
   cfg.dynamicSmemBytes = C::kSmemBytes;
   cfg.stream = c.st;
@@ -418,17 +400,12 @@ static cudaError_t launch_tiles(const LinearCall& c) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = CTAS;
+  attr[1].val.clusterDim.x = 2;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = CTAS == 2 ? 2 : 1;
+  cfg.numAttrs = 2;
   count_launches(1);
   return cudaLaunchKernelEx(&cfg, kernel, ma, mb, mo, c.args);
-}
-
-template <int OUT, bool kGelu, bool kRowScales>
-static cudaError_t launch_one(const LinearCall& c) {
-  return launch_tiles<2, 256, OUT, kGelu, kRowScales>(c);
 }
 
 cudaError_t launch_linear_few(int type, const void* x, int64_t x_row, const LinearCall& c, int out_type, bool gelu);

@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(kWideBackwardThreads) layer_norm_backward_kern
 
 // ---- rows fetched ahead into shared memory -----------------------------------------------------------------------------
 //
-// A group of TPR threads walks rows; cp.async.bulk brings the next kStages rows of every group while one is worked on, so that what is
+// A group of TPR threads walks rows; cp.async.bulk brings the next rows of every group while one is worked on, so that what is
 // in flight does not depend on registers or on where the group is in its arithmetic.  Gain and offset lie in shared memory in 32
 // bits for the whole walk.  TPR is small: what a row costs besides its elements (two or three sums over the threads, a
 // square root, addresses: some 200 instructions a thread) is paid by every thread of it.  (A thread per eight elements, four rows at
@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(kRingThreads) layer_norm_ring_kernel(const Nor
 
 // x and dy rows come in together.  A thread's columns are the same in every row: their sums stay in its registers.
 template <typename T, int NV, int TPR, bool kAligned>
-__global__ void __launch_bounds__(kRingThreads < TPR ? TPR : kRingThreads) layer_norm_backward_ring_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(kRingThreads) layer_norm_backward_ring_kernel(const NormArgs a) {
   constexpr int P = 8 / (int)sizeof(T), V = 2 * P, G = kRingThreads / TPR;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ float slots[2][G][TPR / 32][2];

@@ -83,3 +83,64 @@ def test_modules_follow_devices_types_and_state_dicts():
         linear.Fp8FeedForward.from_sequential(nn.Sequential(nn.Linear(8, 8), nn.ReLU(), nn.Linear(8, 8)))
     with pytest.raises(ValueError):
         m.set_weight(ops.quantize_blocks(torch.randn(8, 200, device=DEV)))
+
+
+def test_first_calls_in_a_capture_and_two_graphs_at_once():
+    """Calls that were never made before capture; two graphs of the same operators replayed on two streams do not share anything."""
+    from svoo_b200 import ops
+    x, w, dy = (torch.randn(*s, device=DEV).half() for s in ((1000, 640), (512, 640), (1000, 512)))
+    one, two = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(one):
+        b = ops.quantize_blocks(w, transposed=True)
+        y = ops.linear_fp8(x, b, None, "gelu")
+        few = ops.linear_fp8(x[:5], b)
+        n, mean, rstd = ops.layer_norm(x, return_stats=True)
+        dx = ops.layer_norm_backward(n, x, mean, rstd)[0]
+        dw = ops.mm_fp8(ops.quantize_columns(dy), ops.quantize_columns(x))
+    with torch.cuda.graph(two):
+        y2 = ops.linear_fp8(x, b, None, "gelu")
+        n2 = ops.layer_norm(x)
+    one.replay()
+    torch.cuda.synchronize()
+    want = [t.clone() for t in (y, few, n, dx, dw)]
+    eager = (ops.linear_fp8(x, ops.quantize_blocks(w), None, "gelu"), ops.linear_fp8(x[:5], b), ops.layer_norm(x),
+             ops.layer_norm_backward(n, x, mean, rstd)[0], ops.mm_fp8(ops.quantize_columns(dy), ops.quantize_columns(x)))
+    assert all(torch.equal(u, v) for u, v in zip(want, eager))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(50):
+        for graph, stream in zip((one, two), streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(u, v) for u, v in zip((y, few, n, dx, dw, y2, n2), want + [want[0], want[2]]))
+
+
+def test_captured_training_step():
+    from svoo_b200 import linear, norm
+    x, w, b = (torch.randn(*s, device=DEV).bfloat16().requires_grad_(True) for s in ((300, 256), (384, 256), (384,)))
+    dy = torch.randn(300, 384, device=DEV).bfloat16()
+
+    def step():
+        return torch.autograd.grad(linear.linear_fp8(norm.layer_norm(x), w, b), (x, w, b), dy)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(u, v) for u, v in zip(got, step()))
+
+
+def test_many_samples_of_one_row():
+    from svoo_b200 import ops
+    x, s, t = (torch.randn(3000, 1, 64, device=DEV) for _ in range(3))
+    y, mean, rstd = ops.layer_norm(x, scale=s, shift=t, return_stats=True)
+    want, xhat, _, _ = R.layer_norm(x, 1 + s.double(), t, 1e-6)
+    assert (y.double() - want).abs().max() < 1e-4            # 80 x 2^-24 x 20 at most before the gain, by far
+    _, dg, do = ops.layer_norm_backward(y, x, mean, rstd, scale=s)
+    assert (dg.double() - y.double() * xhat).abs().max() < 1e-3 and torch.equal(do, y)
