@@ -7,7 +7,7 @@
 // 32 t .. 32 t + 31 of its row, and step j multiplies bytes 4 j .. 4 j + 3 of the four lanes.  e4m3 goes to fp16 exactly, a
 // product of two is a 32-bit number, sums are in 32 bits; each block is scaled by sa sb as linear_tc.cu does.
 // Every warp quantises the rows of its own blocks: again in every CTA, but that is cheaper than a launch.  It is also what bounds the
-// kernel at 16 rows of 5,120 columns (19.5 us, 14.1 with 8 rows or one; eight warps 18.9 and 12.1, but 15.9 against 9.2 on 8,960).
+// kernel at 16 rows of 5,120 columns (12.7 us; 8.7 with one row, 9.3 with 8).
 #include "linear_common.cuh"
 
 namespace svoo {
@@ -64,13 +64,13 @@ __device__ __forceinline__ float quantize_lane(const T* p, int k, int K, bool li
   return s;
 }
 
-// MT: 8 or 16 rows; NT: column tiles of 8
-constexpr int kFewWarps = 16;
-template <typename T, bool kWide, int MT, int NT>
-__global__ void __launch_bounds__(kFewWarps * 32) linear_few_kernel(const T* __restrict__ x, int64_t x_row, const uint8_t* __restrict__ b, int64_t b_pitch,
-                                                         const tc::LinearArgs a, int out_type, bool gelu) {
+// MT: 8 or 16 rows; NT: column tiles of 8; W: warps
+template <typename T, bool kWide, int MT, int NT, int W>
+__global__ void __launch_bounds__(W * 32, W == 8 ? 2 : 1)
+    linear_few_kernel(const T* __restrict__ x, int64_t x_row, const uint8_t* __restrict__ b, int64_t b_pitch, const tc::LinearArgs a,
+                      int out_type, bool gelu) {
   constexpr int NW = NT * 8;
-  __shared__ float part[kFewWarps][MT][NW + 1];
+  __shared__ float part[W][MT][NW + 1];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   const int n0 = blockIdx.x * NW, KB = (a.K + 127) / 128;
   pdl_trigger();
@@ -80,8 +80,8 @@ __global__ void __launch_bounds__(kFewWarps * 32) linear_few_kernel(const T* __r
   for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) sum[i][j] = 0.f;
-  const float* sb = a.sb + (int64_t)(n0 / 128) * a.sb_n;
-  for (int kb = warp; kb < KB; kb += kFewWarps) {
+  const int last = (a.N - 1) / 128;
+  for (int kb = warp; kb < KB; kb += W) {
     const int k = kb * 128 + t * 32;
     // the weights first: they are what takes long
     uint4 w[NT][2];
@@ -91,12 +91,16 @@ __global__ void __launch_bounds__(kFewWarps * 32) linear_few_kernel(const T* __r
 #pragma unroll
       for (int h = 0; h < 2; ++h) w[i][h] = load_weights(b + (int64_t)n * b_pitch + k + h * 16, n < a.N ? a.K - k - h * 16 : 0);
     }
-    const float fb = sb[kb * a.sb_k];
+    float fb[NT];                                           // a CTA's columns may lie in two blocks
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const int nb = (n0 + i * 8) / 128;
+      fb[i] = a.sb[(nb < last ? nb : last) * a.sb_n + kb * a.sb_k];
+    }
     uint32_t q0[8], q1[8];
     float s[2] = {0.f, 0.f};
     s[0] = quantize_lane<T, kWide>(x + g * x_row + k, k, a.K, g < a.M, q0);
     if (MT == 16) s[1] = quantize_lane<T, kWide>(x + (g + 8) * x_row + k, k, a.K, g + 8 < a.M, q1);
-    const float f[2] = {s[0] * fb, s[1] * fb};
     float acc[NT][4];
 #pragma unroll
     for (int i = 0; i < NT; ++i)
@@ -115,7 +119,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) linear_few_kernel(const T* __r
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum[i][j] = fmaf(acc[i][j], f[j / 2], sum[i][j]);
+      for (int j = 0; j < 4; ++j) sum[i][j] = fmaf(acc[i][j], s[j / 2] * fb[i], sum[i][j]);
   }
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
@@ -123,12 +127,12 @@ __global__ void __launch_bounds__(kFewWarps * 32) linear_few_kernel(const T* __r
     for (int j = 0; j < (MT == 16 ? 4 : 2); ++j) part[warp][g + j / 2 * 8][i * 8 + t * 2 + j % 2] = sum[i][j];
   }
   __syncthreads();
-  for (int o = threadIdx.x; o < MT * NW; o += kFewWarps * 32) {
+  for (int o = threadIdx.x; o < MT * NW; o += W * 32) {
     const int r = o / NW, n = n0 + o % NW;
     if (r >= a.M || n >= a.N) continue;
     float v = 0.f;
 #pragma unroll
-    for (int i = 0; i < kFewWarps; ++i) v += part[i][r][o % NW];
+    for (int i = 0; i < W; ++i) v += part[i][r][o % NW];
     float bias[1];
     tc::bias_columns(a, n, 1, bias);
     v += bias[0];
@@ -140,18 +144,24 @@ __global__ void __launch_bounds__(kFewWarps * 32) linear_few_kernel(const T* __r
   }
 }
 
-template <typename T, bool kWide, int MT, int NT>
+template <typename T, bool kWide, int MT, int NT, int W>
 static cudaError_t launch_few_nt(const void* x, int64_t x_row, const LinearCall& c, int out_type, bool gelu) {
   count_launches(1);
-  return launch_pdl(linear_few_kernel<T, kWide, MT, NT>, dim3((unsigned)ceil_div(c.args.N, NT * 8)), dim3(kFewWarps * 32), 0, c.st, (const T*)x, x_row,
+  return launch_pdl(linear_few_kernel<T, kWide, MT, NT, W>, dim3((unsigned)ceil_div(c.args.N, NT * 8)), dim3(W * 32), 0, c.st, (const T*)x, x_row,
                     (const uint8_t*)c.b, c.b_pitch, c.args, out_type, gelu);
+}
+// Columns per CTA so that all of them run at once: an SM holds one CTA of sixteen warps or two of eight.  One row, 16 rows of 5,120 x
+// 5,120, us: 40 columns by sixteen warps (128 CTAs) 8.7, 12.7; 32 by sixteen (160, two rounds) 14.1, 19.5; 32 by eight 12.1, 18.9.  With 16
+// rows and 40 columns a few of the 128 registers spill (112 bytes a thread).
+template <typename T, bool kWide, int MT>
+static cudaError_t launch_few_mt(const void* x, int64_t x_row, const LinearCall& c, int out_type, bool gelu) {
+  if (c.args.N <= 148 * 16) return launch_few_nt<T, kWide, MT, 2, 16>(x, x_row, c, out_type, gelu);
+  if (c.args.N <= 148 * 40) return launch_few_nt<T, kWide, MT, 5, 16>(x, x_row, c, out_type, gelu);
+  return launch_few_nt<T, kWide, MT, 4, 8>(x, x_row, c, out_type, gelu);
 }
 template <typename T, bool kWide>
 static cudaError_t launch_few_t(const void* x, int64_t x_row, const LinearCall& c, int out_type, bool gelu) {
-  const bool wide_tiles = c.args.N >= 148 * 32;             // 32 columns per CTA where that still is one CTA per SM
-  if (c.args.M <= 8)
-    return wide_tiles ? launch_few_nt<T, kWide, 8, 4>(x, x_row, c, out_type, gelu) : launch_few_nt<T, kWide, 8, 2>(x, x_row, c, out_type, gelu);
-  return wide_tiles ? launch_few_nt<T, kWide, 16, 4>(x, x_row, c, out_type, gelu) : launch_few_nt<T, kWide, 16, 2>(x, x_row, c, out_type, gelu);
+  return c.args.M <= 8 ? launch_few_mt<T, kWide, 8>(x, x_row, c, out_type, gelu) : launch_few_mt<T, kWide, 16>(x, x_row, c, out_type, gelu);
 }
 
 // M <= 16, output not e4m3; c.a unused

@@ -448,8 +448,8 @@ cudaError_t launch_linear(const void* a, int64_t a_pitch, const float* sa, int64
 }
 
 // The product on few rows that are not quantised yet, in one launch.  us on the GPU, this / quantisation and split product:
-// 1 x 5,120 x 5,120 14.1 / 12.6, 1 x 1,536 x 1,536 2.6 / 6.9, 1 x 8,960 x 1,536 5.8 / 9.2, 1 x 1,536 x 8,960 9.2 / 10.0; 16 rows 19.5 / 12.6,
-// 4.1 / 6.9, 8.2 / 9.2, 14.1 / 10.0.  The second launch and its workspace cost the host another 4 us (13.6 and 17.7 a call).
+// 1 x 5,120 x 5,120 8.7 / 12.5, 1 x 1,536 x 1,536 2.6 / 6.8, 1 x 8,960 x 1,536 4.8 / 9.2, 1 x 1,536 x 8,960 9.1 / 9.9; 16 rows 12.7 / 12.5,
+// 4.0 / 6.8, 7.2 / 9.2, 13.5 / 9.9.  The second launch and its workspace cost the host another 4 us (13.6 and 17.7 a call).
 bool linear_few_rows(int64_t M, int64_t K, int out_type) { return (M <= 8 || (M <= 16 && K <= 4096)) && out_type != SVOO_TYPE_E4M3; }
 cudaError_t launch_linear_few_rows(int x_type, const void* x, int64_t x_row, const void* b, int64_t b_pitch, const float* sb, int64_t sb_n,
                                    int64_t sb_k, const void* bias, int bias_type, int64_t M, int64_t N, int64_t K, bool gelu, int out_type,

@@ -110,7 +110,7 @@ def test_product_with_blocks(dtype, M, N, K):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 5, 16), (2, 130, 300), (3, 777, 1001), (7, 4800, 130), (8, 33, 2048), (9, 40, 257), (15, 5000, 640), (16, 5120, 1300), (9, 64, 4100),
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 5, 16), (2, 130, 300), (3, 777, 1001), (7, 4800, 130), (8, 33, 2048), (9, 40, 257), (15, 5000, 640), (16, 5120, 1300), (9, 64, 4100), (5, 6000, 200), (12, 2400, 600),
                                    (16, 129, 1000), (17, 129, 1000)])
 def test_linear_of_few_rows(dtype, M, N, K):
     """One launch up to 16 rows: quantised, multiplied, bias and GELU; weights with bytes behind their rows, rows of a wider tensor."""
