@@ -175,16 +175,20 @@ class WanDiT(nn.Module):
 
     def use_token_kernels(self, norms: bool = True, fp8_linears: bool = True) -> "WanDiT":
         """Puts the token-wise half of every block on this package's kernels: layer norms with their modulation in one pass,
-        and (inference only) the projections and the feed-forward in e4m3, their weights quantised here.  The model has to be on
-        its GPU.  Embedders, the output projection and the per-step embeddings stay as they are."""
+        and (inference only) the projections and the feed-forward in e4m3, their weights quantised here, for good: a layer that
+        is in e4m3 already stays so.  The model has to be on its GPU.  Embedders, the output projection and the per-step
+        embeddings stay as they are."""
+        if not all(p.is_cuda for p in self.blocks.parameters()):
+            raise ValueError("use_token_kernels needs a model on its GPU")
         for block in self.blocks:
             block.fused_norms = norms
-            if fp8_linears:
-                for attn in (block.attn1, block.attn2):
-                    for name in ("to_q", "to_k", "to_v"):
-                        setattr(attn, name, fp8.Fp8Linear.from_linear(getattr(attn, name)))
-                    attn.to_out[0] = fp8.Fp8Linear.from_linear(attn.to_out[0])
-                block.ffn = fp8.Fp8FeedForward.from_sequential(block.ffn)
+            if not fp8_linears or isinstance(block.ffn, fp8.Fp8FeedForward):
+                continue
+            for attn in (block.attn1, block.attn2):
+                for name in ("to_q", "to_k", "to_v"):
+                    setattr(attn, name, fp8.Fp8Linear.from_linear(getattr(attn, name)))
+                attn.to_out[0] = fp8.Fp8Linear.from_linear(attn.to_out[0])
+            block.ffn = fp8.Fp8FeedForward.from_sequential(block.ffn)
         return self
 
     def _timestep_embedding(self, timestep):

@@ -144,3 +144,69 @@ def test_many_samples_of_one_row():
     assert (y.double() - want).abs().max() < 1e-4            # 80 x 2^-24 x 20 at most before the gain, by far
     _, dg, do = ops.layer_norm_backward(y, x, mean, rstd, scale=s)
     assert (dg.double() - y.double() * xhat).abs().max() < 1e-3 and torch.equal(do, y)
+
+
+@torch.no_grad()
+def test_token_kernels_twice():
+    """A second call keeps the layers that are in e4m3; norms follow the last call."""
+    cfg, model = dense_dit("Twice")
+    lat = torch.randn(1, 16, *cfg.latent, device=DEV).bfloat16()
+    text = torch.randn(1, 16, 64, device=DEV).bfloat16()
+    t = torch.tensor([900.0], device=DEV)
+    want = model.use_token_kernels()(lat, t, text)
+    layer = model.blocks[0].attn1.to_q
+    assert torch.equal(model.use_token_kernels()(lat, t, text), want)
+    assert model.blocks[0].attn1.to_q is layer
+    model.use_token_kernels(norms=False)
+    assert not model.blocks[0].fused_norms and model.blocks[0].attn1.to_q is layer
+
+
+def check_product(y, a, b):
+    want = a @ b.t()
+    assert ((y.double() - want).abs() <= R.product_bound(a, b, torch.float32, want)).all()
+
+
+@torch.no_grad()
+def test_offsets_beyond_32_bits():
+    """Every kernel on tensors of more than 2^31 elements.  The last rows of norms and quantisers are those of a call on the last
+    rows alone, bit for bit; products are checked against 64 bits."""
+    from svoo_b200 import ops
+    M, C, tail = 140_000, 16_384, 256                       # 140,000 is a multiple of 32, not of 128
+    assert M * C > 2 ** 31
+    x = torch.empty(M, C, device=DEV, dtype=torch.bfloat16).normal_()
+    end = x[M - tail:].clone()
+    # layer norm of the widest rows, and of the same numbers as rows of 5,120 with a pitch of 16,384
+    for src in (x, x[:, 7:5127]):
+        gain = torch.randn(src.shape[1], device=DEV)
+        part = src[M - tail:]
+        y, mean, rstd = ops.layer_norm(src, gain, gain, return_stats=True)
+        y1, mean1, rstd1 = ops.layer_norm(part, gain, gain, return_stats=True)
+        assert torch.equal(y[M - tail:], y1) and torch.equal(mean[M - tail:], mean1) and torch.equal(rstd[M - tail:], rstd1)
+        dx = ops.layer_norm_backward(y, src, mean, rstd, gain)[0]
+        assert torch.equal(dx[M - tail:], ops.layer_norm_backward(y1, part, mean1, rstd1, gain)[0])
+        del y, dx
+    rows, columns = ops.quantize_both(x)
+    alone = ops.quantize_rows(end)
+    for r in (rows, ops.quantize_rows(x)):
+        assert torch.equal(r.q[M - tail:].view(torch.uint8), alone.q.view(torch.uint8)) and torch.equal(r.scale[:, M - tail:], alone.scale)
+    first = M // 128 * 128                                  # the last block along the columns
+    last = ops.quantize_columns(x[first:].clone())
+    for c in (columns, ops.quantize_columns(x)):
+        assert torch.equal(c.q[:, first:].view(torch.uint8), last.q.view(torch.uint8)) and torch.equal(c.scale[-1], last.scale[0])
+    del columns, c, r
+    # products: a of more than 2^31 bytes, b of as many, and a result of as many numbers
+    end_d = R.dequantize(end, 1, 128)
+    w, w_d = ops.quantize_blocks(x[:200].clone()), R.dequantize(x[:200], 128, 128)
+    check_product(ops.mm_fp8(rows, w, out_dtype=torch.float32)[M - tail:], end_d, w_d)
+    del rows
+    big = ops.quantize_blocks(x, transposed=True)
+    end_w, w_d = ops.quantize_blocks(x[first:].clone(), transposed=True), R.dequantize(x[first:], 128, 128)
+    assert torch.equal(big.q[first:].view(torch.uint8), end_w.q.view(torch.uint8))
+    assert torch.equal(big.qt[:, first:].view(torch.uint8), end_w.qt.view(torch.uint8))
+    check_product(ops.linear_fp8(end[:3], big, out_dtype=torch.float32)[:, first:], end_d[:3], w_d)
+    check_product(ops.mm_fp8(alone, big, out_dtype=torch.float32)[:, first:], end_d, w_d)
+    del x, big
+    a, b = (torch.randn(n, 130, device=DEV).bfloat16() for n in (70_001, 40_008))
+    out = ops.mm_fp8(ops.quantize_rows(a), ops.quantize_blocks(b), out_dtype=torch.float32)
+    assert out.numel() > 2 ** 31
+    check_product(out[-177:], R.dequantize(a[-177:], 1, 128), R.dequantize(b, 128, 128))

@@ -164,3 +164,13 @@ def test_product_kernels_do_not_spill():
         assert len(spills) >= kernels and all(s == ("0", "0") for s in spills), res.stderr
         if src == "linear_tc.cu":
             assert set(re.findall(r"Used (\d+) registers", res.stderr)) == {"168"}
+
+
+def test_token_kernels_need_a_model_on_its_gpu():
+    """Refused before anything of the model is changed."""
+    from svoo_b200 import wan_dit
+    cfg = wan_dit.WanDiTConfig(num_layers=1, dim=128, heads=1, ffn_dim=128, text_dim=16, text_len=4, latent=(1, 4, 4))
+    model = wan_dit.WanDiT(cfg)
+    with pytest.raises(ValueError, match="GPU"):
+        model.use_token_kernels()
+    assert not model.blocks[0].fused_norms and isinstance(model.blocks[0].attn1.to_q, torch.nn.Linear)
