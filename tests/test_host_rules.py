@@ -168,6 +168,8 @@ def test_product_kernels_do_not_spill():
 
 def test_token_kernels_need_a_model_on_its_gpu():
     """Refused before anything of the model is changed."""
+    import pytest
+    import torch
     from svoo_b200 import wan_dit
     cfg = wan_dit.WanDiTConfig(num_layers=1, dim=128, heads=1, ffn_dim=128, text_dim=16, text_len=4, latent=(1, 4, 4))
     model = wan_dit.WanDiT(cfg)
