@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kWideThreads) layer_norm_kernel(const NormArgs
 // [group][CTA][dg, do][C], which column_sum_kernel adds in a fixed order.  The next row is fetched before this one's two
 // sums are joined.
 template <typename T, int V, int NV>
-__global__ void __launch_bounds__(kWideBackwardThreads) layer_norm_backward_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(kWideBackwardThreads, 1) layer_norm_backward_kernel(const NormArgs a) {
   constexpr int TPR = kWideBackwardThreads;
   __shared__ float slots[2][2][TPR / 32];
   pdl_trigger();
@@ -231,16 +231,17 @@ constexpr int kForwardStages = 1;                  // the row is in registers at
 constexpr int kBackwardStages = 2;                 // the row is read twice; three or four are no faster
 
 // kAligned: every row starts on 16 bytes and is whole 16-byte pieces.  Other rows are fetched with the bytes that share their first and
-// last 16 (their neighbours', inside the tensor), read at a shift that is the same for the whole row, and written back
-// the same way: staged in shared memory and stored as aligned pieces, single elements at both ends.
+// last 16 (their neighbours', inside the tensor), and the threads of a group take neighbouring elements, one access each.  (16-byte
+// pieces read at the row's shift, written back through shared memory: us against this, forward and backward, 32 bits 2 x 4,097 x 1,001
+// 17.8 / 13.0 and 32.7 / 26.3, 4,097 x 5,121 64.9 / 40.3 and 104.8 / 54.5; bf16 16.0 / 12.8 and 25.8 / 26.3, 8,194 x 5,121 71.5 / 79.4 and
+// 98.4 / 90.9, 32,760 x 1,537 68.8 / 76.1 and 151.8 / 140.1.)
 struct RingLayout {
-  int columns, row, ring, out, bars, total;       // columns rounded up to whole pieces, bytes of a row's place; offsets
+  int columns, row, ring, bars, total;            // columns rounded up to whole pieces, bytes of a row's place; offsets
   __host__ __device__ RingLayout(int C, int e, int param_rows, int row_tensors, int groups, int stages, bool aligned) {
     columns = (C + 7) & ~7;
     row = aligned ? C * e : ((C * e + 15) & ~15) + 16;
     ring = param_rows * columns * 4;
-    out = ring + groups * stages * row_tensors * row;
-    bars = out + (aligned ? 0 : groups * row);
+    bars = ring + groups * stages * row_tensors * row;
     total = bars + groups * stages * 8 + 16;
   }
 };
@@ -329,22 +330,6 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
-// 16 bytes at `shift` (0 .. 15) bytes behind piece c of a row
-__device__ __forceinline__ uint4 shifted_piece(const unsigned char* row, int c, int shift) {
-  const uint4 u = reinterpret_cast<const uint4*>(row)[c], v = reinterpret_cast<const uint4*>(row)[c + 1];
-  uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-  if (shift & 8) {
-#pragma unroll
-    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
-  }
-  if (shift & 4) {
-#pragma unroll
-    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
-  }
-  const int bits = 8 * (shift & 3);
-  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
-                    __funnelshift_r(w[3], w[4], bits));
-}
 // What a bulk copy brings of a row, to `at` bytes behind its place in shared memory.
 struct RowCopy {
   const void* src;
@@ -371,34 +356,51 @@ __device__ __forceinline__ RowCopy plan_row(unsigned char* place, const T* src, 
 __device__ __forceinline__ void start_copy(unsigned char* place, const RowCopy& c, uint32_t bar) {
   if (c.bytes) bulk_load(smem_u32(place) + c.at, c.src, c.bytes, bar);
 }
-// piece c of a row that lies at `shift` in its place
-template <bool kAligned>
-__device__ __forceinline__ uint4 row_piece(const unsigned char* place, int c, int shift) {
-  return kAligned ? reinterpret_cast<const uint4*>(place)[c] : shifted_piece(place, c, shift);
-}
 template <typename T>
 __device__ __forceinline__ int shift_of(const T* row) { return (int)((uintptr_t)row & 15); }
-// Zeroes the elements from `valid` on.
-template <int P>
-__device__ __forceinline__ void cut(uint64_t (&d)[P], int valid) {
+// Piece i of thread t of TPR: V elements.  kAligned: 16 bytes, piece i TPR + t of the row; else element k is column (V i + k) TPR + t.
+template <typename T, int TPR>
+__device__ __forceinline__ int column_of(int i, int k, int t) { return (16 / (int)sizeof(T) * i + k) * TPR + t; }
+// The pairs of a piece of a row that lies at `shift` in its place; zeros behind the last column.
+template <typename T, bool kAligned, int TPR>
+__device__ __forceinline__ void read_piece(const unsigned char* place, int shift, int i, int t, int C, uint64_t (&p)[8 / sizeof(T)]) {
+  if constexpr (kAligned) {
+    unpack<T>(reinterpret_cast<const uint4*>(place)[i * TPR + t], p);
+  } else {
+    const T* row = reinterpret_cast<const T*>(place + shift);
 #pragma unroll
-  for (int k = 0; k < P; ++k) {
-    if (2 * k >= valid) d[k] = 0;
-    else if (2 * k + 1 >= valid) d[k] &= 0xffffffffull;
+    for (int k = 0; k < 8 / (int)sizeof(T); ++k) {
+      const int c = column_of<T, TPR>(i, 2 * k, t);
+      p[k] = f2(c < C ? to_f32(row[c]) : 0.f, c + TPR < C ? to_f32(row[c + TPR]) : 0.f);
+    }
   }
 }
-// A row staged in shared memory (first byte at `staged`) to global memory at any address: aligned 16-byte pieces by all threads of the
-// group, single elements at the ends.
-template <typename T, int TPR>
-__device__ __forceinline__ void store_row(T* dst, const unsigned char* staged, int C, int t) {
-  const int shift = (int)((uintptr_t)dst & 15), bytes = C * (int)sizeof(T);
-  const int head = shift ? 16 - shift : 0;                  // bytes in front of the first aligned piece
-  const int pieces = bytes > head ? (bytes - head) / 16 : 0;
-  unsigned char* out = reinterpret_cast<unsigned char*>(dst);
-  for (int k = t; k < pieces; k += TPR) *reinterpret_cast<uint4*>(out + head + k * 16) = shifted_piece(staged, k, head);
-  const int edge = (head < bytes ? head : bytes) / (int)sizeof(T), tail = bytes > head ? (bytes - head - pieces * 16) / (int)sizeof(T) : 0;
-  if (t < edge) dst[t] = reinterpret_cast<const T*>(staged)[t];
-  if (t < tail) dst[C - tail + t] = reinterpret_cast<const T*>(staged)[C - tail + t];
+// Pairs 2 j and 2 j + 1 of the parameters of a piece
+template <typename T, bool kAligned, int TPR>
+__device__ __forceinline__ ulonglong2 read_param(const float* param, int i, int j, int t, int C) {
+  if constexpr (kAligned) {
+    return reinterpret_cast<const ulonglong2*>(param + (i * TPR + t) * (16 / (int)sizeof(T)))[j];
+  } else {
+    float v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int c = column_of<T, TPR>(i, 4 * j + k, t);
+      v[k] = c < C ? param[c] : 0.f;
+    }
+    return make_ulonglong2(f2(v[0], v[1]), f2(v[2], v[3]));
+  }
+}
+template <typename T, bool kAligned, int TPR>
+__device__ __forceinline__ void write_piece(T* row, int i, int t, int C, const uint64_t (&p)[8 / sizeof(T)]) {
+  if constexpr (kAligned) {
+    reinterpret_cast<uint4*>(row)[i * TPR + t] = pack<T>(p);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 16 / (int)sizeof(T); ++k) {
+      const int c = column_of<T, TPR>(i, k, t);
+      if (c < C) row[c] = from_f32<T>(k & 1 ? hi2(p[k / 2]) : lo2(p[k / 2]));
+    }
+  }
 }
 
 // Row r of the walk of sample `sample` (per_sample) or of all samples: pointer offset in a tensor of these strides
@@ -440,7 +442,6 @@ __global__ void __launch_bounds__(kRingThreads) layer_norm_ring_kernel(const Nor
   float* off = gain + lay.columns;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + lay.bars + G * stages * 8);
   const int group = threadIdx.x / TPR, t = threadIdx.x % TPR, nvec = (a.C + V - 1) / V;
-  const int last = kAligned ? -1 : nvec - 1, valid = a.C - (nvec - 1) * V;    // the piece that may be cut
   const bool per_sample = gridDim.y > 1;
   const int n = (int)(per_sample ? a.rows : a.batch * a.rows), step = gridDim.x * G, first = blockIdx.x * G + group;
   unsigned char* ring = smem + lay.ring + group * stages * lay.row;
@@ -473,11 +474,9 @@ __global__ void __launch_bounds__(kRingThreads) layer_norm_ring_kernel(const Nor
     uint64_t d[NV][P], sum = 0;
     const int shift = kAligned ? 0 : shift_of(row_of(r));
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = i * TPR + t;
-      if (c < nvec) {
-        unpack<T>(row_piece<kAligned>(ring + s * lay.row, c, shift), d[i]);
-        if (!kAligned && c == last) cut(d[i], valid);
+    for (int i = 0; i < NV; ++i) {                         // skipping empty pieces costs more here (4,097 x 7,777 in 32 bits: 52.7 -> 67.7 us)
+      if (!kAligned || i * TPR + t < nvec) {
+        read_piece<T, kAligned, TPR>(ring + s * lay.row, shift, i, t, a.C, d[i]);
 #pragma unroll
         for (int k = 0; k < P; ++k) sum = add2(sum, d[i][k]);
       }
@@ -496,10 +495,16 @@ __global__ void __launch_bounds__(kRingThreads) layer_norm_ring_kernel(const Nor
     sum = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (i * TPR + t < nvec) {
+      if (!kAligned || i * TPR + t < nvec) {
 #pragma unroll
         for (int k = 0; k < P; ++k) d[i][k] = add2(d[i][k], minus);
-        if (!kAligned && i * TPR + t == last) cut(d[i], valid);
+        if constexpr (!kAligned) {
+#pragma unroll
+          for (int k = 0; k < P; ++k) {
+            const int c = column_of<T, TPR>(i, 2 * k, t);
+            d[i][k] = f2(c < a.C ? lo2(d[i][k]) : 0.f, c + TPR < a.C ? hi2(d[i][k]) : 0.f);
+          }
+        }
 #pragma unroll
         for (int k = 0; k < P; ++k) sum = fma2(d[i][k], d[i][k], sum);
       }
@@ -514,27 +519,17 @@ __global__ void __launch_bounds__(kRingThreads) layer_norm_ring_kernel(const Nor
     }
     const uint64_t rs = f2(rstd, rstd);
     T* y = static_cast<T*>(a.y) + row * a.C;
-    unsigned char* staged = smem + lay.out + group * lay.row;
-    uint4* to = kAligned ? reinterpret_cast<uint4*>(y) : reinterpret_cast<uint4*>(staged);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = i * TPR + t;
-      if (c < nvec) {
-        const ulonglong2* g = reinterpret_cast<const ulonglong2*>(gain + c * V);
-        const ulonglong2* o = reinterpret_cast<const ulonglong2*>(off + c * V);
+      if (!kAligned || i * TPR + t < nvec) {
 #pragma unroll
         for (int k = 0; k < P; k += 2) {
-          const ulonglong2 gv = g[k / 2], ov = o[k / 2];
+          const ulonglong2 gv = read_param<T, kAligned, TPR>(gain, i, k / 2, t, a.C), ov = read_param<T, kAligned, TPR>(off, i, k / 2, t, a.C);
           d[i][k] = fma2(mul2(d[i][k], rs), gv.x, ov.x);
           d[i][k + 1] = fma2(mul2(d[i][k + 1], rs), gv.y, ov.y);
         }
-        if (ok || !kAligned) to[c] = pack<T>(d[i]);
+        if (ok) write_piece<T, kAligned, TPR>(y, i, t, a.C, d[i]);
       }
-    }
-    if (!kAligned) {
-      group_sync<TPR>(group);
-      if (ok) store_row<T, TPR>(y, staged, a.C, t);
-      if (TPR == 32) __syncwarp();                         // other groups meet two barriers before the next row is staged
     }
     if (++s == stages) s = 0, phase ^= 1;
   }
@@ -552,7 +547,6 @@ __global__ void __launch_bounds__(kRingThreads) layer_norm_backward_ring_kernel(
   float* gain = reinterpret_cast<float*>(smem);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + lay.bars + G * stages * 8);
   const int group = threadIdx.x / TPR, t = threadIdx.x % TPR, nvec = (a.C + V - 1) / V;
-  const int last = kAligned ? -1 : nvec - 1, valid = a.C - (nvec - 1) * V;
   const bool per_sample = gridDim.y > 1;
   const int n = (int)(per_sample ? a.rows : a.batch * a.rows), step = gridDim.x * G, first = blockIdx.x * G + group;
   unsigned char* ring = smem + lay.ring + group * stages * 2 * lay.row;
@@ -598,16 +592,13 @@ __global__ void __launch_bounds__(kRingThreads) layer_norm_backward_ring_kernel(
     uint64_t s1 = 0, s2 = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = i * TPR + t;
-      if (c < nvec) {
+      if (kAligned ? i * TPR + t < nvec : i * V * TPR < a.C) {
         uint64_t x[P], d[P];
-        unpack<T>(row_piece<kAligned>(xs, c, x_shift), x);
-        unpack<T>(row_piece<kAligned>(ds, c, d_shift), d);
-        if (!kAligned && c == last) cut(x, valid), cut(d, valid);
-        const ulonglong2* g = reinterpret_cast<const ulonglong2*>(gain + c * V);
+        read_piece<T, kAligned, TPR>(xs, x_shift, i, t, a.C, x);
+        read_piece<T, kAligned, TPR>(ds, d_shift, i, t, a.C, d);
 #pragma unroll
         for (int k = 0; k < P; ++k) {
-          const ulonglong2 gv = g[k / 2];
+          const ulonglong2 gv = read_param<T, kAligned, TPR>(gain, i, k / 2, t, a.C);
           const uint64_t h = fma2(x[k], rs, shift), w = mul2(d[k], k & 1 ? gv.y : gv.x);
           dg[i][k] = fma2(d[k], h, dg[i][k]);
           dof[i][k] = add2(dof[i][k], d[k]);
@@ -622,29 +613,22 @@ __global__ void __launch_bounds__(kRingThreads) layer_norm_backward_ring_kernel(
     const float m1 = sums[0] * inv_c, m2 = sums[1] * inv_c;
     const uint64_t a2 = f2(-m2, -m2), a1 = f2(-m1, -m1);
     T* dx = static_cast<T*>(a.dx) + (sample_row + r) * a.C;
-    unsigned char* staged = smem + lay.out + group * lay.row;
-    uint4* to = kAligned ? reinterpret_cast<uint4*>(dx) : reinterpret_cast<uint4*>(staged);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = i * TPR + t;
-      if (c < nvec) {
+      if (kAligned ? i * TPR + t < nvec : i * V * TPR < a.C) {
         uint64_t x[P], d[P];
-        unpack<T>(row_piece<kAligned>(xs, c, x_shift), x);
-        unpack<T>(row_piece<kAligned>(ds, c, d_shift), d);
-        if (!kAligned && c == last) cut(x, valid), cut(d, valid);
-        const ulonglong2* g = reinterpret_cast<const ulonglong2*>(gain + c * V);
+        read_piece<T, kAligned, TPR>(xs, x_shift, i, t, a.C, x);
+        read_piece<T, kAligned, TPR>(ds, d_shift, i, t, a.C, d);
 #pragma unroll
         for (int k = 0; k < P; ++k) {
-          const ulonglong2 gv = g[k / 2];
+          const ulonglong2 gv = read_param<T, kAligned, TPR>(gain, i, k / 2, t, a.C);
           const uint64_t h = fma2(x[k], rs, shift);
           d[k] = mul2(fma2(h, a2, fma2(d[k], k & 1 ? gv.y : gv.x, a1)), rs);
         }
-        if (ok || !kAligned) to[c] = pack<T>(d);
+        if (ok) write_piece<T, kAligned, TPR>(dx, i, t, a.C, d);
       }
     }
     group_sync<TPR>(group);                                // the row has been read: its place takes another
-    if (!kAligned && ok) store_row<T, TPR>(dx, staged, a.C, t);
-    if (!kAligned && TPR == 32) __syncwarp();
     if (t == 0 && ahead < n && ok) {
       fetch(ahead, s);
       ahead += step;
@@ -662,7 +646,17 @@ __global__ void __launch_bounds__(kRingThreads) layer_norm_backward_ring_kernel(
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           const int c = i * TPR + t;
-          if (c < nvec) {
+          if constexpr (!kAligned) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              const int col = column_of<T, TPR>(i, j, t);
+              const float u = j & 1 ? hi2(dg[i][j / 2]) : lo2(dg[i][j / 2]), w = j & 1 ? hi2(dof[i][j / 2]) : lo2(dof[i][j / 2]);
+              if (col < a.C) {
+                acc[col] = k > 0 ? acc[col] + u : u;
+                acc[lay.columns + col] = k > 0 ? acc[lay.columns + col] + w : w;
+              }
+            }
+          } else if (c < nvec) {
             ulonglong2* p = reinterpret_cast<ulonglong2*>(acc + c * V);
             ulonglong2* q = reinterpret_cast<ulonglong2*>(acc + lay.columns + c * V);
 #pragma unroll
@@ -749,12 +743,12 @@ cudaError_t backward_v(const NormArgs& a, int groups, int parts, cudaStream_t st
 
 // Threads per row of the ring kernels: at most 80 elements a thread forward (75,600 x 5,120: 128 threads 306 us, 64 threads
 // 284); backward 80 bytes a thread and tensor (40 elements with two sums each; 32-bit rows take twice the place in the ring, and
-// twice the threads keep two CTAs on an SM: 2 x 4,097 x 1,001 54 us with one).
+// twice the threads keep two CTAs on an SM: 2 x 4,097 x 1,000 22.5 us, with half the threads 35.1; rows that are not aligned count as 32-bit ones, bf16 2 x 4,097 x 1,001 26.3, half 58.7).
 constexpr int kRingColumns = 8192;
 int ring_threads_forward(int C) { return C <= 32 * 64 ? 32 : C <= 64 * 80 ? 64 : 128; }
 int ring_threads_backward(int C, int e) { return C * e <= 32 * 80 ? 32 : C * e <= 64 * 80 ? 64 : C * e <= 128 * 80 ? 128 : 256; }
 // CTAs of a kernel that the SMs hold at this much shared memory; the answer for the last size is kept.
-constexpr int kRingSmem = 230000;                  // above what any layout needs (205,000: forward, fp32, 5,120 unaligned columns)
+constexpr int kRingSmem = 230000;                  // above what any layout needs (164,000: backward, fp32, 8,192 columns)
 template <typename Kernel>
 cudaError_t resident(Kernel* kernel, int smem, int64_t& kept, int& ctas) {
   const int64_t known = __atomic_load_n(&kept, __ATOMIC_RELAXED);
@@ -815,7 +809,7 @@ cudaError_t backward_ring(NormArgs a, int groups, int parts, cudaStream_t st) {
 template <typename T, bool kAligned>
 cudaError_t backward_ring_t(const NormArgs& a, int groups, int parts, cudaStream_t st) {
   constexpr int V = 16 / (int)sizeof(T), Q = 8 / V;
-  const int tpr = ring_threads_backward(a.C, sizeof(T));
+  const int tpr = ring_threads_backward(a.C, kAligned ? sizeof(T) : 4);
   const bool few = ceil_div(ceil_div(a.C, V), tpr) <= 3 * Q;
   switch (tpr) {
     case 32: return few ? backward_ring<T, kAligned, 3 * Q, 32>(a, groups, parts, st) : backward_ring<T, kAligned, 5 * Q, 32>(a, groups, parts, st);
