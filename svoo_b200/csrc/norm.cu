@@ -11,216 +11,6 @@
 
 namespace svoo {
 
-template <typename T, int V>
-__device__ __forceinline__ void load_param(const void* p, bool fp32, int64_t at, float (&out)[V]) {
-  if (fp32 || sizeof(T) == 4) {
-    const float* q = static_cast<const float*>(p) + at;
-    constexpr int W = V < 4 ? V : 4;
-#pragma unroll
-    for (int i = 0; i < V; i += W) {
-      const Vec<float, W> t = load_vec<float, W>(q + i);
-#pragma unroll
-      for (int k = 0; k < W; ++k) out[i + k] = t.v[k];
-    }
-  } else {
-    const Vec<T, V> t = load_vec<T, V>(static_cast<const T*>(p) + at);
-#pragma unroll
-    for (int k = 0; k < V; ++k) out[k] = to_f32(t.v[k]);
-  }
-}
-
-// Sum over the TPR threads of a row, the same in every thread.  `slot`: TPR / 32 floats of the row's own; two calls in a
-// row need two slots (a thread may still read the first when another writes the second).
-template <int TPR>
-__device__ __forceinline__ float row_sum(float s, float* slot, int t) {
-  s = warp_sum(s);
-  if (t % 32 == 0) slot[t / 32] = s;
-  __syncthreads();
-  s = 0.f;
-#pragma unroll
-  for (int w = 0; w < TPR / 32; ++w) s += slot[w];
-  return s;
-}
-
-// ---- rows of more than 8,192 columns: a CTA per row, straight from global memory ------------------------------------------
-//
-// Vector i of thread t, of NV with V elements each, lies at (i * threads + t) * V.
-constexpr int kWideThreads = 256, kWideColumns = 64;               // 16,384 columns
-constexpr int kWideBackwardThreads = 1024, kWideBackwardColumns = 16;
-template <typename T, int V, int NV>
-__global__ void __launch_bounds__(kWideThreads) layer_norm_kernel(const NormArgs a) {
-  constexpr int TPR = kWideThreads;
-  __shared__ float slots[2][TPR / 32];
-  pdl_trigger();
-  pdl_wait();
-  const int t = threadIdx.x;
-  const int64_t row = blockIdx.x;
-  const int64_t b = a.batch == 1 ? 0 : row / a.rows;
-  const T* x = static_cast<const T*>(a.x) + b * a.x_batch + (row - b * a.rows) * a.x_row;
-  const int nvec = a.C / V;
-
-  float v[NV][V];
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = i * TPR + t;
-    if (c < nvec) {
-      const Vec<T, V> r = load_stream<T, V>(x + (int64_t)c * V);
-#pragma unroll
-      for (int k = 0; k < V; ++k) v[i][k] = to_f32(r.v[k]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < V; ++k) v[i][k] = 0.f;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int k = 0; k < V; ++k) s += v[i][k];
-  const float mean = row_sum<TPR>(s, slots[0], t) / a.C;
-  float q = 0.f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (i * TPR + t < nvec) {
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float d = v[i][k] - mean;
-        q += d * d;
-      }
-    }
-  }
-  const float rstd = 1.f / sqrtf(row_sum<TPR>(q, slots[1], t) / a.C + a.eps);
-  if (t == 0 && a.mean) {
-    a.mean[row] = mean;
-    a.rstd[row] = rstd;
-  }
-  T* y = static_cast<T*>(a.y) + row * a.C;
-  const float one = a.plus_one ? 1.f : 0.f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = i * TPR + t;
-    if (c >= nvec) continue;
-    float gain[V], off[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) gain[k] = 1.f, off[k] = 0.f;
-    if (a.gain) {
-      load_param<T, V>(a.gain, a.params_fp32, b * a.gain_batch + c * V, gain);
-#pragma unroll
-      for (int k = 0; k < V; ++k) gain[k] += one;
-    }
-    if (a.offset) load_param<T, V>(a.offset, a.params_fp32, b * a.offset_batch + c * V, off);
-    Vec<T, V> r;
-#pragma unroll
-    for (int k = 0; k < V; ++k) r.v[k] = from_f32<T>((v[i][k] - mean) * rstd * gain[k] + off[k]);
-    *reinterpret_cast<Vec<T, V>*>(y + (int64_t)c * V) = r;
-  }
-}
-
-// A CTA walks the rows blockIdx.x, + gridDim.x, ... of group blockIdx.y (a sample where the modulation is
-// per sample, otherwise all rows) and keeps the column sums of its rows in registers; they go to `partial`
-// [group][CTA][dg, do][C], which column_sum_kernel adds in a fixed order.  The next row is fetched before this one's two
-// sums are joined.
-template <typename T, int V, int NV>
-__global__ void __launch_bounds__(kWideBackwardThreads, 1) layer_norm_backward_kernel(const NormArgs a) {
-  constexpr int TPR = kWideBackwardThreads;
-  __shared__ float slots[2][2][TPR / 32];
-  pdl_trigger();
-  pdl_wait();
-  const int t = threadIdx.x;
-  const bool per_sample = gridDim.y > 1;
-  const int64_t n = per_sample ? a.rows : a.batch * a.rows;
-  const int nvec = a.C / V;
-  float dg[NV][V], dof[NV][V], gain[NV][V];
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int k = 0; k < V; ++k) dg[i][k] = dof[i][k] = 0.f, gain[i][k] = 1.f;
-  if (a.gain) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = i * TPR + t;
-      if (c < nvec) load_param<T, V>(a.gain, a.params_fp32, blockIdx.y * a.gain_batch + c * V, gain[i]);
-      if (a.plus_one) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) gain[i][k] += 1.f;
-      }
-    }
-  }
-  Vec<T, V> xr[NV], dr[NV];
-  float mean = 0.f, rstd = 0.f;
-  auto fetch = [&](int64_t r) {
-    int64_t b = blockIdx.y, s = r;
-    if (!per_sample) b = a.batch == 1 ? 0 : r / a.rows, s = r - b * a.rows;
-    const T* x = static_cast<const T*>(a.x) + b * a.x_batch + s * a.x_row;
-    const T* dy = static_cast<const T*>(a.dy) + b * a.dy_batch + s * a.dy_row;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = i * TPR + t;
-      if (c < nvec) {
-        xr[i] = load_stream<T, V>(x + (int64_t)c * V);
-        dr[i] = load_stream<T, V>(dy + (int64_t)c * V);
-      }
-    }
-    mean = a.mean_in[b * a.rows + s];
-    rstd = a.rstd_in[b * a.rows + s];
-  };
-  if (blockIdx.x < n) fetch(blockIdx.x);
-  int buf = 0;
-  for (int64_t r = blockIdx.x; r < n; r += gridDim.x, buf ^= 1) {
-    float h[NV][V], w[NV][V], s1 = 0.f, s2 = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (i * TPR + t < nvec) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const float d = to_f32(dr[i].v[k]);
-          h[i][k] = (to_f32(xr[i].v[k]) - mean) * rstd;
-          dg[i][k] += d * h[i][k];
-          dof[i][k] += d;
-          w[i][k] = d * gain[i][k];
-          s1 += w[i][k];
-          s2 += w[i][k] * h[i][k];
-        }
-      }
-    }
-    const float rs = rstd;
-    if (r + gridDim.x < n) fetch(r + gridDim.x);
-    s1 = warp_sum(s1);
-    s2 = warp_sum(s2);
-    if (t % 32 == 0) slots[buf][0][t / 32] = s1, slots[buf][1][t / 32] = s2;
-    __syncthreads();                                     // the other buffer is written only after the next row's barrier
-    s1 = s2 = 0.f;
-#pragma unroll
-    for (int k = 0; k < TPR / 32; ++k) s1 += slots[buf][0][k], s2 += slots[buf][1][k];
-    s1 /= a.C;
-    s2 /= a.C;
-    T* dx = static_cast<T*>(a.dx) + (per_sample ? blockIdx.y * a.rows + r : r) * a.C;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = i * TPR + t;
-      if (c >= nvec) continue;
-      Vec<T, V> o;
-#pragma unroll
-      for (int k = 0; k < V; ++k) o.v[k] = from_f32<T>(rs * (w[i][k] - s1 - h[i][k] * s2));
-      *reinterpret_cast<Vec<T, V>*>(dx + (int64_t)c * V) = o;
-    }
-  }
-  if (!a.partial) return;
-  float* p = a.partial + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 * a.C;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = i * TPR + t;
-    if (c >= nvec) continue;
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      p[(int64_t)c * V + k] = dg[i][k];
-      p[a.C + (int64_t)c * V + k] = dof[i][k];
-    }
-  }
-}
-
-// ---- rows fetched ahead into shared memory -----------------------------------------------------------------------------
-//
 // A group of TPR threads walks rows; cp.async.bulk brings the next rows of every group while one is worked on, so that what is
 // in flight does not depend on registers or on where the group is in its arithmetic.  Gain and offset lie in shared memory in 32
 // bits for the whole walk.  TPR is small: what a row costs besides its elements (two or three sums over the threads, a
@@ -640,7 +430,7 @@ __global__ void __launch_bounds__(kRingThreads) layer_norm_backward_ring_kernel(
   if (a.partial) {
     // the groups of the CTA are added in shared memory, in order
     __syncthreads();
-    float* acc = reinterpret_cast<float*>(smem + lay.ring);                            // [dg, do][columns]: fits the ring
+    float* acc = reinterpret_cast<float*>(smem);           // [dg, do][columns]: fits the gain's place and the ring behind it
     for (int k = 0; k < G; ++k) {
       if (k == group) {
 #pragma unroll
@@ -712,43 +502,15 @@ __global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restric
 }
 
 namespace {
-bool multiple(int64_t v, int64_t of) { return v % of == 0; }
-
-// Elements per access: 16 bytes where every row of every tensor starts on such a boundary, else 4 bytes, else one element.
-int norm_vector(const NormArgs& a, int e) {
-  for (int bytes : {16, 4}) {
-    const int v = bytes / e;
-    bool ok = v >= 1;
-    for (int64_t stride : {(int64_t)a.C, a.x_batch, a.x_row, a.dy_batch, a.dy_row}) ok = ok && multiple(stride, v);
-    for (const void* p : {a.x, a.dy, (const void*)a.y, (const void*)a.dx}) ok = ok && multiple((intptr_t)p, bytes);
-    const int pb = a.params_fp32 ? (v < 4 ? v : 4) * 4 : bytes;          // bytes of one parameter access
-    for (const void* p : {a.gain, a.offset}) ok = ok && multiple((intptr_t)p, pb);
-    for (int64_t stride : {a.gain_batch, a.offset_batch}) ok = ok && multiple(stride * (a.params_fp32 ? 4 : e), pb);
-    if (ok) return v;
-  }
-  return 1;
-}
-
-template <typename T, int V>
-cudaError_t forward_v(const NormArgs& a, cudaStream_t st) {
-  count_launches(1);
-  return launch_pdl(layer_norm_kernel<T, V, kWideColumns / V>, dim3((unsigned)(a.batch * a.rows)), dim3(kWideThreads), 0, st, a);
-}
-template <typename T, int V>
-cudaError_t backward_v(const NormArgs& a, int groups, int parts, cudaStream_t st) {
-  count_launches(1);
-  return launch_pdl(layer_norm_backward_kernel<T, V, kWideBackwardColumns / V>, dim3((unsigned)parts, (unsigned)groups), dim3(kWideBackwardThreads), 0,
-                    st, a);
-}
-
 // Threads per row of the ring kernels: at most 80 elements a thread forward (75,600 x 5,120: 128 threads 306 us, 64 threads
 // 284); backward 80 bytes a thread and tensor (40 elements with two sums each; 32-bit rows take twice the place in the ring, and
 // twice the threads keep two CTAs on an SM: 2 x 4,097 x 1,000 22.5 us, with half the threads 35.1; rows that are not aligned count as 32-bit ones, bf16 2 x 4,097 x 1,001 26.3, half 58.7).
-constexpr int kRingColumns = 8192;
-int ring_threads_forward(int C) { return C <= 32 * 64 ? 32 : C <= 64 * 80 ? 64 : 128; }
+// More than 8,192 columns: 256 threads a row (a CTA per row straight from global memory, backward with 1,024 threads that walk rows:
+// 8,194 x 16,384 167 us forward, here 158, backward 587, here 211; 4,097 x 10,001 335 and 301, here 72 and 133).
+int ring_threads_forward(int C) { return C <= 32 * 64 ? 32 : C <= 64 * 80 ? 64 : C <= 128 * 64 ? 128 : 256; }
 int ring_threads_backward(int C, int e) { return C * e <= 32 * 80 ? 32 : C * e <= 64 * 80 ? 64 : C * e <= 128 * 80 ? 128 : 256; }
 // CTAs of a kernel that the SMs hold at this much shared memory; the answer for the last size is kept.
-constexpr int kRingSmem = 230000;                  // above what any layout needs (164,000: backward, fp32, 8,192 columns)
+constexpr int kRingSmem = 230000;                  // above what any layout needs (197,000: 16,384 columns)
 template <typename Kernel>
 cudaError_t resident(Kernel* kernel, int smem, int64_t& kept, int& ctas) {
   const int64_t known = __atomic_load_n(&kept, __ATOMIC_RELAXED);
@@ -775,6 +537,10 @@ cudaError_t forward_ring(NormArgs a, cudaStream_t st) {
   static int64_t kept;
   const int samples = a.gain_batch || a.offset_batch ? (int)a.batch : 1;
   a.stages = kForwardStages;
+  // where an SM holds one CTA of one row anyway, the next row is fetched a row earlier: 4,097 x 12,288 in 32 bits 85.7 -> 75.2 us (two
+  // CTAs with one row each are better: bf16 4,097 x 10,001 72 against 90)
+  if (G == 1 && RingLayout(a.C, sizeof(T), 2, 1, G, 1, kAligned).total > 113000 && RingLayout(a.C, sizeof(T), 2, 1, G, 2, kAligned).total <= kRingSmem)
+    a.stages = 2;
   const int smem = RingLayout(a.C, sizeof(T), 2, 1, G, a.stages, kAligned).total;
   int fit = 0;
   static uint64_t done;
@@ -795,12 +561,13 @@ cudaError_t forward_ring_t(const NormArgs& a, cudaStream_t st) {
     return forward_ring<T, kAligned, 8 * Q, 32>(a, st);
   }
   if (tpr == 64) return nv <= 6 * Q ? forward_ring<T, kAligned, 6 * Q, 64>(a, st) : forward_ring<T, kAligned, 10 * Q, 64>(a, st);
-  return forward_ring<T, kAligned, 8 * Q, 128>(a, st);
+  return tpr == 128 ? forward_ring<T, kAligned, 8 * Q, 128>(a, st) : forward_ring<T, kAligned, 8 * Q, 256>(a, st);
 }
 template <typename T, bool kAligned, int NV, int TPR>
 cudaError_t backward_ring(NormArgs a, int groups, int parts, cudaStream_t st) {
   constexpr int G = kRingThreads / TPR;
   a.stages = kBackwardStages;
+  if (RingLayout(a.C, sizeof(T), 1, 2, G, a.stages, kAligned).total > kRingSmem) a.stages = 1;       // 32-bit rows of more than 11,490 columns
   static uint64_t done;
   const cudaError_t e = allow_smem(&layer_norm_backward_ring_kernel<T, NV, TPR, kAligned>, kRingSmem, done);
   if (e != cudaSuccess) return e;
@@ -810,13 +577,16 @@ template <typename T, bool kAligned>
 cudaError_t backward_ring_t(const NormArgs& a, int groups, int parts, cudaStream_t st) {
   constexpr int V = 16 / (int)sizeof(T), Q = 8 / V;
   const int tpr = ring_threads_backward(a.C, kAligned ? sizeof(T) : 4);
-  const bool few = ceil_div(ceil_div(a.C, V), tpr) <= 3 * Q;
+  const int nv = ceil_div(ceil_div(a.C, V), tpr);
+  const bool few = nv <= 3 * Q;
   switch (tpr) {
     case 32: return few ? backward_ring<T, kAligned, 3 * Q, 32>(a, groups, parts, st) : backward_ring<T, kAligned, 5 * Q, 32>(a, groups, parts, st);
     case 64: return few ? backward_ring<T, kAligned, 3 * Q, 64>(a, groups, parts, st) : backward_ring<T, kAligned, 5 * Q, 64>(a, groups, parts, st);
     case 128: return few ? backward_ring<T, kAligned, 3 * Q, 128>(a, groups, parts, st) : backward_ring<T, kAligned, 5 * Q, 128>(a, groups, parts, st);
-    default: return few ? backward_ring<T, kAligned, 3 * Q, 256>(a, groups, parts, st) : backward_ring<T, kAligned, 5 * Q, 256>(a, groups, parts, st);
+    default: break;
   }
+  if (few) return backward_ring<T, kAligned, 3 * Q, 256>(a, groups, parts, st);
+  return nv <= 5 * Q ? backward_ring<T, kAligned, 5 * Q, 256>(a, groups, parts, st) : backward_ring<T, kAligned, 8 * Q, 256>(a, groups, parts, st);
 }
 // Whether all rows are whole 16-byte pieces.  (The strides of parameters do not matter to the ring kernels.)
 bool ring_aligned(const NormArgs& a, int e) {
@@ -826,22 +596,16 @@ bool ring_aligned(const NormArgs& a, int e) {
     if ((uintptr_t)p % 16) return false;
   return true;
 }
-// by type and elements per access
-#define SVOO_NORM(fn, ...)                                                                                             \
-  (type == SVOO_TYPE_BF16 ? (v == 8 ? fn<__nv_bfloat16, 8>(__VA_ARGS__) : v == 2 ? fn<__nv_bfloat16, 2>(__VA_ARGS__) : fn<__nv_bfloat16, 1>(__VA_ARGS__)) \
-   : type == SVOO_TYPE_FP16 ? (v == 8 ? fn<__half, 8>(__VA_ARGS__) : v == 2 ? fn<__half, 2>(__VA_ARGS__) : fn<__half, 1>(__VA_ARGS__))                    \
-                            : (v == 4 ? fn<float, 4>(__VA_ARGS__) : fn<float, 1>(__VA_ARGS__)))
 #define SVOO_RING(fn, aligned, ...) \
   (type == SVOO_TYPE_BF16 ? (aligned ? fn<__nv_bfloat16, true>(__VA_ARGS__) : fn<__nv_bfloat16, false>(__VA_ARGS__)) \
    : type == SVOO_TYPE_FP16 ? (aligned ? fn<__half, true>(__VA_ARGS__) : fn<__half, false>(__VA_ARGS__))             \
                             : (aligned ? fn<float, true>(__VA_ARGS__) : fn<float, false>(__VA_ARGS__)))
 }  // namespace
 
-// CTAs per group of the backward kernels: what the SMs hold at once, at most one per row (ring: per row of every group, as many
-// as for 32-bit rows whatever the type, so that the workspace does not depend on it).
+// CTAs per group of the backward kernel: what the SMs hold at once, at most one per row of every group, as many as for 32-bit rows
+// whatever the type, so that the workspace does not depend on it.
 int norm_backward_parts(int64_t rows, int groups, int C) {
-  const bool ring = C <= kRingColumns;
-  int64_t parts = (int64_t)148 * (ring ? 2 : 1) / groups, jobs = ring ? ceil_div64(rows, kRingThreads / ring_threads_backward(C, 4)) : rows;
+  int64_t parts = (int64_t)148 * (C <= 8192 ? 2 : 1) / groups, jobs = ceil_div64(rows, kRingThreads / ring_threads_backward(C, 4));
   if (parts > jobs) parts = jobs;
   return parts < 1 ? 1 : (int)parts;
 }
@@ -851,16 +615,13 @@ int64_t norm_backward_bytes(int64_t batch, int64_t rows, int groups, int C) {
 
 cudaError_t launch_layer_norm(int type, const NormArgs& a, cudaStream_t st) {
   const int e = elem_bytes(type);
-  if (a.C <= kRingColumns) return SVOO_RING(forward_ring_t, ring_aligned(a, e), a, st);
-  const int v = norm_vector(a, e);
-  return SVOO_NORM(forward_v, a, st);
+  return SVOO_RING(forward_ring_t, ring_aligned(a, e), a, st);
 }
 
 cudaError_t launch_layer_norm_backward(int type, const NormArgs& a, int groups, void* dgain, void* doffset, cudaStream_t st) {
-  const int elem = elem_bytes(type), v = norm_vector(a, elem);
-  const bool ring = a.C <= kRingColumns, aligned = ring_aligned(a, elem);
+  const bool aligned = ring_aligned(a, elem_bytes(type));
   const int parts = norm_backward_parts(groups > 1 ? a.rows : a.batch * a.rows, groups, a.C);
-  const cudaError_t e = ring ? SVOO_RING(backward_ring_t, aligned, a, groups, parts, st) : SVOO_NORM(backward_v, a, groups, parts, st);
+  const cudaError_t e = SVOO_RING(backward_ring_t, aligned, a, groups, parts, st);
   if (e != cudaSuccess || !a.partial) return e;
   const dim3 grid((unsigned)ceil_div(a.C, 32), (unsigned)groups, 2);
   const bool f32 = a.params_fp32 || type == SVOO_TYPE_FP32;

@@ -47,18 +47,6 @@ struct alignas(sizeof(T) * V) Vec {
 };
 template <typename T, int V>
 __device__ __forceinline__ Vec<T, V> load_vec(const T* p) { return *reinterpret_cast<const Vec<T, V>*>(p); }
-// read once: not kept in L1
-template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> load_stream(const T* p) {
-  Vec<T, V> r;
-  if constexpr (sizeof(r) == 16) {
-    const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p));
-    r = *reinterpret_cast<const Vec<T, V>*>(&u);
-  } else {
-    r = load_vec<T, V>(p);
-  }
-  return r;
-}
 
 __device__ __forceinline__ float warp_sum(float s) {
 #pragma unroll
