@@ -67,7 +67,6 @@ struct LinTile {
 
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, uint32_t src) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(src) : "memory");
-  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
 // One warp's staged box of 32 rows x 128 bytes (16-byte piece p of row r at p ^ (r & 7): the 128-byte swizzle) to out rows
@@ -295,7 +294,8 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
 #pragma unroll
         for (int i = 0; i < 2; ++i) sum[c / 2 + i] = kGelu ? gelu2(v[i]) : v[i];
       };
-      // a box is written again when the store before the last has read it
+      // A box is written again when the store before the last, its own, has read it.  Every box is a group, an empty one where all of it
+      // lies outside the result: otherwise the wait would count a store that is one box older.
       auto begin_box = [&](int i) {
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
         __syncwarp();
@@ -304,7 +304,10 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
       auto end_box = [&](const unsigned char* at, int n) {
         fence_async_proxy();
         __syncwarp();
-        if (lane == 0 && !skip) tma_store_2d(&tm_out, n, row0, smem_u32(at));
+        if (lane == 0) {
+          if (!skip) tma_store_2d(&tm_out, n, row0, smem_u32(at));
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
       };
       if constexpr (OUT == SVOO_TYPE_E4M3) {
         // the thread's 128 columns are one block of its row; columns behind N are zero
