@@ -10,6 +10,9 @@
 
 namespace svoo {
 
+// Bytes that a row of n numbers takes: zeros up to the next multiple of 16, whatever the pitch.  What follows may be another's.
+__device__ __forceinline__ int written(int n) { return (n + 15) & ~15; }
+
 // The largest magnitude of a half warp's 128 values, as the pattern of a 32-bit number: 16-bit numbers by their own patterns,
 // two at a time.
 template <typename T>
@@ -85,7 +88,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = to_f32(raw[u].v[i]);
     const uint2 out = by.e4m3x8<sizeof(T) == 2>(v);
-    if (k < q_pitch) *reinterpret_cast<uint2*>(q + row[u] * q_pitch + k) = out;      // zeros behind the row
+    if (k < written(K)) *reinterpret_cast<uint2*>(q + row[u] * q_pitch + k) = out;
   }
 }
 
@@ -145,7 +148,7 @@ __global__ void __launch_bounds__(512, sizeof(T) == 2 ? 3 : 2) quantize_blocks_k
     for (int i = 0; i < 4; ++i) {
       const Vec<T, 4>& t = v[g * 4 + i];
       o[i] = by.e4m3x4<sizeof(T) == 2>(to_f32(t.v[0]), to_f32(t.v[1]), to_f32(t.v[2]), to_f32(t.v[3]));
-      if (n0 + g * 4 + i < N && k < q_pitch) *reinterpret_cast<uint32_t*>(q + (int64_t)(n0 + g * 4 + i) * q_pitch + k) = o[i];
+      if (n0 + g * 4 + i < N && k < written(K)) *reinterpret_cast<uint32_t*>(q + (int64_t)(n0 + g * 4 + i) * q_pitch + k) = o[i];
     }
     if (qt) {
       transpose4(o);
@@ -158,7 +161,7 @@ __global__ void __launch_bounds__(512, sizeof(T) == 2 ? 3 : 2) quantize_blocks_k
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int c = w * 8 + i, n = nb * kBlock + lane * 4;
-    if (kb * kBlock + c < K && n < qt_pitch)
+    if (kb * kBlock + c < K && n < written(N))
       *reinterpret_cast<uint32_t*>(qt + (int64_t)(kb * kBlock + c) * qt_pitch + n) = words[c][lane ^ (c / 4)];
   }
 }
@@ -222,7 +225,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quantize_tile_ker
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = to_f32(raw[u].v[i]);
         const uint2 out = by.e4m3x8<sizeof(T) == 2>(v);
-        if (k < q_pitch) *reinterpret_cast<uint2*>(q + (int64_t)m * q_pitch + k) = out;
+        if (k < written(K)) *reinterpret_cast<uint2*>(q + (int64_t)m * q_pitch + k) = out;
       }
     }
   }
@@ -275,7 +278,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quantize_tile_ker
 #pragma unroll
     for (int g = 0; g < R / 16; ++g) {
       const int r = seg * R + g * 16;
-      if (m0 + r >= qt_pitch) break;
+      if (m0 + r >= written(M)) break;
       uint32_t o[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
