@@ -403,7 +403,8 @@ int svoo_b200_layer_norm(const void* x, int32_t x_type, int64_t batch, int64_t r
                          int32_t gain_plus_one, float eps, void* y, float* mean, float* rstd, void* stream);
 /* Its gradient: dx (dense, x_type) from dy [batch, rows, C] (x_type, last dimension dense), x and the statistics of the
  * forward call.  dgain, doffset (param_type; both or none): sums over the rows of each sample, [batch, C], where
- * per_sample != 0, otherwise over all rows, [C].  The sums run in a fixed order; with batch 0 nothing is written.
+ * per_sample != 0, otherwise over all rows, [C].  Samples with gains of their own (gain_batch != 0, batch > 1) have gradients
+ * of their own: they want per_sample where dgain is given.  The sums run in a fixed order; with batch 0 nothing is written.
  * workspace: layer_norm_workspace_bytes, needed with dgain. */
 int svoo_b200_layer_norm_workspace_bytes(int64_t batch, int64_t rows, int64_t C, int32_t per_sample, int64_t* bytes_out);
 int svoo_b200_layer_norm_backward(const void* dy, int64_t dy_batch, int64_t dy_row, const void* x, int32_t x_type, int64_t batch,

@@ -136,7 +136,9 @@ int svoo_b200_layer_norm_backward(const void* dy, int64_t dy_batch, int64_t dy_r
                                   const void* gain, int64_t gain_batch, int32_t param_type, int32_t gain_plus_one,
                                   int32_t per_sample, void* dx, void* dgain, void* doffset, void* workspace,
                                   int64_t workspace_bytes, void* stream) {
-  SVOO_TRY(check_norm(x_type, batch, rows, C, x_batch, x_row, param_type, per_sample != 0));
+  const bool own_gain = batch > 1 && gain_batch != 0;       // a gain for every sample, as the forward call has it
+  SVOO_TRY(check_norm(x_type, batch, rows, C, x_batch, x_row, param_type, per_sample != 0 || own_gain));
+  if (own_gain && !per_sample && dgain) return SVOO_ERR_SHAPE;
   if (dy_batch < 0 || dy_row < 0 || gain_batch < 0) return SVOO_ERR_SHAPE;
   if (!dgain != !doffset || (dgain && !workspace)) return SVOO_ERR_NULL;
   if (batch == 0) return SVOO_OK;                          // no sample, no sums of one; shared sums are the caller's to clear
@@ -146,7 +148,7 @@ int svoo_b200_layer_norm_backward(const void* dy, int64_t dy_batch, int64_t dy_r
   if (!aligned(x, e) || !aligned(dy, e) || !aligned(dx, e) || !aligned(gain, pe) || !aligned(dgain, pe) || !aligned(doffset, pe) ||
       !aligned(workspace, 4) || !aligned(mean, 4) || !aligned(rstd, 4))
     return SVOO_ERR_ALIGN;
-  const int64_t groups = norm_groups(batch, per_sample);
+  const int64_t groups = norm_groups(batch, per_sample || own_gain);
   if (dgain && workspace_bytes < norm_backward_bytes(batch, rows, (int)groups, (int)C)) return SVOO_ERR_WORKSPACE;
   NormArgs a = {};
   a.x = x, a.dy = dy, a.dx = dx, a.gain = gain, a.mean_in = mean, a.rstd_in = rstd, a.partial = dgain ? (float*)workspace : nullptr;

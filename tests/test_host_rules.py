@@ -176,3 +176,14 @@ def test_token_kernels_need_a_model_on_its_gpu():
     with pytest.raises(ValueError, match="GPU"):
         model.use_token_kernels()
     assert not model.blocks[0].fused_norms and isinstance(model.blocks[0].attn1.to_q, torch.nn.Linear)
+
+
+def test_gradient_of_samples_with_gains_of_their_own():
+    """Shared sums of gains that differ by sample are refused on the host, as are more such samples than the grid has."""
+    import ctypes
+    from svoo_b200._lib import LIB as L
+    buf = ctypes.create_string_buffer(4096)
+    p = (ctypes.addressof(buf) + 255) // 256 * 256
+    back = lambda b, gb, per, dg: L.svoo_b200_layer_norm_backward(p, 128, 64, p, 0, b, 2, 64, 128, 64, p, p, p, gb, 2, 1, per, p, dg, dg, p, 4, None)  # noqa: E731
+    assert back(2, 64, 0, p) == -2 and back(2, 64, 1, p) == -4 and back(2, 0, 0, p) == -4 and back(1, 64, 0, p) == -4
+    assert back(70000, 64, 0, None) == -2 and back(70000, 64, 1, p) == -2
