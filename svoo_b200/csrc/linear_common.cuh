@@ -103,8 +103,8 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 // GELU of two values: y / 2 (1 + tanh u) = y / (1 + exp(-2 u)), u = sqrt(2 / pi) (y + 0.044715 y^3).  The special-function unit is
-// what it costs most on: the two share a reciprocal (1 / d0 = d1 / (d0 d1)); exponents are cut at 60, where GELU is below 2^-57,
-// so that the product stays finite.
+// what it costs most on: the two share a reciprocal (1 / d0 = d1 / (d0 d1)); exponents are cut at 60, so that the product stays
+// finite.  Behind the cut, y < -7.47, GELU is below 2^-57: zero here, however large y is (the formula's NaN for minus infinity).
 __device__ __forceinline__ uint64_t gelu2(uint64_t y) {
   constexpr float k = -2.f * 0.7978845608028654f * 1.4426950408889634f;
   // constants in scalar operations: a pair of each would take registers that the epilogue does not have
@@ -113,7 +113,7 @@ __device__ __forceinline__ uint64_t gelu2(uint64_t y) {
   const float d[2] = {1.f + fast_exp2(fminf(half_of(a, 0), 60.f)), 1.f + fast_exp2(fminf(half_of(a, 1), 60.f))};
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d[0] * d[1]));
-  return mul2(y, mul2(pack2(d[1], d[0]), pack2(r, r)));
+  return mul2(y, mul2(pack2(d[1], d[0]), pack2(half_of(a, 0) > 60.f ? 0.f : r, half_of(a, 1) > 60.f ? 0.f : r)));
 }
 // the largest of three magnitudes; NaN if one is
 __device__ __forceinline__ float max_magnitude(float top, uint64_t v) {
