@@ -468,8 +468,9 @@ int svoo_b200_linear_train_backward(const void* dy, int32_t x_type, int64_t M, i
                                     int64_t saved_bytes, int32_t keep_x_grad, int32_t keep_w_grad, void* dx, void* dw,
                                     int32_t w_type, void* db, int32_t bias_type, void* scratch, int64_t scratch_bytes,
                                     void* stream);
-/* Copies the product's status word of the current device to *status (device int32): 0, or 1 after a kernel gave up on a
- * bounded wait and left rows unwritten. */
+/* Copies the status word of the layer norms and products on the current device to *status (device int32): 0, or 1 once a kernel
+ * has given up on a bounded wait (about a second) and left rows unwritten, and the gradients of norm parameters that it
+ * was to give NaN.  The word stays 1. */
 int svoo_b200_linear_status(int32_t* status, void* stream);
 
 #ifdef __cplusplus

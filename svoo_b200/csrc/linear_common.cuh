@@ -59,7 +59,7 @@ __device__ __forceinline__ uint32_t at_cta(uint32_t addr, int rank) {
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void pair_sync() {
+__device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src) {

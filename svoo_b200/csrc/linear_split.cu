@@ -31,6 +31,10 @@ __device__ __forceinline__ float4 load_cluster(uint32_t addr) {
   return v;
 }
 
+__device__ __forceinline__ void store_cluster(uint32_t addr, int v) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
 template <int OUT, bool kGelu>
 __global__ void __launch_bounds__(kSplitThreads, 1) linear_split_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                                                                      const LinearArgs a) {
@@ -152,9 +156,14 @@ __global__ void __launch_bounds__(kSplitThreads, 1) linear_split_kernel(const __
     }
   }
   __syncthreads();
-  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+  // a CTA that gave up on a wait has left no sums: the others learn of it, and the tile stays unwritten
+  if (warp == 0) {
+    if (lane < ranks && *abort_flag) store_cluster(at_cta(bars + SPL_BARS * 8 + 8, lane), 1);
+    __syncwarp();
+  }
+  cluster_sync();
   // rows of this CTA; a lane holds four columns
-  const int rows = a.M - row0 < kSplitM ? a.M - row0 : kSplitM;
+  const int rows = *abort_flag ? 0 : a.M - row0 < kSplitM ? a.M - row0 : kSplitM;
   const int n = n0 + lane * 4;
   float bias[4];
   bias_columns(a, n, 1, bias);
@@ -202,7 +211,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) linear_split_kernel(const __
     }
   }
   __syncwarp();
-  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");   // nobody reads this CTA's sums any more
+  cluster_sync();                                            // nobody reads this CTA's sums any more
   if (tid == 0 && *abort_flag) atomicExch(a.status, 1);
   if (warp == 1) {
     tc_fence_after();

@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
   pdl_trigger();
   tc_fence_before();
   __syncthreads();
-  pair_sync();                                             // the other CTA's barriers are set up before they are signalled
+  cluster_sync();                                          // the other CTA's barriers are set up before they are signalled
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc_kernel(const __grid_
   }
   tc_fence_before();
   __syncthreads();
-  pair_sync();
+  cluster_sync();
   if (tid == 0 && *abort_flag) atomicExch(a.status, 1);
   if (warp == 1) {
     tc_fence_after();

@@ -466,7 +466,8 @@ __global__ void __launch_bounds__(kRingThreads) layer_norm_backward_ring_kernel(
       __syncthreads();
     }
     float* out = a.partial + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 * a.C;
-    for (int c = threadIdx.x; c < 2 * a.C; c += kRingThreads) out[c] = acc[c < a.C ? c : c - a.C + lay.columns];
+    const bool whole = !*abort_flag;                       // rows are missing after a wait that expired
+    for (int c = threadIdx.x; c < 2 * a.C; c += kRingThreads) out[c] = whole ? acc[c < a.C ? c : c - a.C + lay.columns] : NAN;
   }
   leave(bars, stages, issued, t, abort_flag, a.status);
 }

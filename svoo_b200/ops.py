@@ -973,8 +973,8 @@ def linear_train_backward(grad: torch.Tensor, saved: torch.Tensor, K: int, keep_
 
 
 def linear_status(device: torch.device) -> int:
-    """Status word of the 8-bit products on this device (synchronises): 0, or 1 after a kernel gave up on a bounded wait and
-    left rows unwritten."""
+    """Status word of the layer norms and 8-bit products on this device (synchronises): 0, or 1 once a kernel has given up on a
+    bounded wait and left rows unwritten.  It stays 1."""
     with torch.cuda.device(device):
         out = torch.zeros(1, dtype=torch.int32, device="cuda")
         check(LIB.svoo_b200_linear_status(out.data_ptr(), _stream()), "linear_status")
