@@ -587,8 +587,7 @@ def run_dit_arm(args):
     if world > 1:
         dist.all_reduce(ms, op=dist.ReduceOp.MAX)
     step_ms, attn_ms = ms.tolist()
-    for p in procs:
-        p.check_status()
+    model.check_status()
     barrier()
     e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
     e0.record()

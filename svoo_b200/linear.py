@@ -80,6 +80,13 @@ class _NoRows(torch.autograd.Function):
         return tuple(grad.new_zeros(like[0], dtype=like[1]) if need else None for like, need in zip(ctx.like, ctx.needs_input_grad))
 
 
+def check_status(device: torch.device) -> None:
+    """Raises if a layer norm or an 8-bit product on this device has given up on one of its bounded waits (its output is then
+    incomplete).  Reads a device word, so it synchronises: call it once per step or at the end of a run."""
+    if ops.linear_status(device) != 0:
+        raise RuntimeError(f"a layer norm or an 8-bit product on {device} timed out on a barrier; output incomplete")
+
+
 def linear_fp8(x: torch.Tensor, weight: Union[torch.Tensor, Fp8Weight], bias: Optional[torch.Tensor] = None,
                activation: Optional[str] = None) -> torch.Tensor:
     """act(x weight^T + bias) for x [..., K] (bf16, fp16 or fp32) -> [..., N] of x's type.  `weight` is an Fp8Weight, or a tensor

@@ -187,3 +187,32 @@ def test_gradient_of_samples_with_gains_of_their_own():
     back = lambda b, gb, per, dg: L.svoo_b200_layer_norm_backward(p, 128, 64, p, 0, b, 2, 64, 128, 64, p, p, p, gb, 2, 1, per, p, dg, dg, p, 4, None)  # noqa: E731
     assert back(2, 64, 0, p) == -2 and back(2, 64, 1, p) == -4 and back(2, 0, 0, p) == -4 and back(1, 64, 0, p) == -4
     assert back(70000, 64, 0, None) == -2 and back(70000, 64, 1, p) == -2
+
+
+def test_a_model_reports_token_kernels_that_gave_up(monkeypatch):
+    """check_status asks every processor, and the token-wise kernels of the model's device once blocks are on them; it raises."""
+    import pytest
+    import torch
+    from svoo_b200 import ops, wan_dit
+    cfg = wan_dit.WanDiTConfig(num_layers=2, dim=128, heads=1, ffn_dim=128, text_dim=16, text_len=4, latent=(1, 4, 4))
+    model = wan_dit.WanDiT(cfg)
+    asked, word = [], [0]
+
+    class Processor:
+        def check_status(self):
+            asked.append("processor")
+
+    def status(device):
+        asked.append(device)
+        return word[0]
+
+    monkeypatch.setattr(ops, "linear_status", status)
+    model.blocks[1].attn1.set_processor(Processor())
+    model.check_status()
+    assert asked == ["processor"]
+    model.blocks[1].fused_norms = True
+    model.check_status()
+    assert asked == ["processor"] * 2 + [torch.device("cpu")]
+    word[0] = 1
+    with pytest.raises(RuntimeError, match="incomplete"):
+        model.check_status()
