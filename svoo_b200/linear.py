@@ -94,6 +94,7 @@ def linear_fp8(x: torch.Tensor, weight: Union[torch.Tensor, Fp8Weight], bias: Op
     products in e4m3 as well: the gradient of the output is quantised in blocks along what each of them sums over, and
     rounding counts as the identity.  An Fp8Weight is a constant; with it the gradient of x needs its transpose
     (ops.quantize_blocks(w, transposed=True)).  An activation has no gradient here."""
+    ops.refuse_tangents(x, weight if isinstance(weight, torch.Tensor) else None, bias)
     training = torch.is_grad_enabled() and (x.requires_grad or (isinstance(weight, torch.Tensor) and weight.requires_grad) or
                                             (bias is not None and bias.requires_grad))
     m = _rows(x)
@@ -112,6 +113,7 @@ def mlp_fp8(x: torch.Tensor, w1: Fp8Weight, bias1: Optional[torch.Tensor], w2: F
             bias2: Optional[torch.Tensor]) -> torch.Tensor:
     """linear(gelu(linear(x, w1, bias1)), w2, bias2), GELU with its tanh formula: the feed-forward of a block.  The hidden rows are
     quantised from their 32-bit values as the first product leaves its registers.  Inference only."""
+    ops.refuse_tangents(x, bias1, bias2)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, bias1, bias2)):
         raise ValueError("mlp_fp8 has no gradient: use two linear_fp8 around the activation")
     h = ops.linear_fp8(_rows(x), w1, bias1, "gelu", ops.E4M3)

@@ -35,7 +35,8 @@ class _LayerNorm(torch.autograd.Function):
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                scale: Optional[torch.Tensor] = None, shift: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
-    """ops.layer_norm with gradients for x and the parameters."""
+    """ops.layer_norm with gradients for x and the parameters (backward mode)."""
+    ops.refuse_tangents(x, weight, bias, scale, shift)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, scale, shift)):
         return _LayerNorm.apply(x, weight, bias, scale, shift, eps)
     return ops.layer_norm(x, weight, bias, scale, shift, eps)

@@ -11,6 +11,7 @@ import functools
 from typing import Dict, Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import LIB, check
 
@@ -563,6 +564,12 @@ def _device(*tensors: Optional[torch.Tensor]) -> int:
         elif at != index:
             raise ValueError("all tensors of a call must be on one device")
     return index
+
+
+def refuse_tangents(*tensors: Optional[torch.Tensor]) -> None:
+    """Raises where a tensor carries a tangent of forward-mode differentiation: the kernels would drop it."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("svoo_b200 operators have no forward-mode gradient")
 
 
 def _ptr(t: Optional[torch.Tensor]) -> int:

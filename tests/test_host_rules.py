@@ -216,3 +216,27 @@ def test_a_model_reports_token_kernels_that_gave_up(monkeypatch):
     word[0] = 1
     with pytest.raises(RuntimeError, match="incomplete"):
         model.check_status()
+
+
+def test_forward_mode_is_refused():
+    """A tangent on any tensor of a call raises before anything else is looked at; without one the call gets to its other checks."""
+    import pytest
+    import torch
+    from torch.autograd import forward_ad
+    from svoo_b200 import linear, norm
+    x, w, v = torch.randn(4, 8), torch.randn(8, 8), torch.randn(8)
+    stored = linear.Fp8Weight(w.to(torch.float8_e4m3fn), torch.ones(1, 1))
+    with forward_ad.dual_level():
+        dual = [forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, w, v)]
+        for fn, args in ((norm.layer_norm, (dual[0],)), (norm.layer_norm, (x, dual[2], v)), (norm.layer_norm, (x, v, dual[2])),
+                         (linear.linear_fp8, (dual[0], w)), (linear.linear_fp8, (x, dual[1])), (linear.linear_fp8, (x, w, dual[2])),
+                         (linear.linear_fp8, (dual[0], stored)), (linear.mlp_fp8, (dual[0], stored, v, stored, v)),
+                         (linear.mlp_fp8, (x, stored, v, stored, dual[2]))):
+            with pytest.raises(NotImplementedError):
+                fn(*args)
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                fn(*args)
+        with pytest.raises(ValueError, match="CUDA"):
+            norm.layer_norm(x, v, v)
+    with pytest.raises(ValueError, match="CUDA"):
+        linear.linear_fp8(x, w)
