@@ -5,7 +5,8 @@
 //   dx = rstd (w - sum(w) / C - xhat sum(w xhat) / C),  w = dy g;    dg = sum_rows dy xhat,  do = sum_rows dy
 //
 // Everything between the loads and the stores is in 32 bits.  The variance is taken around the mean from the row in
-// registers, so a mean far from zero costs no digits.  A row whose values are not all finite comes out NaN.
+// registers, and both directions subtract the mean before they scale, so a mean far from zero costs no digits but those of the mean
+// itself (a few 2^-24 of the row's largest magnitude).  A row whose values are not all finite comes out NaN.
 #include "rows_common.cuh"
 #include "tc_common.cuh"
 
@@ -378,7 +379,7 @@ __global__ void __launch_bounds__(kRingThreads) layer_norm_backward_ring_kernel(
     ok = tc::mbar_wait(bars + 8 * s, phase, abort_flag) && ok;
     const unsigned char *xs = ring + s * 2 * lay.row, *ds = xs + lay.row;
     const int x_shift = kAligned ? 0 : shift_of(x_of(r)), d_shift = kAligned ? 0 : shift_of(dy_of(r));
-    const uint64_t rs = f2(rstd, rstd), shift = f2(-mean * rstd, -mean * rstd);       // xhat = x rstd - mean rstd
+    const uint64_t rs = f2(rstd, rstd), minus = f2(-mean, -mean);      // xhat = (x - mean) rstd, as the forward call has it
     uint64_t s1 = 0, s2 = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(kRingThreads) layer_norm_backward_ring_kernel(
 #pragma unroll
         for (int k = 0; k < P; ++k) {
           const ulonglong2 gv = read_param<T, kAligned, TPR>(gain, i, k / 2, t, a.C);
-          const uint64_t h = fma2(x[k], rs, shift), w = mul2(d[k], k & 1 ? gv.y : gv.x);
+          const uint64_t h = mul2(add2(x[k], minus), rs), w = mul2(d[k], k & 1 ? gv.y : gv.x);
           dg[i][k] = fma2(d[k], h, dg[i][k]);
           dof[i][k] = add2(dof[i][k], d[k]);
           s1 = add2(s1, w);
@@ -399,8 +400,8 @@ __global__ void __launch_bounds__(kRingThreads) layer_norm_backward_ring_kernel(
     }
     float sums[2] = {lo2(s1) + hi2(s1), lo2(s2) + hi2(s2)};
     group_sums<TPR, 2>(sums, slots[turn][group], group);
-    // dx = w rstd - (s1 + xhat s2) rstd = d g rstd + (x (-s2 rstd rstd) + (mean rstd s2 - s1) rstd)
-    const float m1 = sums[0] * inv_c, m2 = sums[1] * inv_c;
+    // dx = rstd (w - s1 - (x - mean) (rstd s2)), s1 and s2 over C
+    const float m1 = sums[0] * inv_c, m2 = sums[1] * inv_c * rstd;
     const uint64_t a2 = f2(-m2, -m2), a1 = f2(-m1, -m1);
     T* dx = static_cast<T*>(a.dx) + (sample_row + r) * a.C;
 #pragma unroll
@@ -412,8 +413,7 @@ __global__ void __launch_bounds__(kRingThreads) layer_norm_backward_ring_kernel(
 #pragma unroll
         for (int k = 0; k < P; ++k) {
           const ulonglong2 gv = read_param<T, kAligned, TPR>(gain, i, k / 2, t, a.C);
-          const uint64_t h = fma2(x[k], rs, shift);
-          d[k] = mul2(fma2(h, a2, fma2(d[k], k & 1 ? gv.y : gv.x, a1)), rs);
+          d[k] = mul2(fma2(add2(x[k], minus), a2, fma2(d[k], k & 1 ? gv.y : gv.x, a1)), rs);
         }
         if (ok) write_piece<T, kAligned, TPR>(dx, i, t, a.C, d);
       }
