@@ -579,14 +579,24 @@ cudaError_t backward_ring_t(const NormArgs& a, int groups, int parts, cudaStream
   constexpr int V = 16 / (int)sizeof(T), Q = 8 / V;
   const int tpr = ring_threads_backward(a.C, kAligned ? sizeof(T) : 4);
   const int nv = ceil_div(ceil_div(a.C, V), tpr);
-  const bool few = nv <= 3 * Q;
+  // up to 128 threads a row, 80 bytes a thread: 32-bit rows and those that count as such stay within 3 Q pieces
+  if constexpr (kAligned && sizeof(T) == 2) {
+    if (nv > 3 * Q) {
+      switch (tpr) {
+        case 32: return backward_ring<T, kAligned, 5 * Q, 32>(a, groups, parts, st);
+        case 64: return backward_ring<T, kAligned, 5 * Q, 64>(a, groups, parts, st);
+        case 128: return backward_ring<T, kAligned, 5 * Q, 128>(a, groups, parts, st);
+        default: break;
+      }
+    }
+  }
   switch (tpr) {
-    case 32: return few ? backward_ring<T, kAligned, 3 * Q, 32>(a, groups, parts, st) : backward_ring<T, kAligned, 5 * Q, 32>(a, groups, parts, st);
-    case 64: return few ? backward_ring<T, kAligned, 3 * Q, 64>(a, groups, parts, st) : backward_ring<T, kAligned, 5 * Q, 64>(a, groups, parts, st);
-    case 128: return few ? backward_ring<T, kAligned, 3 * Q, 128>(a, groups, parts, st) : backward_ring<T, kAligned, 5 * Q, 128>(a, groups, parts, st);
+    case 32: return backward_ring<T, kAligned, 3 * Q, 32>(a, groups, parts, st);
+    case 64: return backward_ring<T, kAligned, 3 * Q, 64>(a, groups, parts, st);
+    case 128: return backward_ring<T, kAligned, 3 * Q, 128>(a, groups, parts, st);
     default: break;
   }
-  if (few) return backward_ring<T, kAligned, 3 * Q, 256>(a, groups, parts, st);
+  if (nv <= 3 * Q) return backward_ring<T, kAligned, 3 * Q, 256>(a, groups, parts, st);
   return nv <= 5 * Q ? backward_ring<T, kAligned, 5 * Q, 256>(a, groups, parts, st) : backward_ring<T, kAligned, 8 * Q, 256>(a, groups, parts, st);
 }
 // Whether all rows are whole 16-byte pieces.  (The strides of parameters do not matter to the ring kernels.)

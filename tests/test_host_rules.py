@@ -240,3 +240,26 @@ def test_forward_mode_is_refused():
             norm.layer_norm(x, v, v)
     with pytest.raises(ValueError, match="CUDA"):
         linear.linear_fp8(x, w)
+
+
+def test_norm_kernels_are_those_that_sizes_choose():
+    """The library holds a norm kernel for a type, alignment and number of pieces and threads only where some number of columns takes it."""
+    import re
+    names = subprocess.run(["nm", "-C", build.build()], capture_output=True, text=True).stdout
+    held = {(d or "", t, int(nv), int(tpr), al == "true") for d, t, nv, tpr, al in
+            re.findall(r"layer_norm(_backward)?_ring_kernel<(\w+), (\d+), (\d+), (true|false)>", names)}
+    chosen = set()
+    for t, e in (("__nv_bfloat16", 2), ("__half", 2), ("float", 4)):
+        per_piece = 16 // e
+        for aligned in (True, False):
+            for C in range(1, 16385):
+                if aligned and C * e % 16:
+                    continue
+                pieces, unit = -(-C // per_piece), 8 // per_piece
+                tpr = 32 if C <= 2048 else 64 if C <= 5120 else 128 if C <= 8192 else 256
+                steps = {32: (2, 4, 6, 8), 64: (6, 10), 128: (8,), 256: (8,)}[tpr]
+                chosen.add(("", t, min(n * unit for n in steps if n * unit * tpr >= pieces), tpr, aligned))
+                wide = C * (e if aligned else 4)
+                tpr = 32 if wide <= 2560 else 64 if wide <= 5120 else 128 if wide <= 10240 else 256
+                chosen.add(("_backward", t, min(n * unit for n in (3, 5, 8) if n * unit * tpr >= pieces), tpr, aligned))
+    assert held == chosen, held ^ chosen
