@@ -247,6 +247,7 @@ __global__ void __launch_bounds__(kRingThreads) layer_norm_ring_kernel(const Nor
   auto row_of = [&](int r) { return static_cast<const T*>(a.x) + row_offset(a, per_sample, blockIdx.y, r, a.x_batch, a.x_row); };
   auto fetch = [&](int r, int s) {
     const RowCopy c = plan_row<T, kAligned>(ring + s * lay.row, row_of(r), a.C, a.x, a.x_end);
+    if (!kAligned) tc::fence_async_proxy();                // elements that plan_row stored here for an earlier row come before this copy
     tc::mbar_expect_tx(bars + 8 * s, c.bytes);
     start_copy(ring + s * lay.row, c, bars + 8 * s);
   };
@@ -354,6 +355,7 @@ __global__ void __launch_bounds__(kRingThreads) layer_norm_backward_ring_kernel(
   auto fetch = [&](int r, int s) {
     unsigned char *px = ring + s * 2 * lay.row, *pd = px + lay.row;
     const RowCopy cx = plan_row<T, kAligned>(px, x_of(r), a.C, a.x, a.x_end), cd = plan_row<T, kAligned>(pd, dy_of(r), a.C, a.dy, a.dy_end);
+    if (!kAligned) tc::fence_async_proxy();                // as in the forward kernel
     tc::mbar_expect_tx(bars + 8 * s, cx.bytes + cd.bytes);
     start_copy(px, cx, bars + 8 * s);
     start_copy(pd, cd, bars + 8 * s);
