@@ -115,3 +115,74 @@ def test_training_step_on_pairs_of_sms(dtype):
     ref = dy.double().sum(0)
     # 64 additions of 128 rows' sums and of 41 such sums
     assert ((db.double() - ref).abs() <= 110 * 2.0 ** -24 * dy.double().abs().sum(0) + 1e-30).all()
+
+
+@pytest.mark.parametrize("xt,wt,bt", [(torch.bfloat16, torch.float32, torch.float16), (torch.float16, torch.bfloat16, torch.float32),
+                                      (torch.float32, torch.float16, torch.bfloat16)])
+@pytest.mark.parametrize("M,N,K", [(40, 72, 200), (9000, 777, 130)])
+def test_training_with_types_of_their_own(M, N, K, xt, wt, bt):
+    """Input, weight and bias of three types: every gradient is of its tensor's type, and the weight's or the bias's may be asked for alone."""
+    from svoo_b200 import linear
+    x, w, b = rand(M, K, xt, 1), rand(N, K, wt, 2, 0.05), rand(1, N, bt, 3)[0]
+    dy = rand(M, N, xt, 4, 0.01)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = linear.linear_fp8(x, w, b)
+    grads = torch.autograd.grad(y, leaves, dy)
+    assert y.dtype == xt and [g.dtype for g in grads] == [xt, wt, bt]
+    x, w, b = (t.detach() for t in leaves)
+    for got, u, v, add in ((y.detach(), R.dequantize(x, 1, 128), R.dequantize(w, 128, 128), b.double()),
+                           (grads[0], R.dequantize(dy, 1, 128), R.dequantize(w, 128, 128).t(), torch.zeros((), device=DEV)),
+                           (grads[1], R.dequantize(dy.t().contiguous(), 1, 128), R.dequantize(x.t().contiguous(), 1, 128), torch.zeros((), device=DEV))):
+        want = u @ v.t() + add
+        assert ((got.double() - want).abs() <= R.product_bound(u, v, got.dtype, want) + 2.0 ** -22 * add.abs()).all()
+    for i in (1, 2):
+        assert torch.equal(torch.autograd.grad(linear.linear_fp8(*leaves), leaves[i:i + 1], dy)[0], grads[i])
+
+
+def test_one_tensor_in_two_places():
+    """x as its own weight: both gradients add up; scale and shift of a norm from one leaf as well."""
+    from svoo_b200 import linear, norm
+    x = rand(300, 200, torch.float32, 5).requires_grad_(True)
+    u = x.detach().clone().requires_grad_(True)
+    dy = rand(300, 300, torch.float32, 6)
+    both, = torch.autograd.grad(linear.linear_fp8(x, x), (x,), dy)
+    one, two = torch.autograd.grad(linear.linear_fp8(x, u), (x, u), dy)
+    assert torch.equal(both, one + two)
+    s = rand(2, 64, torch.float32, 7).requires_grad_(True)
+    z, dz = rand(20, 64, torch.float32, 8).view(2, 10, 64), rand(20, 64, torch.float32, 9).view(2, 10, 64)
+    t = s.detach().clone().requires_grad_(True)
+    both, = torch.autograd.grad(norm.layer_norm(z, scale=s, shift=s), (s,), dz)
+    one, two = torch.autograd.grad(norm.layer_norm(z, scale=s, shift=t), (s, t), dz)
+    assert torch.equal(both, one + two)
+
+
+def test_walking_products_on_two_streams_and_in_a_graph():
+    """A training step whose products walk, eagerly on two streams at once and replayed: the same bits."""
+    from svoo_b200 import linear
+    x, w, b = (t.requires_grad_(True) for t in (rand(5200, 1300, torch.bfloat16, 1), rand(2310, 1300, torch.bfloat16, 2, 0.05), rand(1, 2310, torch.bfloat16, 3)[0]))
+    dy = rand(5200, 2310, torch.bfloat16, 4, 0.01)
+
+    def step():
+        y = linear.linear_fp8(x, w, b)
+        return (y.detach(), *torch.autograd.grad(y, (x, w, b), dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(u, v) for u, v in zip(got, want))
+    streams, results = [torch.cuda.Stream() for _ in range(2)], []
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    for _ in range(10):
+        for st in streams:
+            with torch.cuda.stream(st):
+                results.append(step())
+    torch.cuda.synchronize()
+    assert all(torch.equal(u, v) for r in results for u, v in zip(r, want))
