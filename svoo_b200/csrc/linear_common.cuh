@@ -19,7 +19,7 @@ struct LinearArgs {
   int64_t out_scale_pitch;
   int M, N, K;
   int* status;                                  // the device's word: != 0 after a kernel gave up on a bounded wait
-  bool box_out;                                 // rows of out are whole 16-byte pieces: they leave by TMA
+  bool box_out;                                 // rows of out are whole 16-byte pieces, each on 16 bytes: they leave by TMA
 };
 
 // D[tmem] (+)= A[smem] B[smem]^T, e4m3

@@ -419,7 +419,9 @@ cudaError_t launch_linear(const void* a, int64_t a_pitch, const float* sa, int64
                              int64_t sb_n, int64_t sb_k, bool row_scales, const void* bias, int bias_type, int64_t M, int64_t N, int64_t K,
                              bool gelu, int out_type, void* out, int64_t out_pitch, float* out_scale, int64_t out_scale_pitch, cudaStream_t st) {
   const int e = out_type == SVOO_TYPE_E4M3 ? 1 : elem_bytes(out_type);
-  const bool box_out = out_pitch * e % 16 == 0 && (uintptr_t)out % 16 == 0;
+  // a box that reaches behind a row is cut at 16 bytes, not at the row's last number: a row that ends inside 16 bytes of a wider
+  // pitch leaves element by element (e4m3 rows end at 16 bytes by their contract)
+  const bool box_out = out_pitch * e % 16 == 0 && (uintptr_t)out % 16 == 0 && (e == 1 || N * e % 16 == 0);
   const LinearCall c{a, b, a_pitch, b_pitch,
                      {sa, sb, sa_pitch, sb_n, sb_k, bias, bias_type, out, out_pitch, out_scale, out_scale_pitch, (int)M, (int)N, (int)K, rows_status_word(), box_out}, st};
   if (!c.args.status) return cudaErrorInvalidDevice;
