@@ -186,3 +186,28 @@ def test_walking_products_on_two_streams_and_in_a_graph():
                 results.append(step())
     torch.cuda.synchronize()
     assert all(torch.equal(u, v) for r in results for u, v in zip(r, want))
+
+
+@pytest.mark.parametrize("M,N", [(5, 300), (40, 300), (9600, 300)])
+@pytest.mark.parametrize("K", [1, 130, 200, 250])
+def test_operands_that_are_slices(M, N, K):
+    """The leading columns of wider operands, whose bytes behind the row are not zeros, rows from the middle, and rows of blocks."""
+    from svoo_b200 import ops
+    x, w = rand(M + 8, 256, torch.float32, M), rand(N + 256, 256, torch.float32, N, 0.05)
+    a, b, t = ops.quantize_rows(x), ops.quantize_blocks(w), ops.quantize_rows(w)
+    kb = -(-K // 128)
+    ad = R.dequantize(x, 1, 128)[5:M + 5, :K]
+    a = ops.Fp8Rows(a.q[5:M + 5, :K], a.scale[:kb, 5:M + 5])
+    n = slice(128, 128 + N)
+    bd = R.dequantize(w, 128, 128)[n, :K]
+    y = ops.mm_fp8(a, ops.Fp8Blocks(b.q[n, :K], b.scale[1:1 + -(-N // 128), :kb]), None, None, torch.float32)
+    want = ad @ bd.t()
+    assert ((y.double() - want).abs() <= R.product_bound(ad, bd, torch.float32, want)).all()
+    y = ops.linear_fp8(x[5:M + 5, :K], ops.Fp8Blocks(b.q[n, :K], b.scale[1:1 + -(-N // 128), :kb]))
+    u = R.dequantize(x[5:M + 5, :K], 1, 128)
+    want = u @ bd.t()
+    assert ((y.double() - want).abs() <= R.product_bound(u, bd, torch.float32, want)).all()
+    bd = R.dequantize(w, 1, 128)[n, :K]
+    y = ops.mm_fp8(a, ops.Fp8Rows(t.q[n, :K], t.scale[:kb, n]), None, None, torch.float32)
+    want = ad @ bd.t()
+    assert ((y.double() - want).abs() <= R.product_bound(ad, bd, torch.float32, want)).all()

@@ -80,3 +80,25 @@ def test_far_means_cost_the_gradient_no_digits(dtype, B, C, centre):
     # sums of at most 46 additions a thread and tree and 14 other roundings, each of its term's magnitude
     size = w.abs() + w.abs().mean(-1, keepdim=True) + xhat.abs() * (w * xhat).abs().mean(-1, keepdim=True)
     assert ((dx.double() - want).abs() <= r * 60 * 2.0 ** -24 * size + R.half_step(dtype) * want.abs() + torch.finfo(dtype).tiny).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_that_overlap_or_are_one(dtype):
+    """One row seen as many, windows that overlap, samples that overlap."""
+    from svoo_b200 import ops
+    flat = torch.randn(6000, device=DEV).to(dtype)
+    for x in (flat[:64].expand(50, 64), flat[:1000].view(1, 1000).expand(3, 7, 1000), flat.as_strided((90, 64), (3, 1)), flat.as_strided((2, 30, 129), (40, 100, 1)),
+              flat.as_strided((3, 20, 200), (8, 16, 1), 8), flat[3:67].expand(1, 1, 64)):
+        C = x.shape[-1]
+        g, o = torch.randn(C, device=DEV), torch.randn(C, device=DEV)
+        y, mean, rstd = ops.layer_norm(x, g, o, return_stats=True)
+        want, _, m, r = R.layer_norm(x, g, o, 1e-6)
+        # the mean is off by 80 x 2^-24 of the largest magnitude at most, everything else by less
+        tol = (80 * 2.0 ** -24 * 8 * r * (1 + r)) * g.abs().double() + 2.0 ** -20 * (want.abs() + o.abs()) + R.half_step(dtype) * want.abs()
+        assert x.abs().max() < 7.9 and ((y.double() - want).abs() <= tol).all()
+        got = ops.layer_norm_backward(y, x, mean, rstd, g)
+        ref = R.layer_norm_grad(x, y, g, 1e-6)[0]
+        assert (got[0].double() - ref).norm() <= 1.01 * R.half_step(dtype) * ref.norm() + 1e-5 * (r * g.abs().max() * y.double().abs()).norm()
+        if x.dim() == 2:
+            assert torch.equal(ops.quantize_rows(x).q.view(torch.uint8), ops.quantize_rows(x.contiguous()).q.view(torch.uint8))
+            assert torch.equal(ops.quantize_columns(x).q.view(torch.uint8), ops.quantize_columns(x.contiguous()).q.view(torch.uint8))
