@@ -387,7 +387,9 @@ int svoo_b200_peer_barrier(void* const* peer_flags, int32_t world, int32_t rank,
 /* ------------------------------------------------------------------------------------------
  * Token-wise operators: the layer norms and linear layers of a transformer block.  Sizes may be odd and
  * tensors of zero rows are accepted (nothing is launched, or sums are zero).  Strides and pitches are in
- * elements.  No counterpart in the reference except where named.
+ * elements.  At most 2^26 rows and columns; what lies behind a row inside a wider pitch is left alone.  These entry points came
+ * after version 105 without a new number: who loads the library at run time asks for the symbol.  No counterpart in
+ * the reference except where named.
  * ------------------------------------------------------------------------------------------ */
 
 #define SVOO_MAX_NORM_COLUMNS 16384
@@ -421,7 +423,8 @@ int svoo_b200_layer_norm_backward(const void* dy, int64_t dy_batch, int64_t dy_r
  *            fp32 [ceil(M / 128), K] sums of each 128 rows, which svoo_b200_column_sum adds
  *   both:    rows (q, scale) and columns (qt, scale_t, column_sums) from one reading of x
  *   blocks:  squares of 128 x 128.  q [M, q_pitch], scale [ceil(M / 128), ceil(K / 128)]; qt, if given, is the transpose of q,
- *            [K, qt_pitch >= M] */
+ *            [K, qt_pitch >= M]
+ * columns, both and blocks take at most 65,535 blocks of 128 rows. */
 int svoo_b200_quantize_rows(const void* x, int32_t x_type, int64_t M, int64_t K, int64_t x_row, void* q, int64_t q_pitch, float* scale,
                             int64_t scale_pitch, void* stream);
 int svoo_b200_quantize_columns(const void* x, int32_t x_type, int64_t M, int64_t K, int64_t x_row, void* q, int64_t q_pitch,
@@ -438,8 +441,8 @@ int svoo_b200_column_sum(const float* partial, int64_t parts, int64_t C, void* o
  * a [M, K], a_scale as of quantize_rows.  b [N, K] with b_scale[(n / 128) * b_scale_n + (k / 128) * b_scale_k] (as of
  * quantize_blocks; swap the two for its transpose), or, with b_scale_rows != 0, b_scale[(k / 128) * b_scale_k + n] (as of
  * quantize_rows or quantize_columns; b_scale 16-byte aligned, b_scale_k a multiple of 4; no bias, activation or e4m3 output).
- * out [M, N] of out_type, rows out_pitch apart; SVOO_TYPE_E4M3: the 32-bit results quantised in blocks along N, out_pitch a
- * multiple of 16, out_scale[nb * out_scale_pitch + m].  a and b 16-byte aligned, their pitches multiples of 16. */
+ * out [M, N] of out_type, rows out_pitch apart; SVOO_TYPE_E4M3: the 32-bit results quantised in blocks along N (quotients to within
+ * 2^-23 of themselves, so that one next to a tie may go either way), out_pitch a multiple of 16, out_scale[nb * out_scale_pitch + m].  a and b 16-byte aligned, their pitches multiples of 16. */
 int svoo_b200_mm_fp8(const void* a, int64_t a_pitch, const float* a_scale, int64_t a_scale_pitch, const void* b, int64_t b_pitch,
                      const float* b_scale, int64_t b_scale_n, int64_t b_scale_k, int32_t b_scale_rows, const void* bias,
                      int32_t bias_type, int64_t M, int64_t N, int64_t K, int32_t activation, void* out, int32_t out_type,

@@ -151,8 +151,8 @@ static cudaError_t launch_few_nt(const void* x, int64_t x_row, const LinearCall&
                     (const uint8_t*)c.b, c.b_pitch, c.args, out_type, gelu);
 }
 // Columns per CTA so that all of them run at once: an SM holds one CTA of sixteen warps or two of eight.  One row, 16 rows of 5,120 x
-// 5,120, us: 40 columns by sixteen warps (128 CTAs) 8.7, 12.7; 32 by sixteen (160, two rounds) 14.1, 19.5; 32 by eight 12.1, 18.9.  With 16
-// rows and 40 columns a few of the 128 registers spill (112 bytes a thread).
+// 5,120, us: 40 columns by sixteen warps (128 CTAs) 8.7, 12.7; 32 by sixteen (160, two rounds) 14.1, 19.5; 32 by eight 12.1, 18.9.  With 9 to 16
+// rows a few of the 128 registers spill: 64 to 120 bytes a thread by type with 40 columns, 56 with 32 columns and 16-bit rows that are not aligned.
 template <typename T, bool kWide, int MT>
 static cudaError_t launch_few_mt(const void* x, int64_t x_row, const LinearCall& c, int out_type, bool gelu) {
   if (c.args.N <= 148 * 16) return launch_few_nt<T, kWide, MT, 2, 16>(x, x_row, c, out_type, gelu);

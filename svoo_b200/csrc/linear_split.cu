@@ -1,8 +1,9 @@
 // The product of linear_tc.cu where it has few tiles: the blocks of k of one 128 x 128 tile are shared out among the CTAs of a
 // cluster, which join their sums through distributed shared memory.
 //
-// With few rows the product reads its weights once and does little else; what bounds it is how many SMs ask for them and
-// how much each has in flight.  A 128 x 128 tile has N / 128 of them to offer (5,120 columns: 40), a cluster of up to eight
+// With few rows the product reads its weights once and does little else; what bounds it is how many SMs work on it: a block of k takes
+// a CTA 0.45 us (300 x 300 x 8,000 on one CTA a tile 28.7), some 800 cycles, most of them the latency of four 16-column loads from TMEM, one
+// behind the other, and of the hand-over of the accumulator; the tensor pipe needs 128.  A 128 x 128 tile has N / 128 of them to offer (5,120 columns: 40), a cluster of up to eight
 // CTAs per tile up to eight times as many.  Every CTA sums its blocks of k as linear_tc.cu does, leaves the sums in its
 // shared memory, and takes a share of the tile's rows, a warp per row: the cluster's sums of that row are added in rank order
 // (the same bits on every call), then bias, activation and the store or the quantisation of the row's 128 columns, which are

@@ -25,7 +25,8 @@ constexpr int kBackwardStages = 2;                 // the row is read twice; thr
 // last 16 (their neighbours', inside the tensor), and the threads of a group take neighbouring elements, one access each.  (16-byte
 // pieces read at the row's shift, written back through shared memory: us against this, forward and backward, 32 bits 2 x 4,097 x 1,001
 // 17.8 / 13.0 and 32.7 / 26.3, 4,097 x 5,121 64.9 / 40.3 and 104.8 / 54.5; bf16 16.0 / 12.8 and 25.8 / 26.3, 8,194 x 5,121 71.5 / 79.4 and
-// 98.4 / 90.9, 32,760 x 1,537 68.8 / 76.1 and 151.8 / 140.1.)
+// 98.4 / 90.9, 32,760 x 1,537 68.8 / 76.1 and 151.8 / 140.1: long 16-bit rows forward are 10 % slower for it, the rest is faster, and one form
+// serves all.)
 struct RingLayout {
   int columns, row, ring, bars, total;            // columns rounded up to whole pieces, bytes of a row's place; offsets
   __host__ __device__ RingLayout(int C, int e, int param_rows, int row_tensors, int groups, int stages, bool aligned) {

@@ -769,7 +769,7 @@ def quantize_rows(x: torch.Tensor) -> Fp8Rows:
 
 def quantize_columns(x: torch.Tensor, column_sum_type: Optional[torch.dtype] = None):
     """The transpose of x [M, K] quantised along M: Fp8Rows of shape [K, M].  With column_sum_type also the sums of x's columns,
-    [K] of that type, added in 32 bits in a fixed order: (rows, sums).  M >= 1."""
+    [K] of that type, added in 32 bits in a fixed order: (rows, sums).  1 <= M <= 65,535 x 128."""
     M, K, stride = _matrix(x, "x")
     if M < 1:
         raise ValueError("quantize_columns needs at least one row")
@@ -865,9 +865,10 @@ def _product_output(like: torch.Tensor, M: int, N: int, bias, activation, out_dt
 
 def mm_fp8(a: Fp8Rows, b, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
            out_dtype: torch.dtype = torch.bfloat16):
-    """act(a b^T + bias), sums in 32 bits: a Fp8Rows [M, K]; b Fp8Blocks [N, K], or Fp8Rows [N, K] (then neither of the next two); bias
-    [N], bf16, fp16 or fp32; activation None or "gelu" (its tanh formula).  out_dtype bf16, fp16, fp32, or float8_e4m3fn for
-    the 32-bit results quantised in 1 x 128 blocks, an Fp8Rows, ready to be the next product's a."""
+    """act(a b^T + bias), sums in 32 bits: a Fp8Rows [M, K]; b Fp8Blocks [N, K], or Fp8Rows [N, K], its scales on 16 bytes and their
+    rows a multiple of four apart, as quantize_columns leaves them (then neither of the next two); bias [N], bf16, fp16 or fp32;
+    activation None or "gelu" (its tanh formula).  out_dtype bf16, fp16, fp32, or float8_e4m3fn for the 32-bit results quantised in
+    1 x 128 blocks, an Fp8Rows, ready to be the next product's a."""
     M, K = a.q.shape
     N = b.q.shape[0]
     KB = (K + 127) // 128
