@@ -192,13 +192,13 @@ class WanDiT(nn.Module):
         return self
 
     def check_status(self) -> None:
-        """Raises if a kernel of the forward calls so far gave up on a bounded wait: of the processors' last sparse calls, or, with
-        use_token_kernels, of any norm or linear layer on the model's GPU.  Synchronises: once per step or run."""
+        """Raises if a kernel of the forward calls so far gave up on a bounded wait: of the processors' last sparse calls, or, where
+        a block has norms or linear layers on this package's kernels, of any such on the model's GPU.  Synchronises: once per step or run."""
         for block in self.blocks:
             for attn in (block.attn1, block.attn2):
                 if attn.processor is not None:
                     attn.processor.check_status()
-        if any(block.fused_norms or isinstance(block.ffn, fp8.Fp8FeedForward) for block in self.blocks):
+        if any(block.fused_norms or any(isinstance(m, fp8.Fp8Linear) for m in block.modules()) for block in self.blocks):
             fp8.check_status(self.proj_out.weight.device)
 
     def _timestep_embedding(self, timestep):

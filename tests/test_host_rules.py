@@ -193,7 +193,7 @@ def test_a_model_reports_token_kernels_that_gave_up(monkeypatch):
     """check_status asks every processor, and the token-wise kernels of the model's device once blocks are on them; it raises."""
     import pytest
     import torch
-    from svoo_b200 import ops, wan_dit
+    from svoo_b200 import linear, ops, wan_dit
     cfg = wan_dit.WanDiTConfig(num_layers=2, dim=128, heads=1, ffn_dim=128, text_dim=16, text_len=4, latent=(1, 4, 4))
     model = wan_dit.WanDiT(cfg)
     asked, word = [], [0]
@@ -214,6 +214,11 @@ def test_a_model_reports_token_kernels_that_gave_up(monkeypatch):
     model.check_status()
     assert asked == ["processor"] * 2 + [torch.device("cpu")]
     word[0] = 1
+    with pytest.raises(RuntimeError, match="incomplete"):
+        model.check_status()
+    model.blocks[1].fused_norms = False
+    model.check_status()
+    model.blocks[0].attn2.to_k = linear.Fp8Linear(128, 128)   # one layer, put there by hand
     with pytest.raises(RuntimeError, match="incomplete"):
         model.check_status()
 
